@@ -50,6 +50,8 @@ extern "C" {
  * output.weight as a dequantized f32 table, as streaming-loader.js:324-335
  * does): 256-value blocks of 210 bytes, gguf.js:317-355. */
 #define PB_TYPE_Q6_K 14
+/* rows of the packed operators only (pb_kv8_*, pb_attn_packed) */
+#define PB_TYPE_BF16 30
 /* OR'ed into the type of pb_qmat_upload / pb_qmat_from_device: store the
  * matrix as a table read one row per lane (the layout pb_qmat_head needs)
  * instead of the matvec layout. */
@@ -477,6 +479,99 @@ int pb_batch_decode(pb_batch* b, int steps, int* tokens_host, float* logits_host
  * scale from the one-sequence path at the Llama-3.2-1B shape).  Set between
  * steps.  No counterpart in the reference, which serves one sequence. */
 int pb_batch_set_precision(pb_batch* b, int terms);
+
+/* ------------------------------------------------------------------ */
+/* a paged 8-bit KV cache and attention over packed sequences             */
+/* ------------------------------------------------------------------ */
+
+/* No counterpart in the reference, whose cache is one f32 array per layer
+ * (llama-streaming.js:395-420).  Here a pool of pages (one pool per layer, in
+ * device memory of the caller's, pb_kv8_pool_bytes) is shared by sequences of
+ * any lengths: page table_dev[s * ld_table + i] holds tokens i * page_size ..
+ * of sequence s.  Keys and values are 8-bit codes with a power-of-two scale
+ * for each PB_KV8_BLOCK tokens and head: a quarter of the f32 cache's bytes.
+ *
+ * Packed rows: the calls take the tokens of all sequences as rows of one
+ * array, rows starts_dev[s] .. starts_dev[s + 1] - 1 those of sequence s
+ * (starts_dev has n_seqs + 1 entries and rises; n_rows bounds the last).  A
+ * sequence may have no rows; rows behind the last sequence's are neither read
+ * nor written.  starts, lengths and tables live on the device, so a recorded
+ * graph (pb_capture_begin) follows them from replay to replay.  Row strides
+ * (ld*) count elements; row arrays are 16-byte aligned with strides of a
+ * multiple of 16 bytes.  Types: PB_TYPE_F32, PB_TYPE_F16, PB_TYPE_BF16.
+ *
+ * A table entry or a length that does not fit the pool raises the device
+ * error word (index out of bounds): what it covers is not read or written. */
+#define PB_KV8_INT8 0 /* codes -127 .. 127 */
+#define PB_KV8_E4M3 1 /* 8-bit floats, 448 the largest */
+#define PB_KV8_BLOCK 16
+#define PB_ROPE_NONE 0
+#define PB_ROPE_INTERLEAVED 1 /* pairs (2i, 2i + 1), as llama-streaming.js:310-339 */
+#define PB_ROPE_HALF 2        /* pairs (i, i + rope_dim / 2) */
+typedef struct pb_kv8 pb_kv8;
+typedef struct pb_kv8_config {
+  int code;       /* PB_KV8_* */
+  int n_kv_heads; /* up to 1024 */
+  int head_dim;   /* a multiple of 32, up to 256 */
+  int page_size;  /* tokens: 16, 32, 64 or 128 */
+  int n_pages;    /* of a pool */
+  int rope;       /* PB_ROPE_*: the rotation pb_kv8_append applies to q and k */
+  int rope_dim;   /* the first rope_dim values of a head are rotated (even) */
+  int original_max_pos;
+  double rope_theta; /* the pair frequencies are pb_rope_freqs(rope_theta, rope_dim, rope_factor, ...) */
+  double rope_factor, low_freq_factor, high_freq_factor;
+} pb_kv8_config;
+/* Bytes of one layer's pool, -1 for a bad configuration.  Host only.  A pool's
+ * bytes need no initialisation: a block is written whole before it is read. */
+int64_t pb_kv8_pool_bytes(const pb_kv8_config* c);
+/* The handle: geometry, frequencies and a workspace; it serves any number of
+ * pools.  Its calls run on ctx's stream; free it before the context. */
+int pb_kv8_create(pb_ctx* ctx, const pb_kv8_config* c, pb_kv8** out);
+int pb_kv8_free(pb_kv8* kv);
+/* Append: rows k_dev, v_dev [n_kv_heads * head_dim] of sequence s become its
+ * tokens past_dev[s], past_dev[s] + 1, ...  k is rotated by the token's
+ * position (in double, then rounded to f32), both are coded, and the scale of
+ * a block that already holds tokens grows where the new ones need it (its
+ * older codes are rounded once more under the larger scale).  A value that is
+ * not finite, or above 2^66 in magnitude, makes its block and head read as NaN
+ * until the block is begun anew.  Appending again at an earlier past_dev[s]
+ * rolls the sequence back; a block then begun in its middle keeps its scale.
+ * q_dev [n_heads * head_dim] (optional, with q_out_dev) is rotated into
+ * q_out_dev; k_out_dev, v_out_dev (optional) get the rotated k and v without
+ * the coding, for pb_attn_packed.  Outputs are of type otype and may not
+ * overlap the inputs.  A page that two sequences share is read by both, but
+ * appended to by none. */
+int pb_kv8_append(pb_kv8* kv, void* pages_dev, int type, const void* q_dev, int ldq, const void* k_dev, int ldk,
+                  const void* v_dev, int ldv, int n_heads, const int* starts_dev, const int* past_dev,
+                  const int* table_dev, int ld_table, int n_seqs, int n_rows, int otype, void* q_out_dev, int ldqo,
+                  void* k_out_dev, int ldko, void* v_out_dev, int ldvo);
+/* The values the cache holds: row starts_dev[s] + i of k_out_dev, v_out_dev
+ * (either may be NULL) gets token first_dev[s] + i of sequence s, rounded to
+ * otype (f16 and bf16 hold every code times its scale exactly while it is in
+ * their range).  As pb_model_kv for the f32 cache; also the prefix that
+ * pb_attn_packed attends to when a prompt comes in pieces. */
+int pb_kv8_read(pb_kv8* kv, const void* pages_dev, const int* starts_dev, const int* first_dev, const int* table_dev,
+                int ld_table, int n_seqs, int n_rows, int otype, void* k_out_dev, int ldk, void* v_out_dev, int ldv);
+/* Attention of the newest tokens over the cache (decode, drafted tokens): the
+ * rows of sequence s, rotated already, are its last tokens, lens_dev[s] tokens
+ * being cached with them; each sees the tokens up to its own, kv head h /
+ * (n_heads / n_kv_heads) for head h.  out = sum_j softmax_j(scale q.k_j) v_j
+ * with f32 sums; a row that sees no token (lens_dev[s] less than its rows)
+ * gets zeros.  q_dev and out_dev [n_rows][n_heads * head_dim] are of one type. */
+int pb_kv8_attn(pb_kv8* kv, const void* pages_dev, int type, const void* q_dev, int ldq, int n_heads,
+                const int* starts_dev, const int* lens_dev, const int* table_dev, int ld_table, int n_seqs, int n_rows,
+                double scale, void* out_dev, int ldo);
+/* Attention of whole prompts, packed: rows q_starts_dev[s] .. of q_dev
+ * [q_rows][n_heads * head_dim] attend to rows k_starts_dev[s] .. of k_dev and
+ * v_dev [k_rows][n_kv * head_dim] (llama-streaming.js:422-464 for one sequence
+ * in f32; pb_attn_cached).  causal = 1: the queries are the sequence's last
+ * tokens, query i of nq sees keys up to nk - nq + i; 0: all of them.  A query
+ * that sees no key gets zeros.  f16 or bf16 rows and output, f32 scores and
+ * sums, the probabilities rounded to the rows' type; head_dim a multiple of 8,
+ * up to 128.  q_starts_dev and k_starts_dev may be one array. */
+int pb_attn_packed(pb_ctx* ctx, int type, const void* q_dev, int ldq, const void* k_dev, int ldk, const void* v_dev,
+                   int ldv, const int* q_starts_dev, const int* k_starts_dev, int n_seqs, int q_rows, int k_rows,
+                   int n_heads, int n_kv, int head_dim, double scale, int causal, void* out_dev, int ldo);
 
 /* ------------------------------------------------------------------ */
 /* row split over GPUs (thread-pool.js:165-246 splits a matvec's output   */

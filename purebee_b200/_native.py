@@ -16,6 +16,11 @@ LIB_PATH = os.path.join(HERE, "libpurebee_b200.so")
 
 PB_OK, PB_ERR_ARG, PB_ERR_OOM, PB_ERR_CUDA, PB_ERR_TIMEOUT, PB_ERR_DEVICE, PB_ERR_STATE, PB_ERR_NOTFOUND = range(8)
 TYPE_F32, TYPE_F16, TYPE_Q4_0, TYPE_Q4_1, TYPE_Q8_0 = 0, 1, 2, 3, 8
+TYPE_BF16 = 30  # rows of the packed operators (pb_kv8_*, pb_attn_packed)
+TYPES = {"f32": TYPE_F32, "f16": TYPE_F16, "bf16": TYPE_BF16}
+KV8_INT8, KV8_E4M3 = 0, 1
+KV8_BLOCK = 16
+ROPE_NONE, ROPE_INTERLEAVED, ROPE_HALF = 0, 1, 2
 QMAT_TABLE = 0x100  # OR into the type: LM-head table layout (pb_qmat_head)
 MODEL_STREAMING_Q4, MODEL_LLAMA_Q8A = 0, 1
 MATVEC_FAST, MATVEC_EXACT = 0, 1  # pb_set_matvec_mode
@@ -37,6 +42,13 @@ class ModelConfig(ctypes.Structure):
                 ("hidden_dim", ctypes.c_int), ("n_layers", ctypes.c_int), ("n_heads", ctypes.c_int),
                 ("n_kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("vocab", ctypes.c_int),
                 ("seq_len", ctypes.c_int), ("rope_theta", ctypes.c_double), ("eps", ctypes.c_double)]
+
+
+class KV8Config(ctypes.Structure):
+    """pb_kv8_config: the geometry of a paged 8-bit KV cache and its rotary positions."""
+    _fields_ = [(n, ctypes.c_int) for n in ("code", "n_kv_heads", "head_dim", "page_size", "n_pages", "rope", "rope_dim",
+                                           "original_max_pos")] + \
+               [(n, ctypes.c_double) for n in ("rope_theta", "rope_factor", "low_freq_factor", "high_freq_factor")]
 
 
 class SplitPlan(ctypes.Structure):
@@ -177,6 +189,13 @@ SIGNATURES = {
     "pb_batch_split_plan": (I, [ctypes.POINTER(ModelConfig), I, I, ctypes.POINTER(SplitPlan)]),
     "pb_batch_create_split": (I, [V, I, V, ctypes.POINTER(V)]),
     "pb_batch_create_group": (I, [V, I, I, ctypes.POINTER(V)]),
+    "pb_kv8_pool_bytes": (I64, [ctypes.POINTER(KV8Config)]),
+    "pb_kv8_create": (I, [V, ctypes.POINTER(KV8Config), ctypes.POINTER(V)]),
+    "pb_kv8_free": (I, [V]),
+    "pb_kv8_append": (I, [V, V, I, V, I, V, I, V, I, I, V, V, V, I, I, I, I, V, I, V, I, V, I]),
+    "pb_kv8_read": (I, [V, V, V, V, V, I, I, I, I, V, I, V, I]),
+    "pb_kv8_attn": (I, [V, V, I, V, I, I, V, V, V, I, I, I, D, V, I]),
+    "pb_attn_packed": (I, [V, I, V, I, V, I, V, I, V, V, I, I, I, I, I, I, D, I, V, I]),
     "pb_comm_id": (I, [V]),
     "pb_comm_init": (I, [V, I, I, V, ctypes.POINTER(V)]),
     "pb_comm_free": (I, [V]),
@@ -325,6 +344,12 @@ class Context:
         self._check(rc)
         return Graph(self, g.value)
 
+    def attn_packed(self, type_, q, ldq, k, ldk, v, ldv, q_starts, k_starts, n_seqs, q_rows, k_rows, n_heads, n_kv,
+                    head_dim, scale, causal, out, ldo) -> None:
+        """Attention of whole packed prompts (pb_attn_packed); arrays are device addresses."""
+        self._check(lib().pb_attn_packed(self.h, type_, q, ldq, k, ldk, v, ldv, q_starts, k_starts, n_seqs, q_rows,
+                                         k_rows, n_heads, n_kv, head_dim, scale, causal, out, ldo))
+
     def device_error(self) -> int:
         c = I()
         self._check(lib().pb_device_error(self.h, ctypes.byref(c)))
@@ -351,6 +376,57 @@ class QMat:
     def free(self):
         if self.h and self.ctx.h:
             lib().pb_qmat_free(self.ctx.h, self.h)
+        self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class KV8:
+    """A paged 8-bit KV cache's geometry, rotation and workspace (pb_kv8); it serves any number of page pools.
+
+    Arrays are device addresses (a DeviceBuffer's ptr, a tensor's data_ptr()).
+    """
+
+    def __init__(self, ctx: Context, code: int, n_kv_heads: int, head_dim: int, page_size: int, n_pages: int,
+                 rope: int = ROPE_NONE, rope_dim: int = 0, theta: float = 10000.0, scaling=(0.0, 1.0, 4.0, 8192)):
+        """scaling: factor (0: off), low and high frequency factor, original context (pb_rope_freqs)."""
+        self.ctx = ctx
+        self.h = None
+        factor, low, high, orig = scaling
+        self.config = KV8Config(code, n_kv_heads, head_dim, page_size, n_pages, rope, rope_dim, int(orig), float(theta),
+                                float(factor), float(low), float(high))
+        h = V()
+        ctx._check(lib().pb_kv8_create(ctx.h, ctypes.byref(self.config), ctypes.byref(h)))
+        self.h = h.value
+
+    @property
+    def pool_bytes(self) -> int:
+        """Bytes of one layer's pool."""
+        return int(lib().pb_kv8_pool_bytes(ctypes.byref(self.config)))
+
+    def append(self, pages, type_, q, ldq, k, ldk, v, ldv, n_heads, starts, past, table, ld_table, n_seqs, n_rows, otype,
+               q_out, ldqo, k_out=None, ldko=0, v_out=None, ldvo=0) -> None:
+        """Rotate q and k, append k and v (pb_kv8_append)."""
+        self.ctx._check(lib().pb_kv8_append(self.h, pages, type_, q, ldq, k, ldk, v, ldv, n_heads, starts, past, table,
+                                            ld_table, n_seqs, n_rows, otype, q_out, ldqo, k_out, ldko, v_out, ldvo))
+
+    def read(self, pages, starts, first, table, ld_table, n_seqs, n_rows, otype, k_out, ldk, v_out, ldv) -> None:
+        """Rows of the cache as values (pb_kv8_read)."""
+        self.ctx._check(lib().pb_kv8_read(self.h, pages, starts, first, table, ld_table, n_seqs, n_rows, otype, k_out,
+                                          ldk, v_out, ldv))
+
+    def attn(self, pages, type_, q, ldq, n_heads, starts, lens, table, ld_table, n_seqs, n_rows, scale, out, ldo) -> None:
+        """Attention of the newest tokens over the cache (pb_kv8_attn)."""
+        self.ctx._check(lib().pb_kv8_attn(self.h, pages, type_, q, ldq, n_heads, starts, lens, table, ld_table, n_seqs,
+                                          n_rows, scale, out, ldo))
+
+    def free(self):
+        if self.h and self.ctx.h:
+            lib().pb_kv8_free(self.h)
         self.h = None
 
     def __del__(self):

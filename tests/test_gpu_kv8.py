@@ -1,0 +1,384 @@
+"""The paged 8-bit KV cache on the device (pb_kv8_append, pb_kv8_read, pb_kv8_attn) against 64-bit restatements."""
+import ctypes
+
+import numpy as np
+import packed_ref as R
+import pytest
+
+pytestmark = pytest.mark.gpu
+THETA = 500000.0
+
+
+class Pool:
+    """A handle, one pool and its sequences' page table, beside the restated caches."""
+
+    def __init__(self, native, ctx, code, nkv, hd, page, n_seqs, max_tokens, rope=0, rope_dim=0, scaling=(0.0, 1.0, 4.0, 8192),
+                 seed=0, n_pages=None, spread=1):
+        self.N, self.ctx, self.nkv, self.hd, self.page, self.n_seqs = native, ctx, nkv, hd, page, n_seqs
+        self.rng = np.random.default_rng(seed)
+        self.ld = -(-max_tokens // page) + 1
+        used = self.ld * n_seqs
+        self.n_pages = n_pages or used * spread + 2
+        self.kv = native.KV8(ctx, code, nkv, hd, page, self.n_pages, rope, rope_dim, THETA, scaling)
+        self.pages = ctx.alloc(self.kv.pool_bytes)
+        table = self.rng.permutation(self.n_pages)[:used] if n_pages is None else np.arange(self.n_pages - used, self.n_pages)
+        self.table = ctx.to_device(table.astype(np.int32).reshape(n_seqs, self.ld))
+        self.rope, self.rope_dim, self.scaling = rope, rope_dim, scaling
+        self.ref = [R.Cache(code, nkv, hd) for _ in range(n_seqs)]
+
+    def ints(self, v):
+        return self.ctx.to_device(np.asarray(v, np.int32))
+
+    def append(self, counts, past, nh, t="f32", ot="f32", amp=1.0, edit=None, extra=3, more=0):
+        """Random rows (k, v times amp) through the cache and its restatement; (q rotated, want)."""
+        N, c, hd, nkv = self.N, self.ctx, self.hd, self.nkv
+        n = sum(counts)
+        st = np.concatenate([[0], np.cumsum(counts)])
+        width = (nh + 2 * nkv) * hd + 8 * more
+        x = self.rng.standard_normal((n + extra, width)) * amp
+        x[:, :nh * hd] /= amp
+        if edit:
+            edit(x[:, nh * hd:(nh + 2 * nkv) * hd].reshape(n + extra, 2, nkv, hd))
+        bits = R.to_bits(x, t)
+        x = R.from_bits(bits, t)
+        size = bits.itemsize
+        dx = c.to_device(bits)
+        oq = c.to_device(np.full((n + extra, nh * hd), 7, R.np_dtype(ot)))
+        ok = c.to_device(np.full((n + extra, nkv * hd), 7, R.np_dtype(ot)))
+        ov = c.to_device(np.full((n + extra, nkv * hd), 7, R.np_dtype(ot)))
+        ds, dp = self.ints(st), self.ints(past)
+        self.kv.append(self.pages.ptr, N.TYPES[t], dx.ptr, width, dx.ptr + nh * hd * size, width,
+                       dx.ptr + (nh + nkv) * hd * size, width, nh, ds.ptr, dp.ptr, self.table.ptr, self.ld, self.n_seqs,
+                       n + extra, N.TYPES[ot], oq.ptr, nh * hd, ok.ptr, nkv * hd, ov.ptr, nkv * hd)
+        got = [R.from_bits(b.download(R.np_dtype(ot)).reshape(n + extra, -1, hd), ot) for b in (oq, ok, ov)]
+        want = [np.zeros((n, h, hd)) for h in (nh, nkv, nkv)]
+        fr = R.freqs(THETA, self.rope_dim, self.scaling)
+        for s in range(self.n_seqs):
+            r = slice(st[s], st[s + 1])
+            pos = past[s] + np.arange(counts[s])
+            with np.errstate(invalid="ignore"):
+                qk = R.rotate(x[r, :(nh + nkv) * hd].reshape(-1, nh + nkv, hd), pos, fr, self.rope, self.rope_dim)
+            v = x[r, (nh + nkv) * hd:(nh + 2 * nkv) * hd].reshape(-1, nkv, hd)
+            want[0][r], want[1][r], want[2][r] = qk[:, :nh], qk[:, nh:], v
+            self.ref[s].append(int(past[s]), qk[:, nh:], v)
+        tail = R.from_bits(np.full(1, 7, R.np_dtype(ot)), ot)[0]
+        for g in got:  # rows behind the last sequence stay
+            assert np.all(g[n:] == tail)
+        return [g[:n] for g in got], want
+
+    def read(self, first, counts, t="f32", k=True, v=True, extra=2):
+        c, w = self.ctx, self.nkv * self.hd
+        n = sum(counts)
+        st = self.ints(np.concatenate([[0], np.cumsum(counts)]))
+        fi = self.ints(first)
+        o = [c.to_device(np.full((n + extra, w), 5, R.np_dtype(t))) for _ in range(2)]
+        self.kv.read(self.pages.ptr, st.ptr, fi.ptr, self.table.ptr, self.ld, self.n_seqs, n + extra, self.N.TYPES[t],
+                     o[0].ptr if k else None, w, o[1].ptr if v else None, w)
+        got = [R.from_bits(b.download(R.np_dtype(t)).reshape(n + extra, self.nkv, self.hd), t) for b in o]
+        tail = R.from_bits(np.full(1, 5, R.np_dtype(t)), t)[0]
+        for g, on in zip(got, (k, v)):
+            assert np.all(g[n if on else 0:] == tail)
+        return got[0][:n], got[1][:n]
+
+    def want(self, i, first, counts):
+        return np.concatenate([r.values(i, f + n)[f:] if n else np.zeros((0, self.nkv, self.hd))
+                               for r, f, n in zip(self.ref, first, counts)])
+
+    def check(self):
+        """The whole cache, value for value."""
+        counts = [r.n for r in self.ref]
+        got = self.read([0] * self.n_seqs, counts)
+        for i in (0, 1):
+            np.testing.assert_array_equal(got[i], self.want(i, [0] * self.n_seqs, counts))
+
+    def attn(self, q, counts, lens, t, scale, extra=2):
+        N, c = self.N, self.ctx
+        n, nh, hd = q.shape
+        bits = R.to_bits(np.concatenate([q, np.ones((extra, nh, hd))]), t)
+        dq, st, le = c.to_device(bits), self.ints(np.concatenate([[0], np.cumsum(counts)])), self.ints(lens)
+        o = c.to_device(np.full((n + extra, nh, hd), 3, R.np_dtype(t)))
+        self.kv.attn(self.pages.ptr, N.TYPES[t], dq.ptr, nh * hd, nh, st.ptr, le.ptr, self.table.ptr, self.ld, self.n_seqs,
+                     n + extra, scale, o.ptr, nh * hd)
+        raw = o.download(R.np_dtype(t)).reshape(n + extra, nh, hd)
+        assert np.all(raw[n:] == R.np_dtype(t)(3))
+        return R.from_bits(raw[:n], t), R.from_bits(bits[:n], t)
+
+    def check_attn(self, nh, counts, lens, t, scale=None, amp=1.0, q=None):
+        scale = self.hd ** -0.5 if scale is None else scale
+        q = self.rng.standard_normal((sum(counts), nh, self.hd)) * amp if q is None else q
+        got, q = self.attn(q, counts, lens, t, scale)
+        at = 0
+        for s, (n, ln) in enumerate(zip(counts, lens)):
+            if n:
+                w, mag, dots = R.attention(q[at:at + n], self.ref[s].values(0, ln), self.ref[s].values(1, ln), scale)
+                # p is held in f16 and a second f16 for what that leaves (2^-22), or in one f16 (half a step, 2^-11)
+                # where a tile holds 16 rows of 16-bit queries
+                tol = R.attention_tolerance(w, mag, dots, self.hd, ln, t, 2.0 ** -22 if t == "f32" else 2.0 ** -11)
+                bad = R.differs(got[at:at + n], w, tol, t)
+                assert not bad.any(), (s, np.argwhere(bad)[:4], got[at:at + n][bad][:4], w[bad][:4], tol[bad][:4])
+            at += n
+        return got
+
+
+@pytest.mark.parametrize("code", [0, 1])
+@pytest.mark.parametrize("t,ot,hd,nkv,nh,page,rope,rope_dim,factor", [
+    ("f32", "f32", 64, 2, 6, 16, 1, 64, 0.0), ("f32", "f16", 128, 3, 3, 32, 2, 128, 32.0),
+    ("bf16", "bf16", 96, 2, 4, 64, 2, 32, 8.0), ("f16", "f32", 32, 5, 5, 128, 1, 20, 0.0),
+    ("f16", "f16", 256, 1, 2, 16, 2, 256, 0.0), ("bf16", "f16", 160, 2, 2, 32, 2, 36, 0.0),
+    ("f32", "bf16", 64, 9, 9, 64, 0, 0, 0.0)])
+def test_append_and_read(native, ctx, code, t, ot, hd, nkv, nh, page, rope, rope_dim, factor):
+    p = Pool(native, ctx, code, nkv, hd, page, 5, 200, rope, rope_dim, (factor, 1.0, 4.0, 64), seed=hd + code)
+    counts, past = [37, 0, 1, 90, 16], [0, 0, 0, 0, 0]
+    for step in range(5):
+        got, want = p.append(counts, past, nh, t, ot, amp=1.0 + step, more=step % 2)
+        for g, w in zip(got, want):
+            # f32 arithmetic on the rotated pair (2 products, 1 sum, cos and sin in f32: 5 roundings), then the output's
+            tol = 5 * 2.0 ** -24 * 2 * np.abs(w).max() + np.abs(w) * R.EPS[ot] / 2 + (2.0 ** -25 if ot == "f16" else 0)
+            assert np.all(np.abs(g - w) <= tol)
+        p.check()
+        past = [r.n for r in p.ref]
+        counts = [[1, 1, 1, 1, 1], [0, 5, 17, 1, 3], [1, 0, 0, 0, 31], [2, 2, 2, 2, 2], []][step]
+    # ranges from the middle, 16-bit values of the same codes, one output only
+    first, n = [3, 0, 16, 60, 15], [20, 2, 1, 33, 0]
+    for o in ("f32", "f16", "bf16"):
+        k, v = p.read(first, n, o)
+        np.testing.assert_array_equal(k, R.from_bits(R.to_bits(p.want(0, first, n), o), o))
+        np.testing.assert_array_equal(v, R.from_bits(R.to_bits(p.want(1, first, n), o), o))
+    p.read(first, n, k=False)
+    p.read(first, n, v=False)
+
+
+@pytest.mark.parametrize("code", [0, 1])
+def test_append_scales_grow(native, ctx, code):
+    """Tokens one by one whose size rises and falls by powers of two, zeros first, values at the codes' limits."""
+    p = Pool(native, ctx, code, 2, 64, 32, 1, 70, seed=3)
+    lim = R.LIMIT[code]
+    for i in range(40):
+        def edit(kv, i=i):
+            if i < 3:
+                kv[:] = 0
+            elif i % 7 == 0:
+                kv[:, 0, 0, 5] = lim * 2.0 ** (i % 5 - 2)  # the largest value just fits
+            elif i % 7 == 3:
+                kv[:, 1, 1, 9] = -np.nextafter(np.float32(lim * 2.0 ** (i % 4)), np.float32(1e9))  # just does not
+        p.append([1], [i], 2, amp=2.0 ** ((i * 5) % 11 - 5), edit=edit)
+        p.check()
+    for amp in (1e-30, 1e-12, 1e15):  # below 2^-40 * 127, near, large
+        p.append([16], [0], 2, amp=amp)
+        p.check()
+
+
+@pytest.mark.parametrize("code", [0, 1])
+def test_append_not_finite_and_rollback(native, ctx, code):
+    p = Pool(native, ctx, code, 2, 64, 16, 2, 100, seed=4)
+
+    def edit(kv):
+        kv[20, 0, 0, 3], kv[21, 1, 1, 0], kv[40, 0, 1, 7] = np.inf, np.nan, 2.0 ** 70
+
+    p.append([50, 3], [0, 0], 2, edit=edit)
+    p.check()
+    assert np.isnan(p.ref[0].values(0, 32)[16:32, 0]).all() and np.isfinite(p.ref[0].values(0, 32)[:, 1]).all()
+    p.append([2, 1], [34, 3], 2)  # back into the third block, which keeps its NaN in one head of K
+    p.check()
+    p.append([5, 1], [16, 4], 2)  # back to the second block's start: begun anew
+    p.check()
+    assert np.isfinite(p.ref[0].values(0, 21)).all()
+    p.check_attn(4, [1, 2], [21, 5], "f32")
+
+
+@pytest.mark.parametrize("code", [0, 1])
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd,nkv,nh,page", [(64, 2, 8, 64), (128, 2, 6, 16), (96, 3, 3, 32), (32, 1, 8, 16), (256, 1, 5, 128),
+                                            (128, 1, 16, 32), (64, 2, 22, 64), (192, 2, 4, 16), (224, 1, 1, 16)])
+def test_attention_ragged(native, ctx, code, t, hd, nkv, nh, page):
+    lens = [1, 16, 17, 0, 300, 63, 64, 65]
+    p = Pool(native, ctx, code, nkv, hd, page, len(lens), 310, seed=hd + nh)
+    p.append(lens, [0] * 8, nkv)
+    p.check_attn(nh, [1, 1, 1, 0, 1, 1, 1, 1], lens, t)
+    p.check_attn(nh, [1, 5, 3, 0, 7, 0, 2, 9], lens, t)  # drafted tokens
+
+
+def test_attention_rows_that_see_nothing(native, ctx):
+    lens = [2, 0, 40]
+    p = Pool(native, ctx, 0, 2, 64, 16, 3, 64, seed=8)
+    p.append(lens, [0] * 3, 2)
+    got = p.check_attn(8, [5, 3, 2], lens, "f32")
+    assert np.all(got[:3] == 0) and np.all(got[5:8] == 0) and np.all(got[3:5].any(-1))
+
+
+@pytest.mark.parametrize("code,t,n,nh", [(0, "f16", 5000, 8), (1, "bf16", 20011, 4), (0, "f32", 9999, 16)])
+def test_attention_long_split(native, ctx, code, t, n, nh):
+    """One long sequence beside short ones: many CTAs share a sequence and join their parts."""
+    lens = [n, 3, 700]
+    p = Pool(native, ctx, code, 2, 128, 64, 3, n, seed=n)
+    p.append(lens, [0] * 3, 2)
+    a = p.check_attn(nh, [1, 1, 1], lens, t)
+    st = p.rng.bit_generator.state
+    q = p.rng.standard_normal((6, nh, 128))
+    b = p.check_attn(nh, [3, 1, 2], lens, t, q=q)
+    p.rng.bit_generator.state = st
+    c = p.check_attn(nh, [3, 1, 2], lens, t, q=q)
+    assert np.array_equal(b, c) and np.isfinite(a).all()  # the same bits each time
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+def test_attention_uneven_scales(native, ctx, t):
+    """Blocks of V whose scales lie far apart, a peaked softmax on the small ones, large keys, scale 0 and negative."""
+    p = Pool(native, ctx, 0, 1, 64, 16, 1, 200, seed=12)
+
+    def edit(kv):
+        kv[:, 0] *= 4
+        kv[32:48, 1] *= 2.0 ** 20
+        kv[64:96, 1] *= 2.0 ** -18
+        kv[100, 0] = 0
+    p.append([190], [0], 1, edit=edit)
+    q = np.zeros((3, 4, 64))
+    k = p.ref[0].values(0, 190)[:, 0]
+    q[:, :2], q[:, 2], q[:, 3] = k[70], k[40], p.rng.standard_normal(64)
+    for scale in (0.125, 0.0, -0.3, 3.0):
+        p.check_attn(4, [3], [190], t, scale=scale, q=q)
+
+
+def test_attention_not_finite(native, ctx):
+    """A query with a NaN, blocks that read as NaN: what sees them is NaN, what does not is not touched."""
+    p = Pool(native, ctx, 1, 1, 64, 16, 3, 64, seed=13)
+
+    def edit(kv):
+        kv[33, 0, 0, 0], kv[64 + 40, 1, 0, 2] = np.nan, np.inf
+    p.append([40, 64, 20], [0, 0, 0], 1, edit=edit)
+    q = p.rng.standard_normal((24, 2, 64))
+    q[23, 1, 5] = np.nan
+    got = p.check_attn(2, [10, 11, 3], [40, 48, 20], "f32", q=q)
+    assert np.isfinite(got[:2]).all() and np.isnan(got[2:10]).all()  # tokens 30, 31 come before the block
+    assert np.isfinite(got[10:21]).all()  # nothing of the other sequences reaches the second
+    assert np.isnan(got[21:]).all()  # row 104 is the third's token 0, in the block every query sees
+
+
+def test_pool_past_32_bits(native, ctx):
+    """Pages whose bytes lie past 2^32."""
+    p = Pool(native, ctx, 0, 8, 128, 64, 2, 130, seed=14, n_pages=34000)
+    assert p.kv.pool_bytes > 2 ** 32
+    p.append([130, 70], [0, 0], 8)
+    p.check()
+    p.check_attn(8, [2, 1], [130, 70], "f16")
+
+
+def test_captured_step_follows_device_state(native, ctx):
+    """append + attn recorded once, replayed while lengths, rows and the table's pages change on the device."""
+    N, hd, nkv, nh = native, 64, 2, 4
+    p = Pool(native, ctx, 0, nkv, hd, 16, 3, 80, seed=15)
+    p.append([20, 0, 15], [0, 0, 0], nkv)
+    w = (nh + 2 * nkv) * hd
+    dx, st = ctx.alloc(3 * w * 4), p.ints([0, 1, 2, 3])
+    dp, dl = ctx.alloc(12), ctx.alloc(12)
+    dq, do = ctx.alloc(3 * nh * hd * 4), ctx.alloc(3 * nh * hd * 4)
+
+    def step():
+        p.kv.append(p.pages.ptr, 0, dx.ptr, w, dx.ptr + nh * hd * 4, w, dx.ptr + (nh + nkv) * hd * 4, w, nh, st.ptr, dp.ptr,
+                    p.table.ptr, p.ld, 3, 3, 0, dq.ptr, nh * hd)
+        p.kv.attn(p.pages.ptr, 0, dq.ptr, nh * hd, nh, st.ptr, dl.ptr, p.table.ptr, p.ld, 3, 3, 0.125, do.ptr, nh * hd)
+
+    past = np.array([r.n for r in p.ref], np.int32)
+    graphs = [ctx.capture(step), ctx.capture(step)]
+    for i in range(20):
+        x = p.rng.standard_normal((3, w)).astype(np.float32)
+        dx.upload(x)
+        dp.upload(past)
+        dl.upload(past + 1)
+        graphs[i % 2].launch()
+        out = do.download().reshape(3, nh, hd)
+        for s in range(3):
+            q, k, v = np.split(x[s].astype(np.float64), [nh * hd, (nh + nkv) * hd])
+            p.ref[s].append(int(past[s]), k.reshape(1, nkv, hd), v.reshape(1, nkv, hd))
+            n = int(past[s]) + 1
+            want, mag, dots = R.attention(q.reshape(1, nh, hd), p.ref[s].values(0, n), p.ref[s].values(1, n), 0.125)
+            tol = R.attention_tolerance(want, mag, dots, hd, n, "f32", 2.0 ** -22)
+            assert np.all(np.abs(out[s] - want[0]) <= tol[0])
+        past = past + 1
+    p.check()
+
+
+def test_shared_prefix_page(native, ctx):
+    """Two sequences whose table names the same page read the same tokens."""
+    p = Pool(native, ctx, 0, 2, 64, 16, 2, 32, seed=16)
+    p.append([16, 0], [0, 0], 2)
+    tb = p.table.download(np.int32).reshape(2, p.ld).copy()
+    tb[1, 0] = tb[0, 0]
+    p.table.upload(tb)
+    p.ref[1].append(0, p.ref[0].values(0, 16), p.ref[0].values(1, 16))
+    p.check_attn(4, [1, 1], [16, 16], "bf16")
+    p.append([0, 4], [16, 16], 2)
+    p.check_attn(4, [1, 1], [16, 20], "bf16")
+
+
+def test_nothing_to_do(native, ctx):
+    p = Pool(native, ctx, 0, 2, 64, 16, 2, 32)
+    n0 = ctx.launches
+    for seqs, rows in ((0, 0), (2, 0), (0, 4)):
+        p.kv.append(p.pages.ptr, 0, None, 0, None, 0, None, 0, 0, None, None, None, 0, seqs, rows, 0, None, 0)
+        p.kv.read(p.pages.ptr, None, None, None, 0, seqs, rows, 0, None, 0, None, 0)
+        p.kv.attn(p.pages.ptr, 0, None, 0, 2, None, None, None, 0, seqs, rows, 1.0, None, 0)
+    assert ctx.launches == n0
+
+
+def test_refusals(native, ctx):
+    N = native
+    for bad in (dict(code=7), dict(hd=40), dict(page=24), dict(rope=2, rope_dim=7), dict(rope=1, rope_dim=64, theta=-1.0),
+                dict(rope=1, rope_dim=64, scaling=(8.0, 4.0, 1.0, 100))):
+        kw = dict(code=0, nkv=2, hd=64, page=16, rope=0, rope_dim=0, theta=1e4, scaling=(0.0, 1.0, 4.0, 8192))
+        kw.update(bad)
+        with pytest.raises(N.PureBeeError, match="PB_ERR_ARG"):
+            N.KV8(ctx, kw["code"], kw["nkv"], kw["hd"], kw["page"], 4, kw["rope"], kw["rope_dim"], kw["theta"], kw["scaling"])
+    p = Pool(native, ctx, 0, 2, 64, 16, 1, 32)
+    x, o, i = ctx.alloc(1 << 16), ctx.alloc(1 << 16), p.ints([0, 1])
+    ok = dict(pages=p.pages.ptr, type_=0, q=x.ptr, ldq=256, k=x.ptr, ldk=128, v=x.ptr, ldv=128, n_heads=4, starts=i.ptr,
+              past=i.ptr, table=p.table.ptr, ld_table=p.ld, n_seqs=1, n_rows=1, otype=0, q_out=o.ptr, ldqo=256)
+    bad = [dict(pages=None), dict(pages=p.pages.ptr + 8), dict(type_=2), dict(otype=5), dict(k=None), dict(v=x.ptr + 4),
+           dict(ldk=127), dict(ldk=130), dict(ldv=64), dict(ldq=255), dict(q_out=x.ptr), dict(q_out=None), dict(q=None),
+           dict(n_heads=0), dict(starts=None), dict(past=None), dict(table=None), dict(n_seqs=-1), dict(n_rows=-1),
+           dict(ldqo=200), dict(k_out=x.ptr, ldko=128), dict(k_out=o.ptr + 4, ldko=128), dict(v_out=o.ptr, ldvo=100)]
+    n0 = ctx.launches
+    for b in bad:
+        with pytest.raises(N.PureBeeError, match="PB_ERR_ARG"):
+            p.kv.append(**{**ok, **b})
+    ok = dict(pages=p.pages.ptr, type_=0, q=x.ptr, ldq=256, n_heads=4, starts=i.ptr, lens=i.ptr, table=p.table.ptr,
+              ld_table=p.ld, n_seqs=1, n_rows=1, scale=1.0, out=o.ptr, ldo=256)
+    for b in (dict(n_heads=3), dict(n_heads=0), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(ldq=129),
+              dict(out=o.ptr + 2), dict(type_=8), dict(lens=None), dict(ld_table=-1)):
+        with pytest.raises(N.PureBeeError, match="PB_ERR_ARG"):
+            p.kv.attn(**{**ok, **b})
+    ok = dict(pages=p.pages.ptr, starts=i.ptr, first=i.ptr, table=p.table.ptr, ld_table=p.ld, n_seqs=1, n_rows=1, otype=0,
+              k_out=o.ptr, ldk=128, v_out=o.ptr, ldv=128)
+    for b in (dict(otype=3), dict(ldk=100), dict(v_out=o.ptr + 8), dict(first=None)):
+        with pytest.raises(N.PureBeeError, match="PB_ERR_ARG"):
+            p.kv.read(**{**ok, **b})
+    assert ctx.launches == n0
+
+
+@pytest.mark.parametrize("what", ["page", "negative page", "length", "rows", "past"])
+def test_bad_device_state_raises_the_error_word(native, what):
+    """Tables, lengths and row bounds that do not fit: an error word, nothing written outside."""
+    c = native.Context(0)
+    p = Pool(native, c, 0, 2, 64, 16, 2, 32, seed=17)
+    p.append([20, 20], [0, 0], 2)
+    p.check()
+    tb = p.table.download(np.int32).reshape(2, p.ld).copy()
+    if what in ("page", "negative page"):
+        tb[1, 1] = p.n_pages if what == "page" else -1
+        p.table.upload(tb)
+    x, o = c.alloc(1 << 16), c.alloc(1 << 16)
+    c._check(native.lib().pb_memset(c.h, x.ptr, 0, 1 << 16))
+    if what == "past":
+        bufs = p.ints([0, 1, 2]), p.ints([-5, 1 << 20])
+        p.kv.append(p.pages.ptr, 0, None, 0, x.ptr, 128, x.ptr, 128, 0, bufs[0].ptr, bufs[1].ptr, p.table.ptr, p.ld, 2, 2, 0,
+                    None, 0)
+    else:
+        st = [0, 1, 5] if what == "rows" else [0, 1, 2]
+        ln = [20, 20] if what != "length" else [20, 1000]
+        bufs = p.ints(st), p.ints(ln)
+        p.kv.attn(p.pages.ptr, 0, x.ptr, 256, 4, bufs[0].ptr, bufs[1].ptr, p.table.ptr, p.ld, 2, 2, 1.0, o.ptr, 256)
+    with pytest.raises(native.PureBeeError, match="PB_ERR_DEVICE.*bounds"):
+        c.sync()
+    assert c.device_error() == 1
+    p.kv.free()
+    c.close()
