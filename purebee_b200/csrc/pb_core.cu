@@ -130,6 +130,7 @@ extern "C" int pb_init(int device, pb_ctx** out) {
   if (pb_setup_q4_kernels() != PB_OK || pb_setup_ops_kernels() != PB_OK || pb_setup_gemm_kernels() != PB_OK ||
       pb_setup_mvi_kernels() != PB_OK || pb_setup_mvt_kernels() != PB_OK ||
       pb_setup_sample_kernels() != PB_OK || pb_setup_packed_kernels() != PB_OK ||
+      pb_setup_kv8_kernels() != PB_OK ||
       pb_setup_noalloc(ctx) != PB_OK) {
     pb_shutdown(ctx);
     return PB_ERR_CUDA;

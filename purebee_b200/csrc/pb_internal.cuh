@@ -557,6 +557,7 @@ int pb_setup_ops_kernels(void);
 int pb_setup_gemm_kernels(void);
 int pb_setup_sample_kernels(void);
 int pb_setup_packed_kernels(void);
+int pb_setup_kv8_kernels(void);
 // Top-K sampling (pb_sample.cu): candidate keys needed, and the two launches.
 size_t pb_sample_cand_count(int V, int K);
 int pb_launch_sample(pb_ctx* ctx, const float* logits, int V, int K, double temperature, uint64_t seed,

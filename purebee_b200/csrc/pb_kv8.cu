@@ -233,135 +233,509 @@ k_kv8_read(kv8_geo g, uint8_t* pages, const int* __restrict__ starts, const int*
 // attention of the newest tokens over the cache
 // ============================================================================
 
+// The rows of a sequence that share a kv head (its new tokens x the head's
+// group) are taken TR at a time: a row tile.  The work of all row tiles and kv
+// heads, counted in 16-token blocks, is cut into chunks of at most C blocks of
+// one (sequence, row tile, head), C chosen so that about `slots` CTAs share it
+// evenly whatever the lengths; every CTA finds its own chunk from the lengths
+// on the device (kt_plan), so a recorded graph follows them.  A warp takes
+// every KT_WARPS-th block of the chunk through a ring of its own, one bulk
+// copy a block (K codes, V codes and scales are contiguous), and keeps running
+// maximum, sum and output of its rows; warps join in shared memory, chunks in
+// the workspace, where the last CTA to arrive adds them in order.
+//
+// Both products run as m16n8k16 f16 products straight from the codes (every
+// code is exact in f16): S = Q K^T with rows = queries, columns = tokens, whose
+// accumulators are the A operand of O = P V.  A tile of 8 rows (TR = 8) uses
+// the operand's other 8 rows for what f16 leaves of a value: rows 0-7 hold
+// hi = f16(x), rows 8-15 lo = f16(x - hi), and the two accumulators of a row
+// meet in one thread.  Queries and probabilities then keep 22 bits at no extra
+// product.  TR = 16 takes 16-bit queries (exact in f16 after a power of two
+// per row) and rounds p once, half a step of f16.
+//
+// Scales: S's columns times 2^ke of the block.  V's 2^ve is put into the
+// exponent, p' = 2^(s + ve - m2), with a running reference m2 of s + ve of its
+// own, so p' uses f16's range whatever V's scales; the sum l runs beside it
+// over 2^(s - m1).  out = O / l * 2^(m2 - m1).
 constexpr int KT_WARPS = 4;
+constexpr int KT_STAGES = 4;
+constexpr int KT_MIN_BLOCKS = KT_WARPS;  // the least work of a chunk
+constexpr float KT_RISE = 8.0f, KT_BIAS = 6.0f;  // p' <= 2^(8 + 6)
+constexpr float KT_LOW = -1e30f;
 
-// out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q . k_j - max): one CTA per
-// (row, head), a warp on every fourth block with its own running maximum, sum
-// and output (the online softmax), joined at the end.  f32 throughout.
-__global__ void __launch_bounds__(KT_WARPS * 32)
-k_kv8_attn(kv8_geo g, const uint8_t* pages, const void* __restrict__ q, int type, int ldq, int n_heads,
-           const int* __restrict__ starts, const int* __restrict__ lens, const int* __restrict__ table, int ld_table,
-           int n_seqs, int n_rows, float scale, void* out, int ldo, int* err) {
-  __shared__ float qs[256], ms[KT_WARPS], ls[KT_WARPS], os[KT_WARPS][256];
-  __shared__ int found;
-  pb_pdl_trigger();
-  pb_pdl_wait();
-  const int row = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int gq = lane >> 2, t = lane & 3, kvh = h / (n_heads / g.n_kv), tiles = g.hd / 32;
-  if (tid == 0) found = -1;
-  __syncthreads();
-  for (int s = tid; s < n_seqs; s += KT_WARPS * 32) {
-    const int a = starts[s], b = starts[s + 1];
-    if (a < 0 || b < a || b > n_rows) pb_raise(err, PB_DEVERR_BOUNDS);
-    else if (a <= row && row < b) found = s;
-  }
-  __syncthreads();
-  const int seq = found;
-  if (seq < 0) return;
-  int len = lens[seq];
-  if (len < 0 || (int64_t)len > (int64_t)ld_table * g.page) {
-    if (tid == 0) pb_raise(err, PB_DEVERR_BOUNDS);
+struct kt_args {
+  const uint8_t* pages;
+  const void* q;
+  void* out;
+  const int *starts, *lens, *table;
+  int type, ldq, ldo, n_heads, group, ld_table, n_seqs, n_rows, slots;
+  float scale;  // times log2(e)
+  float* ws;
+  unsigned int* cnt;
+  int* err;
+};
+
+struct kt_item {
+  int seq, rt, chunk, chunks, slot0, C;  // slot0: the first chunk's number among the split ones (of one kv head)
+};
+
+// A sequence's rows and blocks; a bad one has no rows and raises the error word.
+__device__ __forceinline__ void kt_seq(const kv8_geo& g, const kt_args& a, int tr, int s, int& rts, int& blocks) {
+  const int lo = a.starts[s], hi = a.starts[s + 1], len = a.lens[s];
+  rts = blocks = 0;
+  if (lo < 0 || hi < lo || hi > a.n_rows || len < 0 || len > (int64_t)a.ld_table * g.page) {
+    pb_raise(a.err, PB_DEVERR_BOUNDS);
     return;
   }
-  const int see = max(0, len - (starts[seq + 1] - row) + 1);  // keys this row sees
-  for (int d = tid; d < g.hd; d += KT_WARPS * 32) {
-    const int64_t i = (int64_t)row * ldq + h * g.hd + d;
-    qs[d] = (type == PB_TYPE_F32 ? static_cast<const float*>(q)[i] : kv8_from16(static_cast<const uint16_t*>(q)[i], type)) * scale;
+  rts = (int)(((int64_t)(hi - lo) * a.group + tr - 1) / tr);
+  blocks = rts ? (len + PB_KV8_BLOCK - 1) / PB_KV8_BLOCK : 0;
+}
+
+// The chunk number `item` (of one kv head).  Every thread calls it.
+__device__ __forceinline__ bool kt_plan(const kv8_geo& g, const kt_args& a, int tr, int item, kt_item& it) {
+  constexpr int T = KT_WARPS * 32;
+  __shared__ long long wsum[KT_WARPS];
+  __shared__ int isum[KT_WARPS][2];
+  __shared__ kt_item found;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int per = (a.n_seqs + T - 1) / T, s0 = min(a.n_seqs, tid * per), s1 = min(a.n_seqs, s0 + per);
+  int rts = 0, blocks = 0;  // of sequence s0, all there is for up to T sequences
+  long long w = 0;
+  for (int s = s1 - 1; s >= s0; --s) {
+    kt_seq(g, a, tr, s, rts, blocks);
+    w += (long long)rts * blocks;
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+  if (lane == 0) wsum[warp] = w;
+  if (tid == 0) found.seq = -1;
   __syncthreads();
-  float m = -INFINITY, l = 0.0f, acc[8][4];
+  w = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-  for (int b = warp; b * PB_KV8_BLOCK < see; b += KT_WARPS) {
-    const uint8_t* blk = kv8_block(const_cast<uint8_t*>(pages), g, table, ld_table, seq, b, err);
-    if (!blk) break;
-    blk += (int64_t)kvh * g.nblk * g.block_bytes;
-    const int8_t* ep = reinterpret_cast<const int8_t*>(blk + 32 * g.hd);
-    const float ks = kv8_scale(ep[0]), vs = kv8_scale(ep[1]);
-    float s0 = 0.0f, s1 = 0.0f;
-    for (int i = 0; i < tiles; ++i) {
-      const uint4 w4 = reinterpret_cast<const uint4*>(blk + i * 512)[lane];
-      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float qv = qs[i * 32 + 8 * t + j];
-        s0 = fmaf(qv, kv8_decode((w[j >> 2] >> (8 * (j & 3))) & 0xFFu, g.code), s0);
-        s1 = fmaf(qv, kv8_decode((w[2 + (j >> 2)] >> (8 * (j & 3))) & 0xFFu, g.code), s1);
-      }
-    }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-      s1 += __shfl_xor_sync(0xffffffffu, s1, o);
-    }
-    const int tok = b * PB_KV8_BLOCK + gq;  // s0, s1: tokens gq and gq + 8 of the block
-    s0 = tok < see ? s0 * ks : -INFINITY;
-    s1 = tok + 8 < see ? s1 * ks : -INFINITY;
-    float bm = fmaxf(s0, s1);
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, o));
-    const float mn = fmaxf(m, bm), ref = mn == -INFINITY ? 0.0f : mn, f = expf(m - ref);
-    const float p0 = expf(s0 - ref), p1 = expf(s1 - ref);
-    m = mn;
-    float ps = p0 + p1;
-#pragma unroll
-    for (int o = 4; o < 32; o <<= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
-    l = l * f + ps;
-    float pj[4];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9
-    pj[0] = __shfl_sync(0xffffffffu, p0, 8 * t);
-    pj[1] = __shfl_sync(0xffffffffu, p0, 8 * t + 4);
-    pj[2] = __shfl_sync(0xffffffffu, p1, 8 * t);
-    pj[3] = __shfl_sync(0xffffffffu, p1, 8 * t + 4);
-    for (int j = 0; j < 4; ++j)  // a masked token adds nothing, whatever the block's scale
-      pj[j] = b * PB_KV8_BLOCK + 2 * t + (j & 1) + 8 * (j >> 1) < see ? pj[j] * vs : 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i >= tiles) break;
-      const uint4 w4 = reinterpret_cast<const uint4*>(blk + 16 * g.hd + i * 512)[lane];
-      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        float x = acc[i][d] * f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x = fmaf(pj[j], kv8_decode((w[d] >> (8 * j)) & 0xFFu, g.code), x);
-        acc[i][d] = x;
-      }
-    }
+  for (int i = 0; i < KT_WARPS; ++i) w += wsum[i];
+  long long c = (w * g.n_kv + a.slots - 1) / a.slots;
+  c = c < KT_MIN_BLOCKS ? KT_MIN_BLOCKS : (c + KT_WARPS - 1) / KT_WARPS * KT_WARPS;
+  const int C = c > (1 << 28) ? 1 << 28 : (int)c;
+  int mine = 0, split = 0;
+  for (int s = s1 - 1; s >= s0; --s) {
+    if (per > 1) kt_seq(g, a, tr, s, rts, blocks);
+    const int n = blocks > C ? (blocks + C - 1) / C : 1;
+    mine += rts * n;
+    split += n > 1 ? rts * n : 0;
   }
-  if (lane == 0) ms[warp] = m, ls[warp] = l;
+  int before = mine, sbefore = split;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (i >= tiles) break;
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      float x = acc[i][d];
-      x += __shfl_xor_sync(0xffffffffu, x, 1);
-      x += __shfl_xor_sync(0xffffffffu, x, 2);
-      if (t == 0) os[warp][i * 32 + 4 * gq + d] = x;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, before, o), y = __shfl_up_sync(0xffffffffu, sbefore, o);
+    if (lane >= o) before += x, sbefore += y;
+  }
+  if (lane == 31) isum[warp][0] = before, isum[warp][1] = sbefore;
+  __syncthreads();
+  before -= mine, sbefore -= split;
+  for (int i = 0; i < warp; ++i) before += isum[i][0], sbefore += isum[i][1];
+  if (item >= before && item < before + mine) {
+    for (int s = s0; s < s1; ++s) {
+      if (per > 1) kt_seq(g, a, tr, s, rts, blocks);
+      const int n = blocks > C ? (blocks + C - 1) / C : 1;
+      if (item < before + rts * n) {
+        const int x = item - before;
+        found = {s, x / n, x % n, n, sbefore + x / n * n, C};
+        break;
+      }
+      before += rts * n;
+      sbefore += n > 1 ? rts * n : 0;
     }
   }
   __syncthreads();
-  float mx = -INFINITY;
-  bool nan = false;
-  for (int w = 0; w < KT_WARPS; ++w) {
-    mx = fmaxf(mx, ms[w]);
-    nan |= ls[w] != ls[w];
+  it = found;
+  return it.seq >= 0;
+}
+
+__device__ __forceinline__ float kt_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t kt_h2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// what f16 left of the pair
+__device__ __forceinline__ uint32_t kt_lo2(float a, float b, uint32_t hi) {
+  const __half2 h = *reinterpret_cast<const __half2*>(&hi);
+  return kt_h2(__fsub_rn(a, __low2float(h)), __fsub_rn(b, __high2float(h)));
+}
+// four codes -> two f16 pairs, exact
+template <int CODE>
+__device__ __forceinline__ void kt_codes(uint32_t w, uint32_t& p01, uint32_t& p23) {
+  if (CODE == PB_KV8_INT8) {
+    // 0x64 over a byte u is the f16 1024 + u; u = code + 128
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));  // 1152
+    uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 hx = __hsub2(*reinterpret_cast<__half2*>(&x), off), hy = __hsub2(*reinterpret_cast<__half2*>(&y), off);
+    p01 = *reinterpret_cast<const uint32_t*>(&hx);
+    p23 = *reinterpret_cast<const uint32_t*>(&hy);
+  } else {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(p01), "=r"(p23)
+        : "r"(w));
   }
-  for (int d = tid; d < g.hd; d += KT_WARPS * 32) {
-    float o = 0.0f, ll = 0.0f;
-    for (int w = 0; w < KT_WARPS; ++w) {
-      if (ls[w] == 0.0f) continue;  // no key seen (or none with weight): nothing to add
-      const float f = expf(ms[w] - mx);
-      ll += ls[w] * f;
-      o += os[w][d] * f;
+}
+__device__ __forceinline__ void kt_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+               "{%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// O and {m1, m2, l} of n parts of a row, added in order; part i's output at
+// po + i * so, its {m1, m2, l} at pm + i * sm.  L2: written by other SMs.
+template <bool L2>
+__device__ __forceinline__ void kt_join(const float* po, size_t so, const float* pm, size_t sm, int n, float4& ov, float4& mv) {
+  auto ld = [](const float* p) {
+    return L2 ? __ldcg(reinterpret_cast<const float4*>(p)) : *reinterpret_cast<const float4*>(p);
+  };
+  float a1 = KT_LOW, a2 = KT_LOW;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const float4 m = ld(pm + i * sm);
+    a1 = fmaxf(a1, m.x), a2 = fmaxf(a2, m.y);
+  }
+  ov = make_float4(0, 0, 0, 0);
+  float ll = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const float4 m = ld(pm + i * sm), x = ld(po + i * so);
+    const float f = kt_ex2(m.y - a2);
+    ll += m.z * kt_ex2(m.x - a1);
+    ov.x += x.x * f, ov.y += x.y * f, ov.z += x.z * f, ov.w += x.w * f;
+  }
+  mv = make_float4(a1, a2, ll, 0.0f);
+}
+
+static size_t kt_smem(int hd) {
+  const size_t ring = (size_t)KT_WARPS * KT_STAGES * (32 * hd + 16), join = (size_t)KT_WARPS * 16 * (hd + 4) * 4;
+  return ring > join ? ring : join;
+}
+
+template <int HD, int CODE, int TR>
+__global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : 2) k_kv8_attn(kv8_geo g, kt_args a) {
+  constexpr int NT = HD / 32, BB = 32 * HD + 16;
+  constexpr bool HL = TR == 8;
+  constexpr int NR = HL ? 1 : 2;  // rows of the tile in a thread: gq, and gq + 8
+  extern __shared__ __align__(16) unsigned char kt_raw[];
+  __shared__ uint64_t full[KT_WARPS][KT_STAGES];
+  __shared__ unsigned int last;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
+  if (lane == 0) {
+    for (int s = 0; s < KT_STAGES; ++s) pb_mbar_init(&full[warp][s], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  pb_pdl_trigger();
+  pb_pdl_wait();
+  kt_item it;
+  const int kvh = blockIdx.x % g.n_kv;
+  if (!kt_plan(g, a, TR, blockIdx.x / g.n_kv, it)) return;
+  const int row0 = a.starts[it.seq], nq = a.starts[it.seq + 1] - row0, len = a.lens[it.seq];
+  const int rows = nq * a.group;
+  const int b0 = it.chunk * it.C, b1 = min((len + PB_KV8_BLOCK - 1) / PB_KV8_BLOCK, b0 + it.C);
+  const int nb = b1 - b0, mine = nb > warp ? (nb - 1 - warp) / KT_WARPS + 1 : 0;  // this warp's blocks b0 + warp + i KT_WARPS
+  unsigned char* ring = kt_raw + (size_t)warp * KT_STAGES * BB;
+  const int* trow = a.table + (int64_t)it.seq * a.ld_table;
+
+  // page ids of 32 iterations, a lane each; a bad one raises the error word and reads page 0
+  auto load_ids = [&](int i0) {
+    const int i = i0 + lane;
+    if (i >= mine) return 0;
+    const int id = trow[(b0 + warp + i * KT_WARPS) / g.nblk];
+    if (id < 0 || id >= g.n_pages) {
+      pb_raise(a.err, PB_DEVERR_BOUNDS);
+      return 0;
     }
-    const float r = nan ? __int_as_float(0x7fc00000) : see > 0 ? o / ll : 0.0f;
-    const int64_t i = (int64_t)row * ldo + h * g.hd + d;
-    if (type == PB_TYPE_F32) static_cast<float*>(out)[i] = r;
-    else static_cast<uint16_t*>(out)[i] = (uint16_t)kv8_to16(r, type);
+    return id;
+  };
+  int ids = load_ids(0), ids_next = load_ids(32);
+  auto fetch = [&](int i) {  // block i of this warp into its stage; i rises by one a call
+    if (i > 0 && (i & 31) == 0) {
+      ids = ids_next;
+      ids_next = load_ids(i + 32);
+    }
+    const int id = __shfl_sync(0xffffffffu, ids, i & 31);
+    if (lane == 0 && i < mine) {
+      const int b = (b0 + warp + i * KT_WARPS) % g.nblk, s = i % KT_STAGES;
+      pb_mbar_arrive_tx(&full[warp][s], BB);
+      pb_bulk_g2s(ring + s * BB, a.pages + (int64_t)id * g.page_bytes + ((int64_t)kvh * g.nblk + b) * BB, BB, &full[warp][s]);
+    }
+  };
+#pragma unroll 1
+  for (int i = 0; i < KT_STAGES; ++i) fetch(i);
+
+  // Q: x * 2^-e of the row's largest, A fragments in the tiles' order
+  uint32_t qa[NT][2][4];
+  float qf[NR];
+  int see[NR];  // keys the row sees
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const int rho = it.rt * TR + gq + 8 * r;
+    const bool live = rho < rows;
+    const int tok = live ? rho / a.group : 0, h = kvh * a.group + (live ? rho % a.group : 0);
+    see[r] = live ? max(0, len - nq + tok + 1) : 0;
+    const int64_t at = (int64_t)(row0 + tok) * a.ldq + h * HD + 8 * t;
+    float x[NT][8];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      if (live) {
+        kv8_load(a.q, a.type, at + 32 * i, x[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[i][j] = 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[i][j]) & 0x7FFFFFFFu);
+    }
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    // 2^-e brings the largest into [1, 2); a subnormal or non-finite row stays as it is
+    int e = (int)(m >> 23) - 127;
+    if (e < -126 || e > 126) e = 0;
+    const float inv = kv8_pow2(-e);
+    qf[r] = a.scale * kv8_pow2(e);
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const float y0 = x[i][4 * s] * inv, y1 = x[i][4 * s + 1] * inv, y2 = x[i][4 * s + 2] * inv, y3 = x[i][4 * s + 3] * inv;
+        qa[i][s][r] = kt_h2(y0, y1);
+        qa[i][s][2 + r] = kt_h2(y2, y3);
+        if (HL) {
+          qa[i][s][1] = kt_lo2(y0, y1, qa[i][s][0]);
+          qa[i][s][3] = kt_lo2(y2, y3, qa[i][s][2]);
+        }
+      }
   }
+  // the fewest keys a live row of the tile sees: blocks up to there need no mask
+  const int see_min = max(0, len - nq + it.rt * TR / a.group + 1);
+
+  float o[NT][4][4], m1[NR], m2[NR], l[NR];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) o[i][j][x] = 0.0f;
+#pragma unroll
+  for (int r = 0; r < NR; ++r) m1[r] = m2[r] = KT_LOW, l[r] = 0.0f;
+
+  int i = 0;
+  for (; i < mine; ++i) {
+    const int st = i % KT_STAGES;
+    if (!__all_sync(0xffffffffu, pb_mbar_wait(&full[warp][st], (i / KT_STAGES) & 1, a.err))) break;
+    const unsigned char* blk = ring + st * BB;
+    const int es = *reinterpret_cast<const uint16_t*>(blk + 32 * HD);
+    const int ke = (int8_t)(es & 0xFF), ve = (int8_t)(es >> 8);
+    float s[2][4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s[j][x] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const uint4 w = reinterpret_cast<const uint4*>(blk + n * 512)[lane];
+      uint32_t b0_, b1_;
+      kt_codes<CODE>(w.x, b0_, b1_);
+      kt_mma(s[0], qa[n][0][0], qa[n][0][1], qa[n][0][2], qa[n][0][3], b0_, b1_);
+      kt_codes<CODE>(w.z, b0_, b1_);
+      kt_mma(s[1], qa[n][0][0], qa[n][0][1], qa[n][0][2], qa[n][0][3], b0_, b1_);
+      kt_codes<CODE>(w.y, b0_, b1_);
+      kt_mma(s[0], qa[n][1][0], qa[n][1][1], qa[n][1][2], qa[n][1][3], b0_, b1_);
+      kt_codes<CODE>(w.w, b0_, b1_);
+      kt_mma(s[1], qa[n][1][0], qa[n][1][1], qa[n][1][2], qa[n][1][3], b0_, b1_);
+    }
+    const int tok0 = (b0 + warp + i * KT_WARPS) * PB_KV8_BLOCK;
+    const bool mask = tok0 + PB_KV8_BLOCK > see_min;
+    const float ks = kv8_scale(ke);
+    const float vadd = ve == KV8_E_ZERO ? -INFINITY : ve == KV8_E_NAN ? __int_as_float(0x7fc00000) : (float)ve;
+    uint32_t pa[4];
+    float rescale[NR];
+    bool any = false;
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const float f = qf[r] * ks;
+      float x[4];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float* c = s[j >> 1];
+        x[j] = (HL ? c[j & 1] + c[2 + (j & 1)] : c[2 * r + (j & 1)]) * f;
+      }
+      if (mask) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (tok0 + 2 * t + (j & 1) + 8 * (j >> 1) >= see[r]) x[j] = -INFINITY;
+      }
+      float bm = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+      bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 1));
+      bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
+      if (bm > m1[r] + KT_RISE) {
+        l[r] *= kt_ex2(m1[r] - bm);
+        m1[r] = bm;
+      }
+      rescale[r] = 1.0f;
+      const float bv = bm + vadd;
+      if (bv > m2[r] + KT_RISE) {
+        rescale[r] = kt_ex2(m2[r] - bv);
+        m2[r] = bv;
+        any = true;
+      }
+      float p[4];
+      const float off = vadd + (KT_BIAS - m2[r]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        l[r] += kt_ex2(x[j] - m1[r]);
+        p[j] = kt_ex2(x[j] + off);
+      }
+      if (mask) {  // nothing of a masked token, whatever the block's scale
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (tok0 + 2 * t + (j & 1) + 8 * (j >> 1) >= see[r]) p[j] = 0.0f;
+      }
+      pa[r] = kt_h2(p[0], p[1]);
+      pa[2 + r] = kt_h2(p[2], p[3]);
+      if (HL) {
+        pa[1] = kt_lo2(p[0], p[1], pa[0]);
+        pa[3] = kt_lo2(p[2], p[3], pa[2]);
+      }
+    }
+    if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[n][j][x] *= rescale[HL ? 0 : x >> 1];
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const uint4 w = reinterpret_cast<const uint4*>(blk + 16 * HD + n * 512)[lane];
+      const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t b0_, b1_;
+        kt_codes<CODE>(ww[j], b0_, b1_);
+        kt_mma(o[n][j], pa[0], pa[1], pa[2], pa[3], b0_, b1_);
+      }
+    }
+    // every lane's reads of the stage come before the copy that refills it
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    fetch(i + KT_STAGES);
+  }
+  for (int k = i; k < mine && k < i + KT_STAGES; ++k)  // a wait gave up: the copies on their way land first
+    pb_mbar_wait(&full[warp][k % KT_STAGES], (k / KT_STAGES) & 1, a.err);
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {  // l is each lane's own tokens' sum
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+  }
+
+  // join the warps
+  __syncthreads();
+  float* jo = reinterpret_cast<float*>(kt_raw);  // [KT_WARPS][TR][HD]
+  float* jm = jo + KT_WARPS * TR * HD;           // [KT_WARPS][TR][4]: m1, m2, l
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const int row = gq + 8 * r;
+    float* d = jo + (warp * TR + row) * HD + 8 * t;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float y[8];  // accumulator (j, c0 / c1): values j and 4 + j of the lane's 8
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        y[j] = HL ? o[n][j][0] + o[n][j][2] : o[n][j][2 * r];
+        y[4 + j] = HL ? o[n][j][1] + o[n][j][3] : o[n][j][2 * r + 1];
+      }
+      *reinterpret_cast<float4*>(d + 32 * n) = make_float4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<float4*>(d + 32 * n + 4) = make_float4(y[4], y[5], y[6], y[7]);
+    }
+    if (t == 0) *reinterpret_cast<float4*>(jm + (warp * TR + row) * 4) = make_float4(m1[r], m2[r], l[r], 0.0f);
+  }
+  __syncthreads();
+  const int live = min(TR, rows - it.rt * TR);
+  auto finish = [&](int row, int d, const float4& ov, const float4& mv) {
+    const int rho = it.rt * TR + row, h = kvh * a.group + rho % a.group;
+    float y[4] = {0, 0, 0, 0};
+    if (len - nq + rho / a.group >= 0) {  // the row sees a key
+      const float f = 1.0f / mv.z, up = mv.y - mv.x - KT_BIAS;
+      // 2^up in two halves: it may pass f32's range where the row's values do not
+      const float u0 = kt_ex2(0.5f * up);
+      y[0] = ov.x * f * u0 * u0, y[1] = ov.y * f * u0 * u0, y[2] = ov.z * f * u0 * u0, y[3] = ov.w * f * u0 * u0;
+    }
+    kv8_store(a.out, a.type, (int64_t)(row0 + rho / a.group) * a.ldo + h * HD + d, y);
+  };
+  constexpr int SLOT = TR * (HD + 4);  // floats: [TR][HD], [TR][4]
+  for (int x = tid; x < live * (HD / 4); x += KT_WARPS * 32) {
+    const int row = x / (HD / 4), d = x % (HD / 4) * 4;
+    float4 ov, mv;
+    kt_join<false>(jo + row * HD + d, (size_t)TR * HD, jm + row * 4, (size_t)TR * 4, KT_WARPS, ov, mv);
+    if (it.chunks == 1) {
+      finish(row, d, ov, mv);
+    } else {
+      float* slot = a.ws + (size_t)((it.slot0 + it.chunk) * g.n_kv + kvh) * SLOT;
+      __stcg(reinterpret_cast<float4*>(slot + row * HD + d), ov);
+      if (d == 0) __stcg(reinterpret_cast<float4*>(slot + TR * HD + row * 4), mv);
+    }
+  }
+  if (it.chunks == 1) return;
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) {
+    unsigned int* c = a.cnt + (size_t)it.slot0 * g.n_kv + kvh;
+    last = atomicAdd(c, 1u) == (unsigned)it.chunks - 1 ? 1u : 0u;
+    if (last) *c = 0;  // for the next call
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  const float* slot = a.ws + (size_t)(it.slot0 * g.n_kv + kvh) * SLOT;
+  for (int x = tid; x < live * (HD / 4); x += KT_WARPS * 32) {
+    const int row = x / (HD / 4), d = x % (HD / 4) * 4;
+    float4 ov, mv;
+    kt_join<true>(slot + row * HD + d, (size_t)g.n_kv * SLOT, slot + TR * HD + row * 4, (size_t)g.n_kv * SLOT, it.chunks, ov, mv);
+    finish(row, d, ov, mv);
+  }
+}
+
+typedef void (*kt_kernel)(kv8_geo, kt_args);
+template <int HD>
+static kt_kernel kt_pick(int code, int tr) {
+  if (code == PB_KV8_INT8) return tr == 8 ? k_kv8_attn<HD, PB_KV8_INT8, 8> : k_kv8_attn<HD, PB_KV8_INT8, 16>;
+  return tr == 8 ? k_kv8_attn<HD, PB_KV8_E4M3, 8> : k_kv8_attn<HD, PB_KV8_E4M3, 16>;
+}
+static kt_kernel kt_kernel_of(int hd, int code, int tr) {
+  switch (hd) {
+    case 32: return kt_pick<32>(code, tr);
+    case 64: return kt_pick<64>(code, tr);
+    case 96: return kt_pick<96>(code, tr);
+    case 128: return kt_pick<128>(code, tr);
+    case 160: return kt_pick<160>(code, tr);
+    case 192: return kt_pick<192>(code, tr);
+    case 224: return kt_pick<224>(code, tr);
+    default: return kt_pick<256>(code, tr);
+  }
+}
+
+int pb_setup_kv8_kernels(void) {
+  for (int hd = 32; hd <= 256; hd += 32)
+    for (int code = 0; code < 2; ++code)
+      for (int tr = 8; tr <= 16; tr += 8)
+        if (cudaFuncSetAttribute(kt_kernel_of(hd, code, tr), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)kt_smem(hd)) != cudaSuccess)
+          return PB_ERR_CUDA;
+  return PB_OK;
 }
 
 // ============================================================================
@@ -416,9 +790,17 @@ extern "C" int pb_kv8_create(pb_ctx* ctx, const pb_kv8_config* c, pb_kv8** out) 
   kv->ctx = ctx;
   kv->g = g;
   cudaError_t e = cudaMalloc(&kv->freqs, sizeof freqs);
+  // at most 2 * slots chunks of split sequences (a split one has more than C blocks, so no more than 2 blocks / C chunks)
+  kv->slots = 4 * ctx->sm_count;
+  const size_t parts = 2 * (size_t)kv->slots + g.n_kv;
+  if (e == cudaSuccess) e = cudaMalloc(&kv->ws, parts * 16 * (g.hd + 4) * sizeof(float));
+  if (e == cudaSuccess) e = cudaMalloc(&kv->cnt, parts * sizeof(unsigned int));
+  if (e == cudaSuccess) e = cudaMemset(kv->cnt, 0, parts * sizeof(unsigned int));
   if (e == cudaSuccess && g.rope_dim) e = cudaMemcpy(kv->freqs, freqs, g.rope_dim / 2 * sizeof(double), cudaMemcpyHostToDevice);
   if (e != cudaSuccess) {
     cudaFree(kv->freqs);
+    cudaFree(kv->ws);
+    cudaFree(kv->cnt);
     delete kv;
     return pb_cuda_error(ctx, e, "pb_kv8_create");
   }
@@ -525,7 +907,16 @@ extern "C" int pb_kv8_attn(pb_kv8* kv, const void* pages_dev, int type, const vo
     return pb_set_error(ctx, PB_ERR_ARG, "pb_kv8_attn: rows must be 16-byte aligned, their strides multiples of 16 bytes "
                                          "and no narrower than the heads");
   pb_device_scope dev(ctx->device);
-  return pb_launch(ctx, "k_kv8_attn", true, k_kv8_attn, dim3(n_rows, n_heads), dim3(KT_WARPS * 32), 0, g,
-                   static_cast<const uint8_t*>(pages_dev), q_dev, type, ldq, n_heads, starts_dev, lens_dev, table_dev,
-                   ld_table, n_seqs, n_rows, (float)scale, out_dev, ldo, ctx->d_err);
+  // Row tiles of 8 rows with 22-bit queries and probabilities where the rows are f32, or where 8 rows hold a sequence's on
+  // average (the products cost the same); else 16 rows, half the passes over the codes.
+  const int group = n_heads / g.n_kv, tr = type == PB_TYPE_F32 || (int64_t)n_rows * group <= 8 * (int64_t)n_seqs ? 8 : 16;
+  kt_args a = {static_cast<const uint8_t*>(pages_dev), q_dev, out_dev, starts_dev, lens_dev, table_dev, type, ldq, ldo,
+               n_heads, group, ld_table, n_seqs, n_rows, kv->slots, (float)(scale * 1.4426950408889634), kv->ws, kv->cnt,
+               ctx->d_err};
+  if ((int64_t)n_rows * n_heads > 0x7FFFFFFF)
+    return pb_set_error(ctx, PB_ERR_ARG, "pb_kv8_attn: too many rows and heads for one call");
+  const int64_t grid = ((int64_t)n_rows * group / tr + n_seqs) * g.n_kv + kv->slots + g.n_kv;
+  if (grid > 0x7FFFFFFF) return pb_set_error(ctx, PB_ERR_ARG, "pb_kv8_attn: too many rows and heads for one call");
+  return pb_launch(ctx, "k_kv8_attn", true, kt_kernel_of(g.hd, g.code, tr), dim3((unsigned)grid), dim3(KT_WARPS * 32),
+                   kt_smem(g.hd), g, a);
 }
