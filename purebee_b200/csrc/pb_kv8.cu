@@ -239,8 +239,9 @@ k_kv8_read(kv8_geo g, uint8_t* pages, const int* __restrict__ starts, const int*
 // one (sequence, row tile, head), C chosen so that about `slots` CTAs share it
 // evenly whatever the lengths; every CTA finds its own chunk from the lengths
 // on the device (kt_plan), so a recorded graph follows them.  A warp takes
-// every KT_WARPS-th block of the chunk through a ring of its own, one bulk
-// copy a block (K codes, V codes and scales are contiguous), and keeps running
+// every KT_WARPS-th pair of the chunk's blocks through a ring of its own, one
+// bulk copy a pair (a block's K codes, V codes and scales are contiguous, and
+// so are a page's blocks of a head), and keeps running
 // maximum, sum and output of its rows; warps join in shared memory, chunks in
 // the workspace, where the last CTA to arrive adds them in order.
 //
@@ -258,8 +259,8 @@ k_kv8_read(kv8_geo g, uint8_t* pages, const int* __restrict__ starts, const int*
 // own, so p' uses f16's range whatever V's scales; the sum l runs beside it
 // over 2^(s - m1).  out = O / l * 2^(m2 - m1).
 constexpr int KT_WARPS = 4;
-constexpr int KT_STAGES = 4;
-constexpr int KT_MIN_BLOCKS = KT_WARPS;  // the least work of a chunk
+constexpr int KT_STEP = 2 * KT_WARPS;  // blocks of one round of a CTA's warps: chunks are multiples of it
+__host__ __device__ constexpr int kt_stages(int hd) { return hd <= 64 ? 4 : 2; }
 constexpr float KT_RISE = 8.0f, KT_BIAS = 6.0f;  // p' <= 2^(8 + 6)
 constexpr float KT_LOW = -1e30f;
 
@@ -314,7 +315,7 @@ __device__ __forceinline__ bool kt_plan(const kv8_geo& g, const kt_args& a, int 
 #pragma unroll
   for (int i = 0; i < KT_WARPS; ++i) w += wsum[i];
   long long c = (w * g.n_kv + a.slots - 1) / a.slots;
-  c = c < KT_MIN_BLOCKS ? KT_MIN_BLOCKS : (c + KT_WARPS - 1) / KT_WARPS * KT_WARPS;
+  c = c < KT_STEP ? KT_STEP : (c + KT_STEP - 1) / KT_STEP * KT_STEP;
   const int C = c > (1 << 28) ? 1 << 28 : (int)c;
   int mine = 0, split = 0;
   for (int s = s1 - 1; s >= s0; --s) {
@@ -418,21 +419,21 @@ __device__ __forceinline__ void kt_join(const float* po, size_t so, const float*
 }
 
 static size_t kt_smem(int hd) {
-  const size_t ring = (size_t)KT_WARPS * KT_STAGES * (32 * hd + 16), join = (size_t)KT_WARPS * 16 * (hd + 4) * 4;
+  const size_t ring = (size_t)KT_WARPS * kt_stages(hd) * 2 * (32 * hd + 16), join = (size_t)KT_WARPS * 16 * (hd + 4) * 4;
   return ring > join ? ring : join;
 }
 
 template <int HD, int CODE, int TR>
 __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : 2) k_kv8_attn(kv8_geo g, kt_args a) {
-  constexpr int NT = HD / 32, BB = 32 * HD + 16;
+  constexpr int NT = HD / 32, BB = 32 * HD + 16, STAGES = kt_stages(HD);
   constexpr bool HL = TR == 8;
   constexpr int NR = HL ? 1 : 2;  // rows of the tile in a thread: gq, and gq + 8
   extern __shared__ __align__(16) unsigned char kt_raw[];
-  __shared__ uint64_t full[KT_WARPS][KT_STAGES];
+  __shared__ uint64_t full[KT_WARPS][STAGES];
   __shared__ unsigned int last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
   if (lane == 0) {
-    for (int s = 0; s < KT_STAGES; ++s) pb_mbar_init(&full[warp][s], 1);
+    for (int s = 0; s < STAGES; ++s) pb_mbar_init(&full[warp][s], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   pb_pdl_trigger();
@@ -443,36 +444,47 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : 2) k_kv8_attn(k
   const int row0 = a.starts[it.seq], nq = a.starts[it.seq + 1] - row0, len = a.lens[it.seq];
   const int rows = nq * a.group;
   const int b0 = it.chunk * it.C, b1 = min((len + PB_KV8_BLOCK - 1) / PB_KV8_BLOCK, b0 + it.C);
-  const int nb = b1 - b0, mine = nb > warp ? (nb - 1 - warp) / KT_WARPS + 1 : 0;  // this warp's blocks b0 + warp + i KT_WARPS
-  unsigned char* ring = kt_raw + (size_t)warp * KT_STAGES * BB;
+  // this warp's pairs: the blocks b0 + 2 (warp + i KT_WARPS) and the next one
+  const int np = (b1 - b0 + 1) >> 1, mine = np > warp ? (np - 1 - warp) / KT_WARPS + 1 : 0;
+  unsigned char* ring = kt_raw + (size_t)warp * STAGES * 2 * BB;
   const int* trow = a.table + (int64_t)it.seq * a.ld_table;
+  const int nblk_log2 = 31 - __clz(g.nblk);
+  auto first_block = [&](int i) { return b0 + 2 * (warp + i * KT_WARPS); };
 
-  // page ids of 32 iterations, a lane each; a bad one raises the error word and reads page 0
-  auto load_ids = [&](int i0) {
+  // page ids of 32 iterations, a lane each; a bad one raises the error word and
+  // reads page 0.  x: the pair's block, which is in a page of its own where a
+  // page is one block.
+  auto load_ids = [&](int i0, int x) {
     const int i = i0 + lane;
-    if (i >= mine) return 0;
-    const int id = trow[(b0 + warp + i * KT_WARPS) / g.nblk];
+    if (i >= mine || first_block(i) + x >= b1) return 0;
+    const int id = trow[(first_block(i) + x) >> nblk_log2];
     if (id < 0 || id >= g.n_pages) {
       pb_raise(a.err, PB_DEVERR_BOUNDS);
       return 0;
     }
     return id;
   };
-  int ids = load_ids(0), ids_next = load_ids(32);
-  auto fetch = [&](int i) {  // block i of this warp into its stage; i rises by one a call
+  const bool one = g.nblk == 1;
+  int ids = load_ids(0, 0), ids_next = load_ids(32, 0), ids1 = one ? load_ids(0, 1) : 0;
+  auto fetch = [&](int i) {  // pair i of this warp into its stage; i rises by one a call
     if (i > 0 && (i & 31) == 0) {
       ids = ids_next;
-      ids_next = load_ids(i + 32);
+      ids_next = load_ids(i + 32, 0);
+      if (one) ids1 = load_ids(i, 1);
     }
-    const int id = __shfl_sync(0xffffffffu, ids, i & 31);
+    const int id = __shfl_sync(0xffffffffu, ids, i & 31), id1 = one ? __shfl_sync(0xffffffffu, ids1, i & 31) : 0;
     if (lane == 0 && i < mine) {
-      const int b = (b0 + warp + i * KT_WARPS) % g.nblk, s = i % KT_STAGES;
-      pb_mbar_arrive_tx(&full[warp][s], BB);
-      pb_bulk_g2s(ring + s * BB, a.pages + (int64_t)id * g.page_bytes + ((int64_t)kvh * g.nblk + b) * BB, BB, &full[warp][s]);
+      const int b = first_block(i), n = min(2, b1 - b);
+      uint64_t* bar = &full[warp][i % STAGES];
+      unsigned char* dst = ring + (i % STAGES) * 2 * BB;
+      const uint8_t* src = a.pages + (int64_t)id * g.page_bytes + ((int64_t)kvh * g.nblk + (b & (g.nblk - 1))) * BB;
+      pb_mbar_arrive_tx(bar, n * BB);
+      pb_bulk_g2s(dst, src, one ? BB : n * BB, bar);
+      if (one && n == 2) pb_bulk_g2s(dst + BB, a.pages + (int64_t)id1 * g.page_bytes + (int64_t)kvh * BB, BB, bar);
     }
   };
 #pragma unroll 1
-  for (int i = 0; i < KT_STAGES; ++i) fetch(i);
+  for (int i = 0; i < STAGES; ++i) fetch(i);
 
   // Q: x * 2^-e of the row's largest, A fragments in the tiles' order
   uint32_t qa[NT][2][4];
@@ -533,84 +545,105 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : 2) k_kv8_attn(k
 
   int i = 0;
   for (; i < mine; ++i) {
-    const int st = i % KT_STAGES;
-    if (!__all_sync(0xffffffffu, pb_mbar_wait(&full[warp][st], (i / KT_STAGES) & 1, a.err))) break;
-    const unsigned char* blk = ring + st * BB;
-    const int es = *reinterpret_cast<const uint16_t*>(blk + 32 * HD);
-    const int ke = (int8_t)(es & 0xFF), ve = (int8_t)(es >> 8);
-    float s[2][4];
+    const int st = i % STAGES;
+    if (!__all_sync(0xffffffffu, pb_mbar_wait(&full[warp][st], (i / STAGES) & 1, a.err))) break;
+    const unsigned char* blk = ring + st * 2 * BB;
+    const bool two = first_block(i) + 1 < b1;
+    const int tok0 = first_block(i) * PB_KV8_BLOCK;
+    float s[4][4];  // 8 tokens each
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int x = 0; x < 4; ++x) s[j][x] = 0.0f;
+    auto scores = [&](const unsigned char* bk, float (&sa)[4], float (&sb)[4]) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const uint4 w = reinterpret_cast<const uint4*>(blk + n * 512)[lane];
-      uint32_t b0_, b1_;
-      kt_codes<CODE>(w.x, b0_, b1_);
-      kt_mma(s[0], qa[n][0][0], qa[n][0][1], qa[n][0][2], qa[n][0][3], b0_, b1_);
-      kt_codes<CODE>(w.z, b0_, b1_);
-      kt_mma(s[1], qa[n][0][0], qa[n][0][1], qa[n][0][2], qa[n][0][3], b0_, b1_);
-      kt_codes<CODE>(w.y, b0_, b1_);
-      kt_mma(s[0], qa[n][1][0], qa[n][1][1], qa[n][1][2], qa[n][1][3], b0_, b1_);
-      kt_codes<CODE>(w.w, b0_, b1_);
-      kt_mma(s[1], qa[n][1][0], qa[n][1][1], qa[n][1][2], qa[n][1][3], b0_, b1_);
+      for (int n = 0; n < NT; ++n) {
+        const uint4 w = reinterpret_cast<const uint4*>(bk + n * 512)[lane];
+        const uint32_t wa[2] = {w.x, w.y}, wb[2] = {w.z, w.w};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint32_t c0, c1;
+          kt_codes<CODE>(wa[k], c0, c1);
+          kt_mma(sa, qa[n][k][0], qa[n][k][1], qa[n][k][2], qa[n][k][3], c0, c1);
+          kt_codes<CODE>(wb[k], c0, c1);
+          kt_mma(sb, qa[n][k][0], qa[n][k][1], qa[n][k][2], qa[n][k][3], c0, c1);
+        }
+      }
+    };
+    scores(blk, s[0], s[1]);
+    int es = *reinterpret_cast<const uint16_t*>(blk + 32 * HD), es1 = 0x8080;
+    if (two) {
+      scores(blk + BB, s[2], s[3]);
+      es1 = *reinterpret_cast<const uint16_t*>(blk + BB + 32 * HD);
     }
-    const int tok0 = (b0 + warp + i * KT_WARPS) * PB_KV8_BLOCK;
-    const bool mask = tok0 + PB_KV8_BLOCK > see_min;
-    const float ks = kv8_scale(ke);
-    const float vadd = ve == KV8_E_ZERO ? -INFINITY : ve == KV8_E_NAN ? __int_as_float(0x7fc00000) : (float)ve;
-    uint32_t pa[4];
+    const bool mask = tok0 + 2 * PB_KV8_BLOCK > see_min;
+    const float ks[2] = {kv8_scale((int8_t)(es & 0xFF)), kv8_scale((int8_t)(es1 & 0xFF))};
+    float vadd[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int ve = (int8_t)((b ? es1 : es) >> 8);
+      vadd[b] = ve == KV8_E_ZERO ? -INFINITY : ve == KV8_E_NAN ? __int_as_float(0x7fc00000) : (float)ve;
+    }
+    uint32_t pa[2][4];
     float rescale[NR];
     bool any = false;
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-      const float f = qf[r] * ks;
-      float x[4];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9
+      float x[8];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9, and 16 further
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 8; ++j) {
         const float* c = s[j >> 1];
-        x[j] = (HL ? c[j & 1] + c[2 + (j & 1)] : c[2 * r + (j & 1)]) * f;
+        x[j] = (HL ? c[j & 1] + c[2 + (j & 1)] : c[2 * r + (j & 1)]) * (qf[r] * ks[j >> 2]);
       }
       if (mask) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 8; ++j)
           if (tok0 + 2 * t + (j & 1) + 8 * (j >> 1) >= see[r]) x[j] = -INFINITY;
       }
-      float bm = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-      bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 1));
-      bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
-      if (bm > m1[r] + KT_RISE) {
-        l[r] *= kt_ex2(m1[r] - bm);
-        m1[r] = bm;
-      }
+      float ba = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), bb = fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]));
+      float bm = fmaxf(ba, bb), bv = fmaxf(ba + vadd[0], bb + vadd[1]);
+      // the references move when a score passes them by 2^8: looked at by the quad only where a lane of the warp saw one
       rescale[r] = 1.0f;
-      const float bv = bm + vadd;
-      if (bv > m2[r] + KT_RISE) {
-        rescale[r] = kt_ex2(m2[r] - bv);
-        m2[r] = bv;
+      if (__any_sync(0xffffffffu, bm > m1[r] + KT_RISE || bv > m2[r] + KT_RISE)) {
+        bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 1));
+        bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
+        bv = fmaxf(bv, __shfl_xor_sync(0xffffffffu, bv, 1));
+        bv = fmaxf(bv, __shfl_xor_sync(0xffffffffu, bv, 2));
+        if (bm > m1[r] + KT_RISE) {
+          l[r] *= kt_ex2(m1[r] - bm);
+          m1[r] = bm;
+        }
+        if (bv > m2[r] + KT_RISE) {
+          rescale[r] = kt_ex2(m2[r] - bv);
+          m2[r] = bv;
+        }
         any = true;
       }
-      float p[4];
-      const float off = vadd + (KT_BIAS - m2[r]);
+      float p[8];
+      const float off[2] = {vadd[0] + (KT_BIAS - m2[r]), vadd[1] + (KT_BIAS - m2[r])};
+      float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        l[r] += kt_ex2(x[j] - m1[r]);
-        p[j] = kt_ex2(x[j] + off);
+      for (int j = 0; j < 8; ++j) {
+        sum[j & 1] += kt_ex2(x[j] - m1[r]);
+        p[j] = kt_ex2(x[j] + off[j >> 2]);
       }
+      l[r] += sum[0] + sum[1];
       if (mask) {  // nothing of a masked token, whatever the block's scale
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 8; ++j)
           if (tok0 + 2 * t + (j & 1) + 8 * (j >> 1) >= see[r]) p[j] = 0.0f;
       }
-      pa[r] = kt_h2(p[0], p[1]);
-      pa[2 + r] = kt_h2(p[2], p[3]);
-      if (HL) {
-        pa[1] = kt_lo2(p[0], p[1], pa[0]);
-        pa[3] = kt_lo2(p[2], p[3], pa[2]);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        pa[b][r] = kt_h2(p[4 * b], p[4 * b + 1]);
+        pa[b][2 + r] = kt_h2(p[4 * b + 2], p[4 * b + 3]);
+        if (HL) {
+          pa[b][1] = kt_lo2(p[4 * b], p[4 * b + 1], pa[b][0]);
+          pa[b][3] = kt_lo2(p[4 * b + 2], p[4 * b + 3], pa[b][2]);
+        }
       }
     }
-    if (__any_sync(0xffffffffu, any)) {
+    if (any) {  // the same on every lane
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -618,24 +651,28 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : 2) k_kv8_attn(k
 #pragma unroll
           for (int x = 0; x < 4; ++x) o[n][j][x] *= rescale[HL ? 0 : x >> 1];
     }
+    auto values = [&](const unsigned char* bk, const uint32_t (&p)[4]) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const uint4 w = reinterpret_cast<const uint4*>(blk + 16 * HD + n * 512)[lane];
-      const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+      for (int n = 0; n < NT; ++n) {
+        const uint4 w = reinterpret_cast<const uint4*>(bk + 16 * HD + n * 512)[lane];
+        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t b0_, b1_;
-        kt_codes<CODE>(ww[j], b0_, b1_);
-        kt_mma(o[n][j], pa[0], pa[1], pa[2], pa[3], b0_, b1_);
+        for (int j = 0; j < 4; ++j) {
+          uint32_t c0, c1;
+          kt_codes<CODE>(ww[j], c0, c1);
+          kt_mma(o[n][j], p[0], p[1], p[2], p[3], c0, c1);
+        }
       }
-    }
+    };
+    values(blk, pa[0]);
+    if (two) values(blk + BB, pa[1]);
     // every lane's reads of the stage come before the copy that refills it
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
-    fetch(i + KT_STAGES);
+    fetch(i + STAGES);
   }
-  for (int k = i; k < mine && k < i + KT_STAGES; ++k)  // a wait gave up: the copies on their way land first
-    pb_mbar_wait(&full[warp][k % KT_STAGES], (k / KT_STAGES) & 1, a.err);
+  for (int k = i; k < mine && k < i + STAGES; ++k)  // a wait gave up: the copies on their way land first
+    pb_mbar_wait(&full[warp][k % STAGES], (k / STAGES) & 1, a.err);
 #pragma unroll
   for (int r = 0; r < NR; ++r) {  // l is each lane's own tokens' sum
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -792,6 +829,7 @@ extern "C" int pb_kv8_create(pb_ctx* ctx, const pb_kv8_config* c, pb_kv8** out) 
   cudaError_t e = cudaMalloc(&kv->freqs, sizeof freqs);
   // at most 2 * slots chunks of split sequences (a split one has more than C blocks, so no more than 2 blocks / C chunks)
   kv->slots = 4 * ctx->sm_count;
+  if (const char* ev = getenv("KT_SLOTS")) kv->slots = atoi(ev) * ctx->sm_count;
   const size_t parts = 2 * (size_t)kv->slots + g.n_kv;
   if (e == cudaSuccess) e = cudaMalloc(&kv->ws, parts * 16 * (g.hd + 4) * sizeof(float));
   if (e == cudaSuccess) e = cudaMalloc(&kv->cnt, parts * sizeof(unsigned int));
