@@ -234,32 +234,38 @@ k_kv8_read(kv8_geo g, uint8_t* pages, const int* __restrict__ starts, const int*
 // ============================================================================
 
 // The rows of a sequence that share a kv head (its new tokens x the head's
-// group) are taken TR at a time: a row tile.  The work of all row tiles and kv
-// heads, counted in 16-token blocks, is cut into chunks of at most C blocks of
-// one (sequence, row tile, head), C chosen so that about `slots` CTAs share it
-// evenly whatever the lengths; every CTA finds its own chunk from the lengths
-// on the device (kt_plan), so a recorded graph follows them.  A warp takes
-// every KT_WARPS-th pair of the chunk's blocks through a ring of its own, one
-// bulk copy a pair (a block's K codes, V codes and scales are contiguous, and
-// so are a page's blocks of a head), and keeps running
-// maximum, sum and output of its rows; warps join in shared memory, chunks in
-// the workspace, where the last CTA to arrive adds them in order.
+// group) are taken TR at a time: a row tile.  A (sequence, kv head, row tile)
+// is a group; its work is counted in pairs of 16-token blocks, and KT_COST pairs
+// more for what a group costs by itself (measured 4 us against 0.6 us a pair).
+// All groups, one after the other, are cut into equal ranges, one for each CTA
+// of a single wave, whatever the lengths: a CTA walks its range group by group,
+// finds its place from the lengths on the device (kt_plan; so a recorded graph
+// follows them), and writes what is only part of a group to the workspace,
+// where the last CTA of the group to arrive adds the parts in order.
+// A warp takes every KT_WARPS-th pair through a ring of its own, one bulk copy
+// a pair (a block's K codes, V codes and scales are contiguous, and so are a
+// page's blocks of a head), and keeps running maximum, sum and output of its
+// rows; the warps join in shared memory.
 //
-// Both products run as m16n8k16 f16 products straight from the codes (every
-// code is exact in f16): S = Q K^T with rows = queries, columns = tokens, whose
-// accumulators are the A operand of O = P V.  A tile of 8 rows (TR = 8) uses
-// the operand's other 8 rows for what f16 leaves of a value: rows 0-7 hold
-// hi = f16(x), rows 8-15 lo = f16(x - hi), and the two accumulators of a row
-// meet in one thread.  Queries and probabilities then keep 22 bits at no extra
-// product.  TR = 16 takes 16-bit queries (exact in f16 after a power of two
-// per row) and rounds p once, half a step of f16.
+// Rows of the products' M = 16 that a tile of 8 rows (TR = 8) leaves free hold
+// more bits of the same 8 rows; the accumulators of a row meet in one thread.
+// O = P V: m16n8k16 in f16 straight from the codes (every code is exact in
+// f16); S's accumulators, rows = queries and columns = tokens, are its A
+// operand.  TR = 8: rows 0-7 hold hi = f16(p), rows 8-15 lo = f16(p - hi), 22
+// bits at no extra product; TR = 16 rounds p once, half a step of f16.
+// S = Q K^T with int8 codes: m16n8k32 on the codes as they are, q in signed
+// byte digits q = f (i0 + i1 / 254 + i2 / 254^2), f from the row's largest, so
+// the products and sums are exact: three digits (24 bits) for TR = 8, two (16
+// bits below the row's largest) for TR = 16, whose rows have 16-bit queries.
+// With e4m3 codes: m16n8k16 in f16 with q = hi + lo (TR = 8), or q in f16 after
+// a power of two (TR = 16, exact).
 //
 // Scales: S's columns times 2^ke of the block.  V's 2^ve is put into the
 // exponent, p' = 2^(s + ve - m2), with a running reference m2 of s + ve of its
 // own, so p' uses f16's range whatever V's scales; the sum l runs beside it
 // over 2^(s - m1).  out = O / l * 2^(m2 - m1).
 constexpr int KT_WARPS = 4;
-constexpr int KT_STEP = 2 * KT_WARPS;  // blocks of one round of a CTA's warps: chunks are multiples of it
+constexpr int KT_COST = 6;
 __host__ __device__ constexpr int kt_stages(int hd) { return hd <= 64 ? 4 : 2; }
 constexpr float KT_RISE = 8.0f, KT_BIAS = 6.0f;  // p' <= 2^(8 + 6)
 constexpr float KT_LOW = -1e30f;
@@ -269,87 +275,76 @@ struct kt_args {
   const void* q;
   void* out;
   const int *starts, *lens, *table;
-  int type, ldq, ldo, n_heads, group, ld_table, n_seqs, n_rows, slots;
-  float scale;  // times log2(e)
-  float* ws;
-  unsigned int* cnt;
+  int type, ldq, ldo, n_heads, group, ld_table, n_seqs, n_rows;
+  float scale;        // times log2(e)
+  float* ws;          // parts: 2 a CTA, [TR][HD] and {m1, m2, l, -} [TR]
+  unsigned int* cnt;  // arrivals by a group's first part, zero between calls
   int* err;
 };
 
-struct kt_item {
-  int seq, rt, chunk, chunks, slot0, C;  // slot0: the first chunk's number among the split ones (of one kv head)
-};
-
-// A sequence's rows and blocks; a bad one has no rows and raises the error word.
-__device__ __forceinline__ void kt_seq(const kv8_geo& g, const kt_args& a, int tr, int s, int& rts, int& blocks) {
+// A sequence's row tiles and the pairs of each (at least one, so that rows that
+// see nothing are written too); a bad sequence has no tiles and raises the
+// error word.
+__device__ __forceinline__ void kt_seq(const kv8_geo& g, const kt_args& a, int tr, int s, int& rts, int& pairs) {
   const int lo = a.starts[s], hi = a.starts[s + 1], len = a.lens[s];
-  rts = blocks = 0;
+  rts = 0, pairs = 1;
   if (lo < 0 || hi < lo || hi > a.n_rows || len < 0 || len > (int64_t)a.ld_table * g.page) {
     pb_raise(a.err, PB_DEVERR_BOUNDS);
     return;
   }
   rts = (int)(((int64_t)(hi - lo) * a.group + tr - 1) / tr);
-  blocks = rts ? (len + PB_KV8_BLOCK - 1) / PB_KV8_BLOCK : 0;
+  pairs = max(1, (int)(((int64_t)len + 2 * PB_KV8_BLOCK - 1) / (2 * PB_KV8_BLOCK)));
 }
 
-// The chunk number `item` (of one kv head).  Every thread calls it.
-__device__ __forceinline__ bool kt_plan(const kv8_geo& g, const kt_args& a, int tr, int item, kt_item& it) {
+struct kt_range {
+  long long lo, hi, per, base;  // the CTA's units [lo, hi) of all; per: units a CTA; base: the first unit of sequence seq
+  int seq, rts, pairs;          // the sequence that holds unit lo
+};
+
+// This CTA's range.  Every thread calls it; false: nothing to do.
+__device__ __forceinline__ bool kt_plan(const kv8_geo& g, const kt_args& a, int tr, kt_range& rg) {
   constexpr int T = KT_WARPS * 32;
   __shared__ long long wsum[KT_WARPS];
-  __shared__ int isum[KT_WARPS][2];
-  __shared__ kt_item found;
+  __shared__ kt_range found;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int per = (a.n_seqs + T - 1) / T, s0 = min(a.n_seqs, tid * per), s1 = min(a.n_seqs, s0 + per);
-  int rts = 0, blocks = 0;  // of sequence s0, all there is for up to T sequences
-  long long w = 0;
+  const int per_t = (a.n_seqs + T - 1) / T, s0 = min(a.n_seqs, tid * per_t), s1 = min(a.n_seqs, s0 + per_t);
+  int rts = 0, pairs = 1;  // of sequence s0, all there is for up to T sequences
+  long long mine = 0;
   for (int s = s1 - 1; s >= s0; --s) {
-    kt_seq(g, a, tr, s, rts, blocks);
-    w += (long long)rts * blocks;
+    kt_seq(g, a, tr, s, rts, pairs);
+    mine += (long long)rts * g.n_kv * (pairs + KT_COST);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-  if (lane == 0) wsum[warp] = w;
-  if (tid == 0) found.seq = -1;
-  __syncthreads();
-  w = 0;
-#pragma unroll
-  for (int i = 0; i < KT_WARPS; ++i) w += wsum[i];
-  long long c = (w * g.n_kv + a.slots - 1) / a.slots;
-  c = c < KT_STEP ? KT_STEP : (c + KT_STEP - 1) / KT_STEP * KT_STEP;
-  const int C = c > (1 << 28) ? 1 << 28 : (int)c;
-  int mine = 0, split = 0;
-  for (int s = s1 - 1; s >= s0; --s) {
-    if (per > 1) kt_seq(g, a, tr, s, rts, blocks);
-    const int n = blocks > C ? (blocks + C - 1) / C : 1;
-    mine += rts * n;
-    split += n > 1 ? rts * n : 0;
-  }
-  int before = mine, sbefore = split;
+  long long before = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, before, o), y = __shfl_up_sync(0xffffffffu, sbefore, o);
-    if (lane >= o) before += x, sbefore += y;
+    const long long x = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += x;
   }
-  if (lane == 31) isum[warp][0] = before, isum[warp][1] = sbefore;
+  if (lane == 31) wsum[warp] = before;
   __syncthreads();
-  before -= mine, sbefore -= split;
-  for (int i = 0; i < warp; ++i) before += isum[i][0], sbefore += isum[i][1];
-  if (item >= before && item < before + mine) {
-    for (int s = s0; s < s1; ++s) {
-      if (per > 1) kt_seq(g, a, tr, s, rts, blocks);
-      const int n = blocks > C ? (blocks + C - 1) / C : 1;
-      if (item < before + rts * n) {
-        const int x = item - before;
-        found = {s, x / n, x % n, n, sbefore + x / n * n, C};
+  long long all = 0;
+  before -= mine;
+#pragma unroll
+  for (int i = 0; i < KT_WARPS; ++i) {
+    if (i < warp) before += wsum[i];
+    all += wsum[i];
+  }
+  const long long per = max((all + gridDim.x - 1) / gridDim.x, (long long)KT_WARPS), lo = per * blockIdx.x;
+  if (lo >= all) return false;  // the same on every thread
+  if (lo >= before && lo < before + mine) {
+    for (int s = s0;; ++s) {
+      if (per_t > 1) kt_seq(g, a, tr, s, rts, pairs);
+      const long long n = (long long)rts * g.n_kv * (pairs + KT_COST);
+      if (lo < before + n) {
+        found = {lo, min(all, lo + per), per, before, s, rts, pairs};
         break;
       }
-      before += rts * n;
-      sbefore += n > 1 ? rts * n : 0;
+      before += n;
     }
   }
   __syncthreads();
-  it = found;
-  return it.seq >= 0;
+  rg = found;
+  return true;
 }
 
 __device__ __forceinline__ float kt_ex2(float x) {
@@ -393,29 +388,29 @@ __device__ __forceinline__ void kt_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// O and {m1, m2, l} of n parts of a row, added in order; part i's output at
-// po + i * so, its {m1, m2, l} at pm + i * sm.  L2: written by other SMs.
-template <bool L2>
-__device__ __forceinline__ void kt_join(const float* po, size_t so, const float* pm, size_t sm, int n, float4& ov, float4& mv) {
-  auto ld = [](const float* p) {
-    return L2 ? __ldcg(reinterpret_cast<const float4*>(p)) : *reinterpret_cast<const float4*>(p);
-  };
-  float a1 = KT_LOW, a2 = KT_LOW;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const float4 m = ld(pm + i * sm);
-    a1 = fmaxf(a1, m.x), a2 = fmaxf(a2, m.y);
+// Four values of a row's O under the reference m2, the row's sum l under m1.
+struct kt_sum {
+  float4 o = {0, 0, 0, 0};
+  float m1 = KT_LOW, m2 = KT_LOW, l = 0.0f;
+  __device__ __forceinline__ void add(const float4& v, const float4& m) {
+    const float n1 = fmaxf(m1, m.x), n2 = fmaxf(m2, m.y);
+    const float f1 = kt_ex2(m1 - n1), g1 = kt_ex2(m.x - n1), f2 = kt_ex2(m2 - n2), g2 = kt_ex2(m.y - n2);
+    l = l * f1 + m.z * g1;
+    o.x = o.x * f2 + v.x * g2, o.y = o.y * f2 + v.y * g2, o.z = o.z * f2 + v.z * g2, o.w = o.w * f2 + v.w * g2;
+    m1 = n1, m2 = n2;
   }
-  ov = make_float4(0, 0, 0, 0);
-  float ll = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const float4 m = ld(pm + i * sm), x = ld(po + i * so);
-    const float f = kt_ex2(m.y - a2);
-    ll += m.z * kt_ex2(m.x - a1);
-    ov.x += x.x * f, ov.y += x.y * f, ov.z += x.z * f, ov.w += x.w * f;
+};
+// out of a row's four values at d: O / l * 2^(m2 - m1)
+__device__ __forceinline__ void kt_finish(const kv8_geo& g, const kt_args& a, int row0, int rows, int len, int kvh, int rho,
+                                          int d, const kt_sum& s) {
+  const int tok = rho / a.group, h = kvh * a.group + rho % a.group;
+  float y[4] = {0, 0, 0, 0};
+  if (len - rows / a.group + tok >= 0) {  // the row sees a key
+    // 2^up in two halves: it may pass f32's range where the row's values do not
+    const float f = 1.0f / s.l, u0 = kt_ex2(0.5f * (s.m2 - s.m1 - KT_BIAS));
+    y[0] = s.o.x * f * u0 * u0, y[1] = s.o.y * f * u0 * u0, y[2] = s.o.z * f * u0 * u0, y[3] = s.o.w * f * u0 * u0;
   }
-  mv = make_float4(a1, a2, ll, 0.0f);
+  kv8_store(a.out, a.type, (int64_t)(row0 + tok) * a.ldo + h * g.hd + d, y);
 }
 
 static size_t kt_smem(int hd) {
@@ -423,40 +418,73 @@ static size_t kt_smem(int hd) {
   return ring > join ? ring : join;
 }
 
+__device__ __forceinline__ void kt_mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+               "{%0, %1, %2, %3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// a bounded wait whose first look costs no clock
+__device__ __forceinline__ bool kt_wait(uint64_t* bar, uint32_t parity, int* err) {
+  uint32_t ok;
+  asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+               : "=r"(ok)
+               : "r"(pb_smem_addr(bar)), "r"(parity)
+               : "memory");
+  return ok || pb_mbar_wait(bar, parity, err);
+}
+
 template <int HD, int CODE, int TR>
-__global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : 2) k_kv8_attn(kv8_geo g, kt_args a) {
+__global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 : 1) k_kv8_attn(kv8_geo g, kt_args a) {
   constexpr int NT = HD / 32, BB = 32 * HD + 16, STAGES = kt_stages(HD);
   constexpr bool HL = TR == 8;
-  constexpr int NR = HL ? 1 : 2;  // rows of the tile in a thread: gq, and gq + 8
+  constexpr int SLOT = TR * (HD + 4);  // floats of a part: O [TR][HD], {m1, m2, l, -} [TR]
+  constexpr int NR = HL ? 1 : 2;       // rows of the tile in a thread: gq, and gq + 8
   extern __shared__ __align__(16) unsigned char kt_raw[];
   __shared__ uint64_t full[KT_WARPS][STAGES];
+  __shared__ uint64_t part_bar;
   __shared__ unsigned int last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
   if (lane == 0) {
     for (int s = 0; s < STAGES; ++s) pb_mbar_init(&full[warp][s], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (tid == 0) pb_mbar_init(&part_bar, 1);
   pb_pdl_trigger();
   pb_pdl_wait();
-  kt_item it;
-  const int kvh = blockIdx.x % g.n_kv;
-  if (!kt_plan(g, a, TR, blockIdx.x / g.n_kv, it)) return;
-  const int row0 = a.starts[it.seq], nq = a.starts[it.seq + 1] - row0, len = a.lens[it.seq];
-  const int rows = nq * a.group;
-  const int b0 = it.chunk * it.C, b1 = min((len + PB_KV8_BLOCK - 1) / PB_KV8_BLOCK, b0 + it.C);
-  // this warp's pairs: the blocks b0 + 2 (warp + i KT_WARPS) and the next one
-  const int np = (b1 - b0 + 1) >> 1, mine = np > warp ? (np - 1 - warp) / KT_WARPS + 1 : 0;
+  kt_range rg;
+  if (!kt_plan(g, a, TR, rg)) return;
   unsigned char* ring = kt_raw + (size_t)warp * STAGES * 2 * BB;
-  const int* trow = a.table + (int64_t)it.seq * a.ld_table;
   const int nblk_log2 = 31 - __clz(g.nblk);
-  auto first_block = [&](int i) { return b0 + 2 * (warp + i * KT_WARPS); };
+  int used = 0;              // pairs that this warp has been through: its ring's place
+  uint32_t part_phase = 0;   // of part_bar
+  for (long long u = rg.lo; u < rg.hi;) {
+  {
+    long long n;
+    while (u >= rg.base + (n = (long long)rg.rts * g.n_kv * (rg.pairs + KT_COST))) {
+      rg.base += n;
+      kt_seq(g, a, TR, ++rg.seq, rg.rts, rg.pairs);
+    }
+  }
+  const int units = rg.pairs + KT_COST, idx = (int)((u - rg.base) / units), kvh = idx / rg.rts, rho0 = idx % rg.rts * TR;
+  const long long u0 = rg.base + (long long)idx * units;  // the group's first unit: its pairs, then its cost
+  const int p0 = (int)(u - u0), p1 = (int)min((long long)rg.pairs, rg.hi - u0);
+  const bool begins = u == u0, at_lo = u == rg.lo;
+  u = u0 + units;
+  if (p0 >= rg.pairs) continue;
+  const int row0 = a.starts[rg.seq], rows = (a.starts[rg.seq + 1] - row0) * a.group, nq = rows / a.group, len = a.lens[rg.seq];
+  const int blocks = (len + PB_KV8_BLOCK - 1) / PB_KV8_BLOCK, live = min(TR, rows - rho0);
 
-  // page ids of 32 iterations, a lane each; a bad one raises the error word and
-  // reads page 0.  x: the pair's block, which is in a page of its own where a
-  // page is one block.
+  // ---- the copies, ahead of the work: this warp's pairs p0 + warp + i KT_WARPS --
+  const int mine = p1 - p0 > warp ? (p1 - p0 - 1 - warp) / KT_WARPS + 1 : 0;
+  const int* trow = a.table + (int64_t)rg.seq * a.ld_table;
+  auto first_block = [&](int i) { return 2 * (p0 + warp + i * KT_WARPS); };
+  // page ids of 32 pairs, a lane each; a bad one raises the error word and reads
+  // page 0.  x: the pair's block, in a page of its own where a page is one block.
   auto load_ids = [&](int i0, int x) {
     const int i = i0 + lane;
-    if (i >= mine || first_block(i) + x >= b1) return 0;
+    if (i >= mine || first_block(i) + x >= blocks) return 0;
     const int id = trow[(first_block(i) + x) >> nblk_log2];
     if (id < 0 || id >= g.n_pages) {
       pb_raise(a.err, PB_DEVERR_BOUNDS);
@@ -464,44 +492,47 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : 2) k_kv8_attn(k
     }
     return id;
   };
-  const bool one = g.nblk == 1;
-  int ids = load_ids(0, 0), ids_next = load_ids(32, 0), ids1 = one ? load_ids(0, 1) : 0;
+  int ids = load_ids(0, 0), ids_next = load_ids(32, 0), ids1 = g.nblk == 1 ? load_ids(0, 1) : 0;
+  const uint8_t* head = a.pages + (int64_t)kvh * g.nblk * BB;
   auto fetch = [&](int i) {  // pair i of this warp into its stage; i rises by one a call
+    if (i >= mine) return;
     if (i > 0 && (i & 31) == 0) {
       ids = ids_next;
       ids_next = load_ids(i + 32, 0);
-      if (one) ids1 = load_ids(i, 1);
+      if (g.nblk == 1) ids1 = load_ids(i, 1);
     }
-    const int id = __shfl_sync(0xffffffffu, ids, i & 31), id1 = one ? __shfl_sync(0xffffffffu, ids1, i & 31) : 0;
-    if (lane == 0 && i < mine) {
-      const int b = first_block(i), n = min(2, b1 - b);
-      uint64_t* bar = &full[warp][i % STAGES];
-      unsigned char* dst = ring + (i % STAGES) * 2 * BB;
-      const uint8_t* src = a.pages + (int64_t)id * g.page_bytes + ((int64_t)kvh * g.nblk + (b & (g.nblk - 1))) * BB;
+    const int id = __shfl_sync(0xffffffffu, ids, i & 31), id1 = __shfl_sync(0xffffffffu, ids1, i & 31);
+    if (lane == 0) {
+      const int b = first_block(i), n = max(0, min(2, blocks - b)), st = (used + i) % STAGES;
+      uint64_t* bar = &full[warp][st];
+      unsigned char* dst = ring + st * 2 * BB;
+      const uint8_t* src = head + (int64_t)id * g.page_bytes + (b & (g.nblk - 1)) * BB;
       pb_mbar_arrive_tx(bar, n * BB);
-      pb_bulk_g2s(dst, src, one ? BB : n * BB, bar);
-      if (one && n == 2) pb_bulk_g2s(dst + BB, a.pages + (int64_t)id1 * g.page_bytes + (int64_t)kvh * BB, BB, bar);
+      if (n > 0) pb_bulk_g2s(dst, src, (g.nblk == 1 ? 1 : n) * BB, bar);
+      if (n > 1 && g.nblk == 1) pb_bulk_g2s(dst + BB, head + (int64_t)id1 * g.page_bytes, BB, bar);
     }
   };
 #pragma unroll 1
   for (int i = 0; i < STAGES; ++i) fetch(i);
 
-  // Q: x * 2^-e of the row's largest, A fragments in the tiles' order
-  uint32_t qa[NT][2][4];
+  // Q as A fragments in the tiles' order, scaled by the row's largest; qf undoes it
+  constexpr bool DIGITS = CODE == PB_KV8_INT8;
+  constexpr int QN = DIGITS && HL ? 6 : 8;  // registers a tile
+  uint32_t qa[NT][QN];
   float qf[NR];
   int see[NR];  // keys the row sees
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
-    const int rho = it.rt * TR + gq + 8 * r;
-    const bool live = rho < rows;
-    const int tok = live ? rho / a.group : 0, h = kvh * a.group + (live ? rho % a.group : 0);
-    see[r] = live ? max(0, len - nq + tok + 1) : 0;
+    const int rho = rho0 + gq + 8 * r;
+    const bool on = rho < rows;
+    const int tok = on ? rho / a.group : 0, h = kvh * a.group + (on ? rho % a.group : 0);
+    see[r] = on ? max(0, len - nq + tok + 1) : 0;
     const int64_t at = (int64_t)(row0 + tok) * a.ldq + h * HD + 8 * t;
     float x[NT][8];
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      if (live) {
+      if (on) {
         kv8_load(a.q, a.type, at + 32 * i, x[i]);
       } else {
 #pragma unroll
@@ -512,26 +543,46 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : 2) k_kv8_attn(k
     }
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    // 2^-e brings the largest into [1, 2); a subnormal or non-finite row stays as it is
-    int e = (int)(m >> 23) - 127;
-    if (e < -126 || e > 126) e = 0;
-    const float inv = kv8_pow2(-e);
-    qf[r] = a.scale * kv8_pow2(e);
+    // 2^-e brings the largest into [1/2, 1); a row below 2^-118 counts as zeros, one that is not finite as NaN
+    const int e = (int)(m >> 23) - 126;
+    const bool nan = m >= 0x7F800000u, tiny = e < -118;
+    const float inv = nan || tiny ? 0.0f : e > 126 ? kv8_pow2(-126) * kv8_pow2(126 - e) : kv8_pow2(-e), up = nan ? __int_as_float(0x7fc00000) : tiny ? 0.0f : 1.0f;
+    qf[r] = a.scale * (up * kv8_pow2(max(-126, min(127, e)))) * (DIGITS ? 1.0f / 127.0f : 1.0f);
+    if (e == 128) qf[r] *= 2.0f;  // 2^128 in two steps
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const float y0 = x[i][4 * s] * inv, y1 = x[i][4 * s + 1] * inv, y2 = x[i][4 * s + 2] * inv, y3 = x[i][4 * s + 3] * inv;
-        qa[i][s][r] = kt_h2(y0, y1);
-        qa[i][s][2 + r] = kt_h2(y2, y3);
-        if (HL) {
-          qa[i][s][1] = kt_lo2(y0, y1, qa[i][s][0]);
-          qa[i][s][3] = kt_lo2(y2, y3, qa[i][s][2]);
+      for (int s = 0; s < 2; ++s) {  // values 4s .. 4s + 3 of the lane's 8
+        float y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = inv == 0.0f ? 0.0f : x[i][4 * s + j] * inv;
+        if constexpr (DIGITS) {
+          uint32_t d0 = 0, d1 = 0, d2 = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float v = y[j] * 127.0f;
+            const int i0 = __float2int_rn(v);
+            const float r1 = (v - (float)i0) * 254.0f;
+            const int i1 = __float2int_rn(r1), i2 = __float2int_rn((r1 - (float)i1) * 254.0f);
+            d0 |= (uint32_t)(i0 & 0xFF) << (8 * j);
+            d1 |= (uint32_t)(i1 & 0xFF) << (8 * j);
+            d2 |= (uint32_t)(i2 & 0xFF) << (8 * j);
+          }
+          if (HL) qa[i][2 * s] = d0, qa[i][2 * s + 1] = d1, qa[i][4 + s] = d2;
+          else qa[i][2 * s + r] = d0, qa[i][(QN == 8 ? 4 : 0) + 2 * s + r] = d1;
+        } else {
+          uint32_t* q4 = &qa[i][(QN == 8 ? 4 : 0) * s];
+          q4[r] = kt_h2(y[0], y[1]);
+          q4[2 + r] = kt_h2(y[2], y[3]);
+          if (HL) {
+            q4[1] = kt_lo2(y[0], y[1], q4[0]);
+            q4[3] = kt_lo2(y[2], y[3], q4[2]);
+          }
         }
       }
   }
   // the fewest keys a live row of the tile sees: blocks up to there need no mask
-  const int see_min = max(0, len - nq + it.rt * TR / a.group + 1);
+  const int see_min = max(0, len - nq + rho0 / a.group + 1);
 
   float o[NT][4][4], m1[NR], m2[NR], l[NR];
 #pragma unroll
@@ -545,62 +596,103 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : 2) k_kv8_attn(k
 
   int i = 0;
   for (; i < mine; ++i) {
-    const int st = i % STAGES;
-    if (!__all_sync(0xffffffffu, pb_mbar_wait(&full[warp][st], (i / STAGES) & 1, a.err))) break;
+    const int st = (used + i) % STAGES;
+    if (!__all_sync(0xffffffffu, kt_wait(&full[warp][st], ((used + i) / STAGES) & 1, a.err))) break;
     const unsigned char* blk = ring + st * 2 * BB;
-    const bool two = first_block(i) + 1 < b1;
-    const int tok0 = first_block(i) * PB_KV8_BLOCK;
-    float s[4][4];  // 8 tokens each
+    const int b = first_block(i), tok0 = b * PB_KV8_BLOCK;
+    const bool one = b < blocks, two = b + 1 < blocks;
+    // x: scores times log2(e), tokens 2t, 2t + 1, 2t + 8, 2t + 9 of a block
+    auto scores = [&](const unsigned char* bk, float ks, float (&x0)[4], float (&x1)[4]) {
+      if constexpr (DIGITS) {
+        int ca[2][4], cb[2][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) s[j][x] = 0.0f;
-    auto scores = [&](const unsigned char* bk, float (&sa)[4], float (&sb)[4]) {
+          for (int z = 0; z < 4; ++z) ca[j][z] = cb[j][z] = 0;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const uint4 w = reinterpret_cast<const uint4*>(bk + n * 512)[lane];
-        const uint32_t wa[2] = {w.x, w.y}, wb[2] = {w.z, w.w};
+        for (int n = 0; n < NT; ++n) {
+          const uint4 w = reinterpret_cast<const uint4*>(bk + n * 512)[lane];
+          const uint32_t* q = qa[n];
+          kt_mma_s8(ca[0], q[0], q[1], q[2], q[3], w.x, w.y);
+          kt_mma_s8(ca[1], q[0], q[1], q[2], q[3], w.z, w.w);
+          if (HL) {
+            kt_mma_s8(cb[0], q[4], 0u, q[5], 0u, w.x, w.y);
+            kt_mma_s8(cb[1], q[4], 0u, q[5], 0u, w.z, w.w);
+          } else {
+            kt_mma_s8(cb[0], q[4], q[5], q[QN - 2], q[QN - 1], w.x, w.y);
+            kt_mma_s8(cb[1], q[4], q[5], q[QN - 2], q[QN - 1], w.z, w.w);
+          }
+        }
+        const float f0 = qf[0] * ks, f1 = qf[NR - 1] * ks;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          uint32_t c0, c1;
-          kt_codes<CODE>(wa[k], c0, c1);
-          kt_mma(sa, qa[n][k][0], qa[n][k][1], qa[n][k][2], qa[n][k][3], c0, c1);
-          kt_codes<CODE>(wb[k], c0, c1);
-          kt_mma(sb, qa[n][k][0], qa[n][k][1], qa[n][k][2], qa[n][k][3], c0, c1);
+        for (int j = 0; j < 4; ++j) {
+          const int *c = ca[j >> 1], *d = cb[j >> 1], z = j & 1;
+          if (HL) {  // |i1 sum| * 254 + |i2 sum| stays below 2^31 (256 * 127 * 127 * 255)
+            x0[j] = __fmaf_rn((float)(c[2 + z] * 254 + d[z]), f0 * (1.0f / 64516.0f), (float)c[z] * f0);
+          } else {
+            x0[j] = __fmaf_rn((float)d[z], f0 * (1.0f / 254.0f), (float)c[z] * f0);
+            x1[j] = __fmaf_rn((float)d[2 + z], f1 * (1.0f / 254.0f), (float)c[2 + z] * f1);
+          }
+        }
+      } else {
+        float c[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int z = 0; z < 4; ++z) c[j][z] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint4 w = reinterpret_cast<const uint4*>(bk + n * 512)[lane];
+          const uint32_t wa[2] = {w.x, w.y}, wb_[2] = {w.z, w.w};
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t* q = &qa[n][(QN == 8 ? 4 : 0) * k];
+            uint32_t c0, c1;
+            kt_codes<CODE>(wa[k], c0, c1);
+            kt_mma(c[0], q[0], q[1], q[2], q[3], c0, c1);
+            kt_codes<CODE>(wb_[k], c0, c1);
+            kt_mma(c[1], q[0], q[1], q[2], q[3], c0, c1);
+          }
+        }
+        const float f0 = qf[0] * ks, f1 = qf[NR - 1] * ks;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float* y = c[j >> 1];
+          x0[j] = (HL ? y[j & 1] + y[2 + (j & 1)] : y[j & 1]) * f0;
+          if (!HL) x1[j] = y[2 + (j & 1)] * f1;
         }
       }
     };
-    scores(blk, s[0], s[1]);
-    int es = *reinterpret_cast<const uint16_t*>(blk + 32 * HD), es1 = 0x8080;
-    if (two) {
-      scores(blk + BB, s[2], s[3]);
-      es1 = *reinterpret_cast<const uint16_t*>(blk + BB + 32 * HD);
+    float x[2][2][4];  // [block][row]
+    int ve[2] = {KV8_E_ZERO, KV8_E_ZERO};
+    // log2 of V's scale where the block's values count in f16's way; the others (no values, not finite) take a way of their own
+    float vadd[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const unsigned char* bk = blk + h * BB;
+      if (h == 0 ? one : two) {
+        const int es = *reinterpret_cast<const uint16_t*>(bk + 32 * HD);
+        ve[h] = (int8_t)(es >> 8);
+        vadd[h] = ve[h] == KV8_E_ZERO ? -INFINITY : ve[h] == KV8_E_NAN ? __int_as_float(0x7fc00000) : (float)ve[h];
+        scores(bk, kv8_scale((int8_t)(es & 0xFF)), x[h][0], x[h][1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[h][0][j] = x[h][1][j] = -INFINITY;
+      }
     }
     const bool mask = tok0 + 2 * PB_KV8_BLOCK > see_min;
-    const float ks[2] = {kv8_scale((int8_t)(es & 0xFF)), kv8_scale((int8_t)(es1 & 0xFF))};
-    float vadd[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int ve = (int8_t)((b ? es1 : es) >> 8);
-      vadd[b] = ve == KV8_E_ZERO ? -INFINITY : ve == KV8_E_NAN ? __int_as_float(0x7fc00000) : (float)ve;
-    }
     uint32_t pa[2][4];
     float rescale[NR];
     bool any = false;
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-      float x[8];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9, and 16 further
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float* c = s[j >> 1];
-        x[j] = (HL ? c[j & 1] + c[2 + (j & 1)] : c[2 * r + (j & 1)]) * (qf[r] * ks[j >> 2]);
-      }
       if (mask) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (tok0 + 2 * t + (j & 1) + 8 * (j >> 1) >= see[r]) x[j] = -INFINITY;
+          if (tok0 + 2 * t + (j & 1) + 8 * (j >> 1) >= see[r]) x[j >> 2][r][j & 3] = -INFINITY;
       }
-      float ba = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), bb = fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]));
+      const float *xa = x[0][r], *xb = x[1][r];
+      const float ba = fmaxf(fmaxf(xa[0], xa[1]), fmaxf(xa[2], xa[3])), bb = fmaxf(fmaxf(xb[0], xb[1]), fmaxf(xb[2], xb[3]));
       float bm = fmaxf(ba, bb), bv = fmaxf(ba + vadd[0], bb + vadd[1]);
       // the references move when a score passes them by 2^8: looked at by the quad only where a lane of the warp saw one
       rescale[r] = 1.0f;
@@ -619,27 +711,32 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : 2) k_kv8_attn(k
         }
         any = true;
       }
-      float p[8];
-      const float off[2] = {vadd[0] + (KT_BIAS - m2[r]), vadd[1] + (KT_BIAS - m2[r])};
-      float sum[2] = {0.0f, 0.0f};
+      const float top = KT_BIAS - m2[r];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        sum[j & 1] += kt_ex2(x[j] - m1[r]);
-        p[j] = kt_ex2(x[j] + off[j >> 2]);
-      }
-      l[r] += sum[0] + sum[1];
-      if (mask) {  // nothing of a masked token, whatever the block's scale
+      for (int h = 0; h < 2; ++h) {
+        float p[4], sum = 0.0f;
+        if (ve[h] == KV8_E_ZERO || ve[h] == KV8_E_NAN) {  // p' is 0 or NaN there: the sum by itself
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (tok0 + 2 * t + (j & 1) + 8 * (j >> 1) >= see[r]) p[j] = 0.0f;
-      }
+          for (int j = 0; j < 4; ++j) {
+            sum += kt_ex2(x[h][r][j] - m1[r]);
+            p[j] = x[h][r][j] == -INFINITY ? 0.0f : kt_ex2(x[h][r][j] + (vadd[h] + top));  // -inf: masked
+          }
+          l[r] += sum;
+        } else {
+          // l's 2^(x - m1) is p' times one factor a block: V's exponents lie within 100 of each other, so p' keeps
+          // its f32 precision wherever 2^(x - m1) counts
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        pa[b][r] = kt_h2(p[4 * b], p[4 * b + 1]);
-        pa[b][2 + r] = kt_h2(p[4 * b + 2], p[4 * b + 3]);
+          for (int j = 0; j < 4; ++j) {
+            p[j] = kt_ex2(x[h][r][j] + (vadd[h] + top));
+            sum += p[j];
+          }
+          l[r] = __fmaf_rn(sum, kt_ex2(-(vadd[h] + top) - m1[r]), l[r]);
+        }
+        pa[h][r] = kt_h2(p[0], p[1]);
+        pa[h][2 + r] = kt_h2(p[2], p[3]);
         if (HL) {
-          pa[b][1] = kt_lo2(p[4 * b], p[4 * b + 1], pa[b][0]);
-          pa[b][3] = kt_lo2(p[4 * b + 2], p[4 * b + 3], pa[b][2]);
+          pa[h][1] = kt_lo2(p[0], p[1], pa[h][0]);
+          pa[h][3] = kt_lo2(p[2], p[3], pa[h][2]);
         }
       }
     }
@@ -664,7 +761,7 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : 2) k_kv8_attn(k
         }
       }
     };
-    values(blk, pa[0]);
+    if (one) values(blk, pa[0]);
     if (two) values(blk + BB, pa[1]);
     // every lane's reads of the stage come before the copy that refills it
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -672,24 +769,21 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : 2) k_kv8_attn(k
     fetch(i + STAGES);
   }
   for (int k = i; k < mine && k < i + STAGES; ++k)  // a wait gave up: the copies on their way land first
-    pb_mbar_wait(&full[warp][k % STAGES], (k / STAGES) & 1, a.err);
-#pragma unroll
-  for (int r = 0; r < NR; ++r) {  // l is each lane's own tokens' sum
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-  }
+    pb_mbar_wait(&full[warp][(used + k) % STAGES], ((used + k) / STAGES) & 1, a.err);
+  used += mine;
 
-  // join the warps
+  // ---- join the warps ------------------------------------------------------------
   __syncthreads();
-  float* jo = reinterpret_cast<float*>(kt_raw);  // [KT_WARPS][TR][HD]
-  float* jm = jo + KT_WARPS * TR * HD;           // [KT_WARPS][TR][4]: m1, m2, l
+  float* jo = reinterpret_cast<float*>(kt_raw) + warp * SLOT;  // a part as in the workspace
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);  // each lane's own tokens' sum so far
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     const int row = gq + 8 * r;
-    float* d = jo + (warp * TR + row) * HD + 8 * t;
+    float* d = jo + row * HD + 8 * t;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float y[8];  // accumulator (j, c0 / c1): values j and 4 + j of the lane's 8
+      float y[8];  // accumulators (j, c0 / c1): values j and 4 + j of the lane's 8
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         y[j] = HL ? o[n][j][0] + o[n][j][2] : o[n][j][2 * r];
@@ -698,51 +792,80 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : 2) k_kv8_attn(k
       *reinterpret_cast<float4*>(d + 32 * n) = make_float4(y[0], y[1], y[2], y[3]);
       *reinterpret_cast<float4*>(d + 32 * n + 4) = make_float4(y[4], y[5], y[6], y[7]);
     }
-    if (t == 0) *reinterpret_cast<float4*>(jm + (warp * TR + row) * 4) = make_float4(m1[r], m2[r], l[r], 0.0f);
+    if (t == 0) *reinterpret_cast<float4*>(jo + TR * HD + row * 4) = make_float4(m1[r], m2[r], l[r], 0.0f);
   }
   __syncthreads();
-  const int live = min(TR, rows - it.rt * TR);
-  auto finish = [&](int row, int d, const float4& ov, const float4& mv) {
-    const int rho = it.rt * TR + row, h = kvh * a.group + rho % a.group;
-    float y[4] = {0, 0, 0, 0};
-    if (len - nq + rho / a.group >= 0) {  // the row sees a key
-      const float f = 1.0f / mv.z, up = mv.y - mv.x - KT_BIAS;
-      // 2^up in two halves: it may pass f32's range where the row's values do not
-      const float u0 = kt_ex2(0.5f * up);
-      y[0] = ov.x * f * u0 * u0, y[1] = ov.y * f * u0 * u0, y[2] = ov.z * f * u0 * u0, y[3] = ov.w * f * u0 * u0;
+  // thread's values x = tid + T j: 4 at column x % (HD / 4) of row x / (HD / 4)
+  constexpr int T = KT_WARPS * 32, COLS = HD / 4, J = (TR * COLS + T - 1) / T;
+  kt_sum acc[J];
+  auto add_parts = [&](int n) {  // n parts from shared memory
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int x = tid + T * j;
+      if (x < live * COLS) {
+        const float* p = reinterpret_cast<const float*>(kt_raw) + 4 * x;
+        for (int i = 0; i < n; ++i, p += SLOT)
+          acc[j].add(*reinterpret_cast<const float4*>(p), *reinterpret_cast<const float4*>(p - 4 * x + TR * HD + x / COLS * 4));
+      }
     }
-    kv8_store(a.out, a.type, (int64_t)(row0 + rho / a.group) * a.ldo + h * HD + d, y);
   };
-  constexpr int SLOT = TR * (HD + 4);  // floats: [TR][HD], [TR][4]
-  for (int x = tid; x < live * (HD / 4); x += KT_WARPS * 32) {
-    const int row = x / (HD / 4), d = x % (HD / 4) * 4;
-    float4 ov, mv;
-    kt_join<false>(jo + row * HD + d, (size_t)TR * HD, jm + row * 4, (size_t)TR * 4, KT_WARPS, ov, mv);
-    if (it.chunks == 1) {
-      finish(row, d, ov, mv);
-    } else {
-      float* slot = a.ws + (size_t)((it.slot0 + it.chunk) * g.n_kv + kvh) * SLOT;
-      __stcg(reinterpret_cast<float4*>(slot + row * HD + d), ov);
-      if (d == 0) __stcg(reinterpret_cast<float4*>(slot + TR * HD + row * 4), mv);
+  auto finish = [&]() {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int x = tid + T * j;
+      if (x < live * COLS) kt_finish(g, a, row0, rows, len, kvh, rho0 + x / COLS, x % COLS * 4, acc[j]);
+    }
+  };
+  add_parts(KT_WARPS);
+  // Parts of a group: a CTA has at most two, of the group it begins with (part
+  // 2 cta) and of the one it ends with (part 2 cta + 1, if that is another).
+  const int c0 = (int)(u0 / rg.per), n_parts = (int)((u0 + rg.pairs - 1) / rg.per) - c0 + 1;  // the CTAs that share the group
+  if (begins && p1 == rg.pairs) {
+    finish();
+  } else {
+    float* part = a.ws + (size_t)(2 * blockIdx.x + (at_lo ? 0 : 1)) * SLOT;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int x = tid + T * j;
+      if (x < live * COLS) {
+        __stcg(reinterpret_cast<float4*>(part + 4 * x), acc[j].o);
+        if (x % COLS == 0) __stcg(reinterpret_cast<float4*>(part + TR * HD + x / COLS * 4), make_float4(acc[j].m1, acc[j].m2, acc[j].l, 0.0f));
+      }
+    }
+    const int first_part = 2 * c0 + (u0 == c0 * rg.per ? 0 : 1);
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+      last = atomicAdd(a.cnt + first_part, 1u) == (unsigned)n_parts - 1 ? 1u : 0u;
+      if (last) a.cnt[first_part] = 0;  // for the next call
+    }
+    __syncthreads();
+    if (last) {  // all parts, by bulk copies into the ring as many at a time as it holds
+      constexpr int HOLD = (int)(KT_WARPS * STAGES * 2 * BB / (SLOT * sizeof(float)));
+      __threadfence();
+#pragma unroll
+      for (int j = 0; j < J; ++j) acc[j] = kt_sum();
+      for (int i0 = 0; i0 < n_parts; i0 += HOLD) {
+        const int n = min(HOLD, n_parts - i0);
+        if (tid == 0) {
+          asm volatile("fence.proxy.async;" ::: "memory");
+          pb_mbar_arrive_tx(&part_bar, n * SLOT * 4);
+          for (int i = 0; i < n; ++i)
+            pb_bulk_g2s(kt_raw + (size_t)i * SLOT * 4, a.ws + (size_t)(i0 + i == 0 ? first_part : 2 * (c0 + i0 + i)) * SLOT,
+                        SLOT * 4, &part_bar);
+        }
+        pb_mbar_wait(&part_bar, part_phase, a.err);
+        part_phase ^= 1;
+        add_parts(n);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
+      }
+      finish();
     }
   }
-  if (it.chunks == 1) return;
-  __threadfence();
+  // the ring, which the joins used, and `last` are free again
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncthreads();
-  if (tid == 0) {
-    unsigned int* c = a.cnt + (size_t)it.slot0 * g.n_kv + kvh;
-    last = atomicAdd(c, 1u) == (unsigned)it.chunks - 1 ? 1u : 0u;
-    if (last) *c = 0;  // for the next call
-  }
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
-  const float* slot = a.ws + (size_t)(it.slot0 * g.n_kv + kvh) * SLOT;
-  for (int x = tid; x < live * (HD / 4); x += KT_WARPS * 32) {
-    const int row = x / (HD / 4), d = x % (HD / 4) * 4;
-    float4 ov, mv;
-    kt_join<true>(slot + row * HD + d, (size_t)g.n_kv * SLOT, slot + TR * HD + row * 4, (size_t)g.n_kv * SLOT, it.chunks, ov, mv);
-    finish(row, d, ov, mv);
   }
 }
 
@@ -827,10 +950,8 @@ extern "C" int pb_kv8_create(pb_ctx* ctx, const pb_kv8_config* c, pb_kv8** out) 
   kv->ctx = ctx;
   kv->g = g;
   cudaError_t e = cudaMalloc(&kv->freqs, sizeof freqs);
-  // at most 2 * slots chunks of split sequences (a split one has more than C blocks, so no more than 2 blocks / C chunks)
-  kv->slots = 4 * ctx->sm_count;
-  if (const char* ev = getenv("KT_SLOTS")) kv->slots = atoi(ev) * ctx->sm_count;
-  const size_t parts = 2 * (size_t)kv->slots + g.n_kv;
+  kv->ctas = (g.hd <= 128 ? 3 : g.hd <= 192 ? 2 : 1) * ctx->sm_count;  // one wave of k_kv8_attn
+  const size_t parts = 2 * (size_t)kv->ctas;
   if (e == cudaSuccess) e = cudaMalloc(&kv->ws, parts * 16 * (g.hd + 4) * sizeof(float));
   if (e == cudaSuccess) e = cudaMalloc(&kv->cnt, parts * sizeof(unsigned int));
   if (e == cudaSuccess) e = cudaMemset(kv->cnt, 0, parts * sizeof(unsigned int));
@@ -949,12 +1070,9 @@ extern "C" int pb_kv8_attn(pb_kv8* kv, const void* pages_dev, int type, const vo
   // average (the products cost the same); else 16 rows, half the passes over the codes.
   const int group = n_heads / g.n_kv, tr = type == PB_TYPE_F32 || (int64_t)n_rows * group <= 8 * (int64_t)n_seqs ? 8 : 16;
   kt_args a = {static_cast<const uint8_t*>(pages_dev), q_dev, out_dev, starts_dev, lens_dev, table_dev, type, ldq, ldo,
-               n_heads, group, ld_table, n_seqs, n_rows, kv->slots, (float)(scale * 1.4426950408889634), kv->ws, kv->cnt,
-               ctx->d_err};
+               n_heads, group, ld_table, n_seqs, n_rows, (float)(scale * 1.4426950408889634), kv->ws, kv->cnt, ctx->d_err};
   if ((int64_t)n_rows * n_heads > 0x7FFFFFFF)
     return pb_set_error(ctx, PB_ERR_ARG, "pb_kv8_attn: too many rows and heads for one call");
-  const int64_t grid = ((int64_t)n_rows * group / tr + n_seqs) * g.n_kv + kv->slots + g.n_kv;
-  if (grid > 0x7FFFFFFF) return pb_set_error(ctx, PB_ERR_ARG, "pb_kv8_attn: too many rows and heads for one call");
-  return pb_launch(ctx, "k_kv8_attn", true, kt_kernel_of(g.hd, g.code, tr), dim3((unsigned)grid), dim3(KT_WARPS * 32),
+  return pb_launch(ctx, "k_kv8_attn", true, kt_kernel_of(g.hd, g.code, tr), dim3(kv->ctas), dim3(KT_WARPS * 32),
                    kt_smem(g.hd), g, a);
 }

@@ -45,11 +45,11 @@ struct pb_kv8 {
   pb_ctx* ctx = nullptr;
   kv8_geo g;
   double* freqs = nullptr;  // [rope_dim / 2] pair frequencies
-  // partial results of split sequences (pb_kv8_attn) and their arrival
-  // counters (zero between calls); fixed, so recorded graphs stay valid
+  // parts of the groups that pb_kv8_attn splits and their arrival counters (zero
+  // between calls); fixed, so recorded graphs stay valid
   float* ws = nullptr;
   unsigned int* cnt = nullptr;
-  int slots = 0;
+  int ctas = 0;  // of pb_kv8_attn
 };
 
 // The calls' device is the context's, whichever is current on the thread.
