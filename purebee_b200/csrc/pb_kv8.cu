@@ -24,34 +24,44 @@ struct kv8_append_args {
 };
 
 // 8 consecutive values of a head from d on, rotated: the pair (2i, 2i + 1) or
-// (i, i + rope_dim / 2) by the angle of index i, in double, rounded once.
-// cs: the token's {cos, sin} by index.
-__device__ __forceinline__ void kv8_load_rotated(const void* p, int type, int64_t base, int d, int rope, int rope_dim,
-                                                 const double2* cs, float (&v)[8]) {
+// (i, i + rope_dim / 2) by the angle of index i, in R, rounded once.  cs: the
+// token's {cos, sin} by index.
+template <typename R, typename R2>
+__device__ __forceinline__ void ka_load_rotated(const void* p, int type, int64_t base, int d, int rope, int rope_dim,
+                                                const R2* cs, float (&v)[8]) {
   kv8_load(p, type, base + d, v);
   if (rope == PB_ROPE_NONE || d >= rope_dim) return;
+  const int half = rope_dim >> 1;
   if (rope == PB_ROPE_INTERLEAVED) {
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
       if (d + i < rope_dim) {
-        const double2 c = cs[(d + i) >> 1];
-        const double x0 = v[i], x1 = v[i + 1];
+        const R2 c = cs[(d + i) >> 1];
+        const R x0 = v[i], x1 = v[i + 1];
         v[i] = (float)(x0 * c.x - x1 * c.y);
         v[i + 1] = (float)(x0 * c.y + x1 * c.x);
       }
     }
+  } else if ((half & 7) == 0) {  // the 8 partners are 8 consecutive values too
+    const bool low = d < half;
+    const int j = low ? d : d - half;
+    float y[8];
+    kv8_load(p, type, base + (low ? d + half : j), y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const R2 c = cs[j + i];
+      v[i] = low ? (float)((R)v[i] * c.x - (R)y[i] * c.y) : (float)((R)y[i] * c.y + (R)v[i] * c.x);
+    }
   } else {
-    const int half = rope_dim >> 1;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int a = d + i;
       if (a < rope_dim) {
         const bool low = a < half;
         const int64_t o = base + (low ? a + half : a - half);
-        const double y = type == PB_TYPE_F32 ? (double)static_cast<const float*>(p)[o]
-                                             : (double)kv8_from16(static_cast<const uint16_t*>(p)[o], type);
-        const double2 c = cs[low ? a : a - half];
-        const double x = v[i];
+        const R y = type == PB_TYPE_F32 ? static_cast<const float*>(p)[o] : kv8_from16(static_cast<const uint16_t*>(p)[o], type);
+        const R2 c = cs[low ? a : a - half];
+        const R x = v[i];
         v[i] = low ? (float)(x * c.x - y * c.y) : (float)(y * c.y + x * c.x);
       }
     }
@@ -60,133 +70,194 @@ __device__ __forceinline__ void kv8_load_rotated(const void* p, int type, int64_
 
 constexpr int KA_THREADS = 256;
 
-// One CTA: the tokens of one 16-token block of one sequence, a share of the
-// heads (blockIdx.y).  hd / 32 warps work on one head's K or V, a warp on a
-// 16 x 32 tile in the layout's own order.
-__global__ void __launch_bounds__(KA_THREADS) k_kv8_append(kv8_geo g, kv8_append_args a) {
+// A CTA has the tokens of one 16-token block of one sequence, and a share of
+// the kv heads (blockIdx.y < y_kv: hd / 32 warps work on a head's K or V, a
+// warp on a 16 x 32 tile in the layout's order) or of the query heads (a thread
+// takes 8 values at a time).  Memory bound: q, k and v are read
+// once (a partner of the half layout twice, the second time from L1), q_out and
+// the codes written once.  Angles, cosines and sines are computed in double,
+// for a block's tokens once per CTA; k is rotated in double, so that its codes
+// are those of the exact values, q in f32.
+template <int TYPE, int ROPE>
+__global__ void __launch_bounds__(KA_THREADS, 3) k_kv8_append(kv8_geo g, kv8_append_args a, int y_kv) {
   extern __shared__ __align__(16) unsigned char ka_raw[];
-  double2* cs = reinterpret_cast<double2*>(ka_raw);  // [16][rope_dim / 2]
-  __shared__ int found;
+  __shared__ kv8_found found;
   __shared__ uint32_t amax[KA_THREADS / 32];
   pb_pdl_trigger();
   pb_pdl_wait();
   kv8_unit un;
   if (!kv8_find_unit(a.starts, a.first, a.n_seqs, a.n_rows, blockIdx.x, &found, un, a.err)) return;
-  uint8_t* block0 = kv8_block(a.pages, g, a.table, a.ld_table, un.seq, un.blk, a.err);
-  if (!block0) return;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
   const int pos0 = un.blk * PB_KV8_BLOCK, kept = un.lo - pos0, end = un.hi - pos0;  // new tokens: [kept, end) of the block
-  const int half = g.rope == PB_ROPE_NONE ? 0 : g.rope_dim >> 1;
+  const int half = ROPE == PB_ROPE_NONE ? 0 : g.rope_dim >> 1;
+  const bool kv_part = (int)blockIdx.y < y_kv;
+  double2* csd = reinterpret_cast<double2*>(ka_raw);  // [16][half], for k
+  float2* csf = reinterpret_cast<float2*>(ka_raw);    // [16][half], for q
+  uint8_t* block0 = kv8_block(a.pages, g, a.table, a.ld_table, un.seq, un.blk, a.err);
+  if (!block0) return;
   for (int i = tid; i < (end - kept) * half; i += KA_THREADS) {
     const int tok = kept + i / half, j = i % half;
     double s, c;
     sincos((double)(pos0 + tok) * a.freqs[j], &s, &c);
-    cs[tok * half + j] = make_double2(c, s);
+    if (kv_part) csd[tok * half + j] = make_double2(c, s);
+    else csf[tok * half + j] = make_float2((float)c, (float)s);
   }
   __syncthreads();
-  auto row_of = [&](int tok) { return (int64_t)(un.row0 + pos0 + tok - un.first); };
-  const int ny = gridDim.y, y = blockIdx.y;
-  const int kv0 = (int)((int64_t)g.n_kv * y / ny), kv1 = (int)((int64_t)g.n_kv * (y + 1) / ny);
-  const int tiles = g.hd / 32, groups = (KA_THREADS / 32) / tiles, grp = warp / tiles, tile = warp % tiles;
-  const int ntask = 2 * (kv1 - kv0);
-  for (int task0 = 0; task0 < ntask; task0 += groups) {
-    const int task = task0 + grp;
-    const bool on = grp < groups && task < ntask;
-    const bool is_v = task & 1;
-    const int h = kv0 + (task >> 1);
-    uint8_t* blk = block0 + (int64_t)h * g.nblk * g.block_bytes;
-    int8_t* ep = reinterpret_cast<int8_t*>(blk + 32 * g.hd) + (is_v ? 1 : 0);
-    uint4* word = reinterpret_cast<uint4*>(blk + (is_v ? 16 * g.hd : 0) + tile * 512) + lane;
-    float val[16];  // in the order of the lane's 16 bytes
-    int e_old = KV8_E_ZERO;
-    uint4 old = make_uint4(0, 0, 0, 0);
-    uint32_t m = 0;
-    if (on) {
-      if (kept > 0) {
-        e_old = *ep;
-        old = *word;
-      }
-      if (!is_v) {
+  const int64_t row0 = (int64_t)un.row0 + pos0 - un.first;  // row of the block's token 0, were it there
+  if (kv_part) {
+    const int y = blockIdx.y;
+    const int kv0 = (int)((int64_t)g.n_kv * y / y_kv), kv1 = (int)((int64_t)g.n_kv * (y + 1) / y_kv);
+    const int tiles = g.hd / 32, groups = (KA_THREADS / 32) / tiles, grp = warp / tiles, tile = warp % tiles;
+    for (int task0 = 2 * kv0; task0 < 2 * kv1; task0 += groups) {
+      const int task = task0 + grp;
+      const bool on = grp < groups && task < 2 * kv1, is_v = task & 1;
+      const int h = task >> 1;
+      uint8_t* blk = block0 + (int64_t)h * g.nblk * g.block_bytes;
+      int8_t* ep = reinterpret_cast<int8_t*>(blk + 32 * g.hd) + (is_v ? 1 : 0);
+      uint4* word = reinterpret_cast<uint4*>(blk + (is_v ? 16 * g.hd : 0) + tile * 512) + lane;
+      float val[16];  // in the order of the lane's 16 bytes
+      int e_old = KV8_E_ZERO;
+      uint4 old = make_uint4(0, 0, 0, 0);
+      uint32_t m = 0;
+      if (on) {
+        if (kept > 0) {
+          e_old = *ep;
+          old = *word;
+        }
+        if (!is_v) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int tok = gq + 8 * j, d = tile * 32 + 8 * t;
-          float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-          if (tok >= kept && tok < end) {
-            kv8_load_rotated(a.k, a.type, row_of(tok) * a.ldk + h * g.hd, d, g.rope, g.rope_dim, cs + tok * half, x);
-            if (a.k_out) kv8_store(a.k_out, a.otype, row_of(tok) * a.ldko + h * g.hd + d, x);
+          for (int j = 0; j < 2; ++j) {
+            const int tok = gq + 8 * j, d = tile * 32 + 8 * t;
+            float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (tok >= kept && tok < end) {
+              ka_load_rotated<double>(a.k, TYPE, (row0 + tok) * a.ldk + h * g.hd, d, ROPE, g.rope_dim, csd + tok * half, x);
+              if (a.k_out) kv8_store(a.k_out, a.otype, (row0 + tok) * a.ldko + h * g.hd + d, x);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) val[8 * j + i] = x[i];
           }
+        } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) val[8 * j + i] = x[i];
-        }
-      } else {
+          for (int j = 0; j < 4; ++j) {  // tokens 2t, 2t + 1, 2t + 8, 2t + 9
+            const int tok = 2 * t + (j & 1) + 8 * (j >> 1), d = tile * 32 + 4 * gq;
+            float x[4] = {0, 0, 0, 0};
+            if (tok >= kept && tok < end) {
+              kv8_load(a.v, TYPE, (row0 + tok) * a.ldv + h * g.hd + d, x);
+              if (a.v_out) kv8_store(a.v_out, a.otype, (row0 + tok) * a.ldvo + h * g.hd + d, x);
+            }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {  // tokens 2t, 2t + 1, 2t + 8, 2t + 9
-          const int tok = 2 * t + (j & 1) + 8 * (j >> 1), d = tile * 32 + 4 * gq;
-          float x[4] = {0, 0, 0, 0};
-          if (tok >= kept && tok < end) {
-            kv8_load(a.v, a.type, row_of(tok) * a.ldv + h * g.hd + d, x);
-            if (a.v_out) kv8_store(a.v_out, a.otype, row_of(tok) * a.ldvo + h * g.hd + d, x);
+            for (int i = 0; i < 4; ++i) val[4 * i + j] = x[i];
           }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) val[4 * i + j] = x[i];
         }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(val[i]) & 0x7FFFFFFFu);
       }
+      m = __reduce_max_sync(0xffffffffu, m);
+      __syncthreads();  // the round before has read amax
+      if (lane == 0) amax[warp] = m;
+      __syncthreads();  // and every warp of a head has read its exponent before one writes it
+      if (on) {
+        for (int w = 0; w < tiles; ++w) m = max(m, amax[grp * tiles + w]);
+        const int need = kv8_need(m, g.code), e = max(e_old, need);
+        if (tile == 0 && lane == 0) *ep = (int8_t)e;
+        const bool down = e_old != KV8_E_ZERO && e_old < e && e != KV8_E_NAN;
+        const bool none = e == KV8_E_ZERO || e == KV8_E_NAN;
+        const float inv = none ? 0.0f : kv8_pow2(-e), shift = down ? kv8_pow2(e_old - e) : 1.0f;
+        uint32_t nw[4];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(val[i]) & 0x7FFFFFFFu);
-    }
-    m = __reduce_max_sync(0xffffffffu, m);
-    __syncthreads();  // the round before has read amax
-    if (lane == 0) amax[warp] = m;
-    __syncthreads();  // and every warp of a head has read its exponent before one writes it
-    if (on) {
-      for (int w = 0; w < tiles; ++w) m = max(m, amax[grp * tiles + w]);
-      const int need = kv8_need(m, g.code), e = max(e_old, need);
-      if (tile == 0 && lane == 0) *ep = (int8_t)e;
-      const bool down = e_old != KV8_E_ZERO && e_old < e && e != KV8_E_NAN;
-      const float inv = e == KV8_E_ZERO || e == KV8_E_NAN ? 0.0f : kv8_pow2(-e);
-      const float shift = down ? kv8_pow2(e_old - e) : 1.0f;
-      uint32_t ow[4] = {old.x, old.y, old.z, old.w}, nw[4];
+        for (int w = 0; w < 4; ++w)
+          nw[w] = none ? 0u : kv8_encode4(val[4 * w] * inv, val[4 * w + 1] * inv, val[4 * w + 2] * inv, val[4 * w + 3] * inv, g.code);
+        if (kept > 0) {  // beside the block's older tokens
+          const uint32_t ow[4] = {old.x, old.y, old.z, old.w};
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t r = 0;
+          for (int w = 0; w < 4; ++w) {
+            uint32_t r = 0;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const int i = 4 * w + b;
-          const int tok = is_v ? 2 * t + (b & 1) + 8 * (b >> 1) : gq + 8 * (i >> 3);
-          uint32_t c = (ow[w] >> (8 * b)) & 0xFFu;
-          if (tok >= kept && tok < end) c = inv != 0.0f ? kv8_encode(val[i] * inv, g.code) : 0u;
-          else if (down) c = kv8_encode(kv8_decode(c, g.code) * shift, g.code);
-          r |= c << (8 * b);
+            for (int b = 0; b < 4; ++b) {
+              const int tok = is_v ? 2 * t + (b & 1) + 8 * (b >> 1) : gq + 8 * (w >> 1);
+              uint32_t c = (ow[w] >> (8 * b)) & 0xFFu;
+              if (tok >= kept && tok < end) c = (nw[w] >> (8 * b)) & 0xFFu;
+              else if (tok >= end) c = 0u;
+              else if (down) c = kv8_encode(kv8_decode(c, g.code) * shift, g.code);
+              r |= c << (8 * b);
+            }
+            nw[w] = r;
+          }
         }
-        nw[w] = r;
+        *word = make_uint4(nw[0], nw[1], nw[2], nw[3]);
       }
-      *word = make_uint4(nw[0], nw[1], nw[2], nw[3]);
     }
-  }
-  if (a.q) {
+  } else {
+    const int y = blockIdx.y - y_kv, ny = gridDim.y - y_kv;
     const int h0 = (int)((int64_t)a.n_heads * y / ny), h1 = (int)((int64_t)a.n_heads * (y + 1) / ny);
-    const int per = (h1 - h0) * (g.hd / 8);
-    for (int i = tid; i < (end - kept) * per; i += KA_THREADS) {
-      const int tok = kept + i / per, r = i % per, h = h0 + r / (g.hd / 8), d = r % (g.hd / 8) * 8;
-      float x[8];
-      kv8_load_rotated(a.q, a.type, row_of(tok) * a.ldq + h * g.hd, d, g.rope, g.rope_dim, cs + tok * half, x);
-      kv8_store(a.q_out, a.otype, row_of(tok) * a.ldqo + h * g.hd + d, x);
+    // a thread's item: 8 values of a head, or 8 and their partners, for all of the block's tokens, two at a time
+    const bool paired = ROPE == PB_ROPE_HALF && (half & 7) == 0;
+    const int np = paired ? half / 8 : 0, per_head = np + (g.hd - (paired ? g.rope_dim : 0)) / 8;
+    for (int r = tid; r < (h1 - h0) * per_head; r += KA_THREADS) {
+      const int h = h0 + r / per_head, c = r % per_head;
+      const bool pair = c < np;
+      const int d = paired ? (pair ? 8 * c : g.rope_dim + 8 * (c - np)) : 8 * c;
+      const int64_t qi = row0 * a.ldq + h * g.hd + d, oi = row0 * a.ldqo + h * g.hd + d;
+      for (int t0 = kept; t0 < end; t0 += 2) {
+        float x[2][8], z[2][8];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int tok = t0 + u;
+          if (tok >= end) break;
+          if (paired) {
+            kv8_load(a.q, TYPE, qi + tok * (int64_t)a.ldq, x[u]);
+            if (pair) kv8_load(a.q, TYPE, qi + tok * (int64_t)a.ldq + half, z[u]);
+          } else {
+            ka_load_rotated<float>(a.q, TYPE, qi + tok * (int64_t)a.ldq - d, d, ROPE, g.rope_dim, csf + tok * half, x[u]);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int tok = t0 + u;
+          if (tok >= end) break;
+          if (pair) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float2 cs = csf[tok * half + d + i];
+              const float x0 = x[u][i], x1 = z[u][i];
+              x[u][i] = x0 * cs.x - x1 * cs.y;
+              z[u][i] = x0 * cs.y + x1 * cs.x;
+            }
+            kv8_store(a.q_out, a.otype, oi + tok * (int64_t)a.ldqo + half, z[u]);
+          }
+          kv8_store(a.q_out, a.otype, oi + tok * (int64_t)a.ldqo, x[u]);
+        }
+      }
     }
   }
+}
+
+typedef void (*ka_kernel)(kv8_geo, kv8_append_args, int);
+template <int TYPE>
+static ka_kernel ka_pick(int rope) {
+  return rope == PB_ROPE_HALF          ? k_kv8_append<TYPE, PB_ROPE_HALF>
+         : rope == PB_ROPE_INTERLEAVED ? k_kv8_append<TYPE, PB_ROPE_INTERLEAVED>
+                                       : k_kv8_append<TYPE, PB_ROPE_NONE>;
+}
+static ka_kernel ka_kernel_of(int type, int rope) {
+  return type == PB_TYPE_F32 ? ka_pick<PB_TYPE_F32>(rope) : type == PB_TYPE_F16 ? ka_pick<PB_TYPE_F16>(rope) : ka_pick<PB_TYPE_BF16>(rope);
 }
 
 // ============================================================================
 // read: rows of the cache as values
 // ============================================================================
 
-constexpr int KR_THREADS = 256;
+constexpr int KR_THREADS = 256, KR_TILES = 2;
 
-// One CTA: one 16-token block of one sequence; a warp takes 16 x 32 tiles.
-__global__ void __launch_bounds__(KR_THREADS)
+// A CTA has one 16-token block of one sequence, a warp the K or V of a head, up
+// to KR_TILES tiles loaded at once.  Memory bound: the codes are read once, the
+// rows written in pieces of 64 bytes and more.
+template <int CODE>
+__global__ void __launch_bounds__(KR_THREADS, 3)
 k_kv8_read(kv8_geo g, uint8_t* pages, const int* __restrict__ starts, const int* __restrict__ first,
            const int* __restrict__ table, int ld_table, int n_seqs, int n_rows, int otype, void* k_out, int ldk,
            void* v_out, int ldv, int* err) {
-  __shared__ int found;
+  __shared__ kv8_found found;
   pb_pdl_trigger();
   pb_pdl_wait();
   kv8_unit un;
@@ -195,35 +266,50 @@ k_kv8_read(kv8_geo g, uint8_t* pages, const int* __restrict__ starts, const int*
   if (!block0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, t = lane & 3;
   const int pos0 = un.blk * PB_KV8_BLOCK, kept = un.lo - pos0, end = un.hi - pos0, tiles = g.hd / 32;
-  auto row_of = [&](int tok) { return (int64_t)(un.row0 + pos0 + tok - un.first); };
-  for (int i = warp + blockIdx.y * (KR_THREADS / 32); i < 2 * g.n_kv * tiles; i += gridDim.y * (KR_THREADS / 32)) {
-    const bool is_v = i >= g.n_kv * tiles;
-    const int r = is_v ? i - g.n_kv * tiles : i, h = r / tiles, tile = r % tiles;
+  const int64_t row0 = (int64_t)un.row0 + pos0 - un.first;
+  for (int i = warp + blockIdx.y * (KR_THREADS / 32); i < 2 * g.n_kv; i += gridDim.y * (KR_THREADS / 32)) {
+    const bool is_v = i & 1;
+    const int h = i >> 1;
     if (is_v ? !v_out : !k_out) continue;
     const uint8_t* blk = block0 + (int64_t)h * g.nblk * g.block_bytes;
-    const float sc = kv8_scale(reinterpret_cast<const int8_t*>(blk + 32 * g.hd)[is_v ? 1 : 0]);
-    const uint4 w4 = reinterpret_cast<const uint4*>(blk + (is_v ? 16 * g.hd : 0) + tile * 512)[lane];
-    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-    float val[16];
+    const uint4* word = reinterpret_cast<const uint4*>(blk + (is_v ? 16 * g.hd : 0)) + lane;
+    const int e = reinterpret_cast<const int8_t*>(blk + 32 * g.hd)[is_v ? 1 : 0];
+    for (int n0 = 0; n0 < tiles; n0 += KR_TILES) {
+      uint4 w4[KR_TILES];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) val[j] = kv8_decode((w[j >> 2] >> (8 * (j & 3))) & 0xFFu, g.code) * sc;
-    if (!is_v) {
+      for (int n = 0; n < KR_TILES; ++n)
+        if (n0 + n < tiles) w4[n] = word[32 * (n0 + n)];
+      const float sc = kv8_scale(e);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int tok = gq + 8 * j;
-        if (tok < kept || tok >= end) continue;
-        float x[8];
+      for (int n = 0; n < KR_TILES; ++n) {
+        if (n0 + n >= tiles) break;
+        const uint32_t w[4] = {w4[n].x, w4[n].y, w4[n].z, w4[n].w};
+        float val[16];
 #pragma unroll
-        for (int b = 0; b < 8; ++b) x[b] = val[8 * j + b];
-        kv8_store(k_out, otype, row_of(tok) * ldk + h * g.hd + tile * 32 + 8 * t, x);
-      }
-    } else {
+        for (int j = 0; j < 4; ++j) {
+          uint32_t p01, p23;
+          kv8_codes<CODE>(w[j], p01, p23);
+          const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&p01));
+          const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&p23));
+          val[4 * j] = lo.x * sc, val[4 * j + 1] = lo.y * sc, val[4 * j + 2] = hi.x * sc, val[4 * j + 3] = hi.y * sc;
+        }
+        if (!is_v) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int tok = 2 * t + (j & 1) + 8 * (j >> 1);
-        if (tok < kept || tok >= end) continue;
-        const float x[4] = {val[j], val[4 + j], val[8 + j], val[12 + j]};
-        kv8_store(v_out, otype, row_of(tok) * ldv + h * g.hd + tile * 32 + 4 * gq, x);
+          for (int j = 0; j < 2; ++j) {
+            const int tok = gq + 8 * j;
+            float x[8];
+#pragma unroll
+            for (int b = 0; b < 8; ++b) x[b] = val[8 * j + b];
+            if (tok >= kept && tok < end) kv8_store(k_out, otype, (row0 + tok) * ldk + h * g.hd + (n0 + n) * 32 + 8 * t, x);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int tok = 2 * t + (j & 1) + 8 * (j >> 1);
+            const float x[4] = {val[j], val[4 + j], val[8 + j], val[12 + j]};
+            if (tok >= kept && tok < end) kv8_store(v_out, otype, (row0 + tok) * ldv + h * g.hd + (n0 + n) * 32 + 4 * gq, x);
+          }
+        }
       }
     }
   }
@@ -362,27 +448,9 @@ __device__ __forceinline__ uint32_t kt_lo2(float a, float b, uint32_t hi) {
   const __half2 h = *reinterpret_cast<const __half2*>(&hi);
   return kt_h2(__fsub_rn(a, __low2float(h)), __fsub_rn(b, __high2float(h)));
 }
-// four codes -> two f16 pairs, exact
-template <int CODE>
-__device__ __forceinline__ void kt_codes(uint32_t w, uint32_t& p01, uint32_t& p23) {
-  if (CODE == PB_KV8_INT8) {
-    // 0x64 over a byte u is the f16 1024 + u; u = code + 128
-    const uint32_t u = w ^ 0x80808080u;
-    const __half2 off = __half2half2(__ushort_as_half(0x6480));  // 1152
-    uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
-    const __half2 hx = __hsub2(*reinterpret_cast<__half2*>(&x), off), hy = __hsub2(*reinterpret_cast<__half2*>(&y), off);
-    p01 = *reinterpret_cast<const uint32_t*>(&hx);
-    p23 = *reinterpret_cast<const uint32_t*>(&hy);
-  } else {
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
-        "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-        : "=r"(p01), "=r"(p23)
-        : "r"(w));
-  }
-}
 __device__ __forceinline__ void kt_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                "{%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -420,7 +488,7 @@ static size_t kt_smem(int hd) {
 
 __device__ __forceinline__ void kt_mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                "{%0, %1, %2, %3};"
                : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -648,9 +716,9 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
           for (int k = 0; k < 2; ++k) {
             const uint32_t* q = &qa[n][(QN == 8 ? 4 : 0) * k];
             uint32_t c0, c1;
-            kt_codes<CODE>(wa[k], c0, c1);
+            kv8_codes<CODE>(wa[k], c0, c1);
             kt_mma(c[0], q[0], q[1], q[2], q[3], c0, c1);
-            kt_codes<CODE>(wb_[k], c0, c1);
+            kv8_codes<CODE>(wb_[k], c0, c1);
             kt_mma(c[1], q[0], q[1], q[2], q[3], c0, c1);
           }
         }
@@ -756,7 +824,7 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           uint32_t c0, c1;
-          kt_codes<CODE>(ww[j], c0, c1);
+          kv8_codes<CODE>(ww[j], c0, c1);
           kt_mma(o[n][j], p[0], p[1], p[2], p[3], c0, c1);
         }
       }
@@ -1022,9 +1090,15 @@ extern "C" int pb_kv8_append(pb_kv8* kv, void* pages_dev, int type, const void* 
                        n_seqs, n_rows, otype, ldqo, ldko, ldvo, q_out_dev, k_out_dev, v_out_dev, kv->freqs,
                        static_cast<uint8_t*>(pages_dev), ctx->d_err};
   const int64_t units = kv8_units(n_rows, n_seqs);
-  int ny = units >= 4 * ctx->sm_count ? 1 : g.n_kv;
+  // Shares of the heads: CTAs for two waves or so (3 fit on an SM), as each computes its block's angles; no finer than a kv
+  // head, or 512 values of q a token
+  const int64_t want = 6 * ctx->sm_count / units + 1;
+  const int y_kv = (int)(want / 2 < 1 ? 1 : want / 2 > g.n_kv ? g.n_kv : want / 2);
+  const int q_most = pb_cdiv((int64_t)n_heads * g.hd, 1024);
+  const int y_q = !q_dev ? 0 : (int)(want / 2 < 1 ? 1 : want / 2 > q_most ? q_most : want / 2);
   const size_t smem = (size_t)PB_KV8_BLOCK * (g.rope_dim / 2) * sizeof(double2);
-  return pb_launch(ctx, "k_kv8_append", true, k_kv8_append, dim3((unsigned)units, ny), dim3(KA_THREADS), smem, g, a);
+  return pb_launch(ctx, "k_kv8_append", true, ka_kernel_of(type, g.rope), dim3((unsigned)units, y_kv + y_q), dim3(KA_THREADS), smem, g,
+                   a, y_kv);
 }
 
 extern "C" int pb_kv8_read(pb_kv8* kv, const void* pages_dev, const int* starts_dev, const int* first_dev,
@@ -1043,8 +1117,9 @@ extern "C" int pb_kv8_read(pb_kv8* kv, const void* pages_dev, const int* starts_
                                          "and no narrower than the heads");
   pb_device_scope dev(ctx->device);
   const int64_t units = kv8_units(n_rows, n_seqs);
-  const int ny = units >= 4 * ctx->sm_count ? 1 : pb_cdiv(2 * g.n_kv * (g.hd / 32), KR_THREADS / 32);
-  return pb_launch(ctx, "k_kv8_read", true, k_kv8_read, dim3((unsigned)units, ny), dim3(KR_THREADS), 0, g,
+  const int ny = units >= 4 * ctx->sm_count ? 1 : pb_cdiv(2 * g.n_kv, KR_THREADS / 32);
+  return pb_launch(ctx, "k_kv8_read", true, g.code == PB_KV8_INT8 ? k_kv8_read<PB_KV8_INT8> : k_kv8_read<PB_KV8_E4M3>,
+                   dim3((unsigned)units, ny), dim3(KR_THREADS), 0, g,
                    static_cast<uint8_t*>(const_cast<void*>(pages_dev)), starts_dev, first_dev, table_dev, ld_table, n_seqs,
                    n_rows, otype, k_out_dev, ldk, v_out_dev, ldv, ctx->d_err);
 }

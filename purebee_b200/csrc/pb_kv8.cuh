@@ -133,6 +133,39 @@ __device__ __forceinline__ uint32_t kv8_encode(float y, int code) {
   if (code == PB_KV8_INT8) return (uint32_t)__float2int_rn(y) & 0xFFu;
   return (uint32_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
 }
+// four of them as bytes; int8: adding 1.5 * 2^23 rounds to an integer in the low bits
+__device__ __forceinline__ uint32_t kv8_encode4(float y0, float y1, float y2, float y3, int code) {
+  if (code == PB_KV8_INT8) {
+    const float big = 12582912.0f;
+    const uint32_t a = __float_as_uint(__fadd_rn(y0, big)), b = __float_as_uint(__fadd_rn(y1, big));
+    const uint32_t c = __float_as_uint(__fadd_rn(y2, big)), d = __float_as_uint(__fadd_rn(y3, big));
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+  }
+  uint32_t r;
+  asm("{\n\t.reg .b16 l, h;\n\tcvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\t"
+      "mov.b32 %0, {l, h};\n\t}"
+      : "=r"(r)
+      : "f"(y0), "f"(y1), "f"(y2), "f"(y3));
+  return r;
+}
+// four codes -> two f16 pairs, exact
+template <int CODE>
+__device__ __forceinline__ void kv8_codes(uint32_t w, uint32_t& p01, uint32_t& p23) {
+  if (CODE == PB_KV8_INT8) {
+    // 0x64 over a byte u is the f16 1024 + u; u = code + 128
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));  // 1152
+    uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 hx = __hsub2(*reinterpret_cast<__half2*>(&x), off), hy = __hsub2(*reinterpret_cast<__half2*>(&y), off);
+    p01 = *reinterpret_cast<const uint32_t*>(&hx);
+    p23 = *reinterpret_cast<const uint32_t*>(&hy);
+  } else {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(p01), "=r"(p23)
+        : "r"(w));
+  }
+}
 __device__ __forceinline__ float kv8_decode(uint32_t b, int code) {
   if (code == PB_KV8_INT8) return (float)(int8_t)b;
   return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3)));
@@ -148,32 +181,35 @@ struct kv8_unit {
   int seq, row0, first, n;  // the sequence, its first row, first token and token count
   int blk, lo, hi;          // the block and the tokens of it that the rows hold, as positions
 };
+struct kv8_found {
+  int seq, row0, n, first;
+};
 // Every thread of the block calls it; `sh` is shared.  False: nothing to do.
 // Row bounds that do not rise, or leave [0, n_rows], raise the error word.
 __device__ __forceinline__ bool kv8_find_unit(const int* __restrict__ starts, const int* __restrict__ first, int n_seqs,
-                                              int n_rows, int u, int* sh, kv8_unit& un, int* err) {
-  if (threadIdx.x == 0) sh[0] = -1;
+                                              int n_rows, int u, kv8_found* sh, kv8_unit& un, int* err) {
+  if (threadIdx.x == 0) sh->seq = -1;
   __syncthreads();
   for (int s = threadIdx.x; s < n_seqs; s += blockDim.x) {
-    const int a = starts[s], b = starts[s + 1];
+    const int a = starts[s], b = starts[s + 1], f = first[s];
     if (a < 0 || b < a || b > n_rows) {
       pb_raise(err, PB_DEVERR_BOUNDS);
     } else if ((a >> 4) + 2 * s <= u && u < (b >> 4) + 2 * s + 2) {
-      sh[0] = s;
+      *sh = {s, a, b - a, f};
     }
   }
   __syncthreads();
-  const int s = sh[0];
-  if (s < 0) return false;
-  un.seq = s;
-  un.row0 = starts[s];
-  un.n = starts[s + 1] - un.row0;
-  un.first = first[s];
+  const kv8_found f = *sh;
+  if (f.seq < 0) return false;
+  un.seq = f.seq;
+  un.row0 = f.row0;
+  un.n = f.n;
+  un.first = f.first;
   if (un.first < 0 || un.first > 0x7FFFFFF0 - un.n) {
     if (threadIdx.x == 0) pb_raise(err, PB_DEVERR_BOUNDS);
     return false;
   }
-  un.blk = un.first / PB_KV8_BLOCK + (u - ((un.row0 >> 4) + 2 * s));
+  un.blk = un.first / PB_KV8_BLOCK + (u - ((un.row0 >> 4) + 2 * un.seq));
   un.lo = max(un.first, un.blk * PB_KV8_BLOCK);
   un.hi = min(un.first + un.n, un.blk * PB_KV8_BLOCK + PB_KV8_BLOCK);
   return un.lo < un.hi;
