@@ -3,7 +3,7 @@
 // layout and the codes).
 #include <math.h>
 
-#include <vector>
+#include <type_traits>
 
 #include "pb_kv8.cuh"
 
@@ -23,211 +23,266 @@ struct kv8_append_args {
   int* err;
 };
 
-// 8 consecutive values of a head from d on, rotated: the pair (2i, 2i + 1) or
-// (i, i + rope_dim / 2) by the angle of index i, in R, rounded once.  cs: the
-// token's {cos, sin} by index.
-template <typename R, typename R2>
-__device__ __forceinline__ void ka_load_rotated(const void* p, int type, int64_t base, int d, int rope, int rope_dim,
-                                                const R2* cs, float (&v)[8]) {
-  kv8_load(p, type, base + d, v);
-  if (rope == PB_ROPE_NONE || d >= rope_dim) return;
-  const int half = rope_dim >> 1;
-  if (rope == PB_ROPE_INTERLEAVED) {
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      if (d + i < rope_dim) {
-        const R2 c = cs[(d + i) >> 1];
-        const R x0 = v[i], x1 = v[i + 1];
-        v[i] = (float)(x0 * c.x - x1 * c.y);
-        v[i + 1] = (float)(x0 * c.y + x1 * c.x);
-      }
-    }
-  } else if ((half & 7) == 0) {  // the 8 partners are 8 consecutive values too
-    const bool low = d < half;
-    const int j = low ? d : d - half;
-    float y[8];
-    kv8_load(p, type, base + (low ? d + half : j), y);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const R2 c = cs[j + i];
-      v[i] = low ? (float)((R)v[i] * c.x - (R)y[i] * c.y) : (float)((R)y[i] * c.y + (R)v[i] * c.x);
-    }
+constexpr int KA_THREADS = 128;
+constexpr int KA_ROWS = 32 << 10;  // bytes of a CTA's rows (16 tokens of its heads)
+
+template <int TYPE>
+__device__ __forceinline__ float ka_at(const unsigned char* row, int d) {
+  if (TYPE == PB_TYPE_F32) return reinterpret_cast<const float*>(row)[d];
+  return kv8_from16(reinterpret_cast<const uint16_t*>(row)[d], TYPE);
+}
+template <int TYPE>
+__device__ __forceinline__ void ka_at4(const unsigned char* row, int d, float (&v)[4]) {
+  if (TYPE == PB_TYPE_F32) {
+    const float4 x = *reinterpret_cast<const float4*>(row + 4 * d);
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
   } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int a = d + i;
-      if (a < rope_dim) {
-        const bool low = a < half;
-        const int64_t o = base + (low ? a + half : a - half);
-        const R y = type == PB_TYPE_F32 ? static_cast<const float*>(p)[o] : kv8_from16(static_cast<const uint16_t*>(p)[o], type);
-        const R2 c = cs[low ? a : a - half];
-        const R x = v[i];
-        v[i] = low ? (float)(x * c.x - y * c.y) : (float)(y * c.y + x * c.x);
-      }
-    }
+    const uint2 x = *reinterpret_cast<const uint2*>(row + 2 * d);
+    v[0] = kv8_from16(x.x & 0xFFFFu, TYPE), v[1] = kv8_from16(x.x >> 16, TYPE);
+    v[2] = kv8_from16(x.y & 0xFFFFu, TYPE), v[3] = kv8_from16(x.y >> 16, TYPE);
   }
 }
 
-constexpr int KA_THREADS = 256;
+// The rows' rotation, in R: nt tokens x heads from shared memory (`stride` bytes
+// a token), the pair (2i, 2i + 1) or (i, i + rope_dim / 2) by the angle of index
+// i; cs: {cos, sin} [token][half].  A thread has an item (4 values of a head at
+// d, and their partners in the half layout) for tokens tok0, tok0 + share, ...:
+// put(tok, h, d, values, largest) stores 4 rotated values, put1 one;
+// most(h, largest) gets the largest magnitude of the item.  A thread gives both
+// values of a pair, so put may write in place.
+template <int TYPE, int ROPE, typename R, typename R2, typename Put, typename Put1, typename Most>
+__device__ __forceinline__ void ka_rotate(const unsigned char* rows, int stride, int nt, int heads, int hd, int rope_dim,
+                                          const R2* cs, Put put, Put1 put1, Most most) {
+  constexpr int ES = TYPE == PB_TYPE_F32 ? 4 : 2;
+  const int half = ROPE == PB_ROPE_NONE ? 0 : rope_dim >> 1;
+  auto larger = [](uint32_t m, float v) { return max(m, __float_as_uint(v) & 0x7FFFFFFFu); };
+  if (ROPE == PB_ROPE_HALF && (half & 3) != 0) {  // pairs one by one
+    const int per = heads * (hd - half);
+    for (int x = threadIdx.x; x < nt * per; x += KA_THREADS) {
+      const int tok = x / per, h = x % per / (hd - half), i = x % per % (hd - half);
+      const unsigned char* row = rows + tok * stride + h * hd * ES;
+      uint32_t m = 0;
+      if (i < half) {
+        const R2 c = cs[tok * half + i];
+        const R x0 = ka_at<TYPE>(row, i), x1 = ka_at<TYPE>(row, i + half);
+        const float y0 = (float)(x0 * c.x - x1 * c.y), y1 = (float)(x0 * c.y + x1 * c.x);
+        put1(tok, h, i, y0);
+        put1(tok, h, i + half, y1);
+        m = larger(larger(m, y0), y1);
+      } else {
+        const float y = ka_at<TYPE>(row, i + half);
+        put1(tok, h, i + half, y);
+        m = larger(m, y);
+      }
+      most(h, m);
+    }
+    return;
+  }
+  const int np = ROPE == PB_ROPE_HALF ? half / 4 : 0, per_head = (hd - 4 * np) / 4, items = heads * per_head;
+  // threads beyond the items of a token take other tokens
+  const int share = items < KA_THREADS ? KA_THREADS / items : 1, tok0 = share > 1 ? threadIdx.x / items : 0;
+  if (tok0 >= share) return;
+  for (int x = share > 1 ? threadIdx.x % items : threadIdx.x; x < items; x += KA_THREADS) {
+    const int h = x / per_head, c = x % per_head, d = c < np ? 4 * c : 4 * c + 4 * np;
+    const bool pair = ROPE == PB_ROPE_HALF && c < np, turn = ROPE == PB_ROPE_INTERLEAVED && d < rope_dim;
+    const unsigned char* row = rows + tok0 * stride + h * hd * ES;
+    const R2* z = cs + tok0 * half + (pair ? d : d >> 1);
+    uint32_t m = 0;
+#pragma unroll 2
+    for (int tok = tok0; tok < nt; tok += share, row += share * stride, z += share * half) {
+      float v[4];
+      ka_at4<TYPE>(row, d, v);
+      if (pair) {
+        float w[4];
+        ka_at4<TYPE>(row, d + half, w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const R2 cz = z[i];
+          const R x0 = v[i], x1 = w[i];
+          v[i] = (float)(x0 * cz.x - x1 * cz.y);
+          w[i] = (float)(x0 * cz.y + x1 * cz.x);
+          m = larger(m, w[i]);
+        }
+        put(tok, h, d + half, w);
+      } else if (turn) {
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          if (d + i < rope_dim) {
+            const R2 cz = z[i >> 1];
+            const R x0 = v[i], x1 = v[i + 1];
+            v[i] = (float)(x0 * cz.x - x1 * cz.y);
+            v[i + 1] = (float)(x0 * cz.y + x1 * cz.x);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = larger(m, v[i]);
+      put(tok, h, d, v);
+    }
+    most(h, m);
+  }
+}
 
-// A CTA has the tokens of one 16-token block of one sequence, and a share of
-// the kv heads (blockIdx.y < y_kv: hd / 32 warps work on a head's K or V, a
-// warp on a 16 x 32 tile in the layout's order) or of the query heads (a thread
-// takes 8 values at a time).  Memory bound: q, k and v are read
-// once (a partner of the half layout twice, the second time from L1), q_out and
-// the codes written once.  Angles, cosines and sines are computed in double,
-// for a block's tokens once per CTA; k is rotated in double, so that its codes
-// are those of the exact values, q in f32.
+// A CTA has the tokens of one 16-token block of one sequence and a share of the
+// kv heads (blockIdx.y < y_kv) or of the query heads.  Memory bound: its rows
+// come by bulk copies, all at once, while the angles are computed (one sincos a
+// pair and block in double, the other tokens by the addition theorem: 15 steps
+// add about 2^-48); q_out goes out from the rotation, k is rotated within shared
+// memory, and a warp then codes a head's K or V, tile by tile in the layout's
+// order.  Many small CTAs keep about 128 KB a SM in flight.  k is rotated in
+// double, so that its codes are those of the exact values; q in f32.
 template <int TYPE, int ROPE>
-__global__ void __launch_bounds__(KA_THREADS, 3) k_kv8_append(kv8_geo g, kv8_append_args a, int y_kv) {
+__global__ void __launch_bounds__(KA_THREADS, 4) k_kv8_append(kv8_geo g, kv8_append_args a, int y_kv) {
+  constexpr int ES = TYPE == PB_TYPE_F32 ? 4 : 2;
   extern __shared__ __align__(16) unsigned char ka_raw[];
   __shared__ kv8_found found;
-  __shared__ uint32_t amax[KA_THREADS / 32];
+  __shared__ uint64_t bar;
+  __shared__ uint32_t amax[KA_ROWS / (PB_KV8_BLOCK * 32 * ES)];  // by head: of k, of v
+  if (threadIdx.x == 0) {
+    pb_mbar_init(&bar, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   pb_pdl_trigger();
   pb_pdl_wait();
   kv8_unit un;
   if (!kv8_find_unit(a.starts, a.first, a.n_seqs, a.n_rows, blockIdx.x, &found, un, a.err)) return;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
-  const int pos0 = un.blk * PB_KV8_BLOCK, kept = un.lo - pos0, end = un.hi - pos0;  // new tokens: [kept, end) of the block
-  const int half = ROPE == PB_ROPE_NONE ? 0 : g.rope_dim >> 1;
-  const bool kv_part = (int)blockIdx.y < y_kv;
-  double2* csd = reinterpret_cast<double2*>(ka_raw);  // [16][half], for k
-  float2* csf = reinterpret_cast<float2*>(ka_raw);    // [16][half], for q
   uint8_t* block0 = kv8_block(a.pages, g, a.table, a.ld_table, un.seq, un.blk, a.err);
   if (!block0) return;
-  for (int i = tid; i < (end - kept) * half; i += KA_THREADS) {
-    const int tok = kept + i / half, j = i % half;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
+  const int pos0 = un.blk * PB_KV8_BLOCK, kept = un.lo - pos0, nt = un.hi - un.lo, end = kept + nt;  // new tokens: [kept, end)
+  const int64_t row0 = (int64_t)un.row0 + un.lo - un.first;  // the first one's row
+  const int half = ROPE == PB_ROPE_NONE ? 0 : g.rope_dim >> 1;
+  const bool kv_part = (int)blockIdx.y < y_kv;
+  const int y = kv_part ? blockIdx.y : blockIdx.y - y_kv, ny = kv_part ? y_kv : gridDim.y - y_kv, all = kv_part ? g.n_kv : a.n_heads;
+  const int h0 = (int)((int64_t)all * y / ny), heads = (int)((int64_t)all * (y + 1) / ny) - h0;
+  if (heads == 0) return;
+  // [cs][rows of q, or of k and of v][k rotated, where the rows are not f32]; a token's rows are 16 bytes further apart than
+  // they are long, which spreads tokens over the banks
+  const int bytes = heads * g.hd * ES, stride = bytes + 16, fstride = heads * g.hd * 4 + 16;
+  unsigned char* rows = ka_raw + PB_KV8_BLOCK * half * sizeof(double2);
+  unsigned char* vrows = rows + nt * stride;
+  unsigned char* krot = TYPE == PB_TYPE_F32 ? rows : vrows + nt * stride;
+  if (tid == 0) pb_mbar_arrive_tx(&bar, nt * bytes * (kv_part ? 2 : 1));
+  __syncthreads();
+  if (tid < nt) {
+    if (kv_part) {
+      pb_bulk_g2s(rows + tid * stride, static_cast<const char*>(a.k) + ((row0 + tid) * a.ldk + h0 * g.hd) * ES, bytes, &bar);
+      pb_bulk_g2s(vrows + tid * stride, static_cast<const char*>(a.v) + ((row0 + tid) * a.ldv + h0 * g.hd) * ES, bytes, &bar);
+    } else {
+      pb_bulk_g2s(rows + tid * stride, static_cast<const char*>(a.q) + ((row0 + tid) * a.ldq + h0 * g.hd) * ES, bytes, &bar);
+    }
+  }
+  double2* csd = reinterpret_cast<double2*>(ka_raw);  // [token][half], for k
+  float2* csf = reinterpret_cast<float2*>(ka_raw);    // for q
+  for (int j = tid; j < half; j += KA_THREADS) {
+    const double f = a.freqs[j], c1 = a.freqs[128 + j], s1 = a.freqs[256 + j];  // cos f, sin f
     double s, c;
-    sincos((double)(pos0 + tok) * a.freqs[j], &s, &c);
-    if (kv_part) csd[tok * half + j] = make_double2(c, s);
-    else csf[tok * half + j] = make_float2((float)c, (float)s);
+    sincos((double)un.lo * f, &s, &c);
+    for (int tok = 0; tok < nt; ++tok) {
+      if (kv_part) csd[tok * half + j] = make_double2(c, s);
+      else csf[tok * half + j] = make_float2((float)c, (float)s);
+      const double cn = __fma_rn(c, c1, -(s * s1));
+      s = __fma_rn(s, c1, c * s1);
+      c = cn;
+    }
+  }
+  if (kv_part)
+    for (int i = tid; i < 2 * heads; i += KA_THREADS) amax[i] = 0;
+  const bool ok = pb_mbar_wait(&bar, 0, a.err);
+  if (!__syncthreads_and(ok)) return;
+  if (!kv_part) {
+    auto out = [&](auto ot) {
+      constexpr int OT = decltype(ot)::value;
+      auto at = [&](int tok, int h, int d) { return (row0 + tok) * a.ldqo + (h0 + h) * g.hd + d; };
+      ka_rotate<TYPE, ROPE, float>(rows, stride, nt, heads, g.hd, g.rope_dim, csf,
+                                   [&](int tok, int h, int d, const float (&v)[4]) { kv8_store(a.q_out, OT, at(tok, h, d), v); },
+                                   [&](int tok, int h, int d, float v) { kv8_store1(a.q_out, OT, at(tok, h, d), v); },
+                                   [](int, uint32_t) {});
+    };
+    if (a.otype == PB_TYPE_F32) out(std::integral_constant<int, PB_TYPE_F32>());
+    else if (a.otype == PB_TYPE_F16) out(std::integral_constant<int, PB_TYPE_F16>());
+    else out(std::integral_constant<int, PB_TYPE_BF16>());
+    return;
+  }
+  {
+    auto at = [&](int tok, int h, int d) { return (row0 + tok) * a.ldko + (h0 + h) * g.hd + d; };
+    auto keep = [&](int tok, int h, int d) { return reinterpret_cast<float*>(krot + tok * fstride) + h * g.hd + d; };
+    ka_rotate<TYPE, ROPE, double>(
+        rows, stride, nt, heads, g.hd, g.rope_dim, csd,
+        [&](int tok, int h, int d, const float (&v)[4]) {
+          *reinterpret_cast<float4*>(keep(tok, h, d)) = make_float4(v[0], v[1], v[2], v[3]);
+          if (a.k_out) kv8_store(a.k_out, a.otype, at(tok, h, d), v);
+        },
+        [&](int tok, int h, int d, float v) {
+          *keep(tok, h, d) = v;
+          if (a.k_out) kv8_store1(a.k_out, a.otype, at(tok, h, d), v);
+        },
+        [&](int h, uint32_t m) { atomicMax(&amax[2 * h], m); });
+    ka_rotate<TYPE, PB_ROPE_NONE, float>(  // v as it is: its largest values, and v_out
+        vrows, stride, nt, heads, g.hd, 0, csf,
+        [&](int tok, int h, int d, const float (&v)[4]) {
+          if (a.v_out) kv8_store(a.v_out, a.otype, (row0 + tok) * a.ldvo + (h0 + h) * g.hd + d, v);
+        },
+        [](int, int, int, float) {}, [&](int h, uint32_t m) { atomicMax(&amax[2 * h + 1], m); });
   }
   __syncthreads();
-  const int64_t row0 = (int64_t)un.row0 + pos0 - un.first;  // row of the block's token 0, were it there
-  if (kv_part) {
-    const int y = blockIdx.y;
-    const int kv0 = (int)((int64_t)g.n_kv * y / y_kv), kv1 = (int)((int64_t)g.n_kv * (y + 1) / y_kv);
-    const int tiles = g.hd / 32, groups = (KA_THREADS / 32) / tiles, grp = warp / tiles, tile = warp % tiles;
-    for (int task0 = 2 * kv0; task0 < 2 * kv1; task0 += groups) {
-      const int task = task0 + grp;
-      const bool on = grp < groups && task < 2 * kv1, is_v = task & 1;
-      const int h = task >> 1;
-      uint8_t* blk = block0 + (int64_t)h * g.nblk * g.block_bytes;
-      int8_t* ep = reinterpret_cast<int8_t*>(blk + 32 * g.hd) + (is_v ? 1 : 0);
-      uint4* word = reinterpret_cast<uint4*>(blk + (is_v ? 16 * g.hd : 0) + tile * 512) + lane;
-      float val[16];  // in the order of the lane's 16 bytes
-      int e_old = KV8_E_ZERO;
+  const int tiles = g.hd / 32;
+  for (int task = warp; task < 2 * heads; task += KA_THREADS / 32) {
+    const bool is_v = task & 1;
+    const int h = task >> 1;
+    uint8_t* blk = block0 + (int64_t)(h0 + h) * g.nblk * g.block_bytes;
+    int8_t* ep = reinterpret_cast<int8_t*>(blk + 32 * g.hd) + (is_v ? 1 : 0);
+    uint4* word = reinterpret_cast<uint4*>(blk + (is_v ? 16 * g.hd : 0)) + lane;  // 32 a tile
+    const int e_old = kept > 0 ? *ep : KV8_E_ZERO;
+    const int need = kv8_need(amax[task], g.code), e = max(e_old, need);
+    __syncwarp();  // every lane has the old exponent
+    if (lane == 0) *ep = (int8_t)e;
+    const bool down = e_old != KV8_E_ZERO && e_old < e && e != KV8_E_NAN;
+    const bool none = e == KV8_E_ZERO || e == KV8_E_NAN;
+    const float inv = none ? 0.0f : kv8_pow2(-e), shift = down ? kv8_pow2(e_old - e) : 1.0f;
+#pragma unroll 2
+    for (int n = 0; n < tiles; ++n) {
       uint4 old = make_uint4(0, 0, 0, 0);
-      uint32_t m = 0;
-      if (on) {
-        if (kept > 0) {
-          e_old = *ep;
-          old = *word;
+      if (kept > 0) old = word[32 * n];
+      float val[4][4];  // in the order of the lane's 16 bytes: words x bytes
+      if (!is_v) {  // tokens gq, gq + 8 at 8t ..
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int tok = gq + 8 * (w >> 1) - kept;
+          if (tok >= 0 && tok < nt) ka_at4<PB_TYPE_F32>(krot + tok * fstride, h * g.hd + n * 32 + 8 * t + 4 * (w & 1), val[w]);
+          else val[w][0] = val[w][1] = val[w][2] = val[w][3] = 0.0f;
         }
-        if (!is_v) {
+      } else {  // values 4gq .. at tokens 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int tok = gq + 8 * j, d = tile * 32 + 8 * t;
-            float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (tok >= kept && tok < end) {
-              ka_load_rotated<double>(a.k, TYPE, (row0 + tok) * a.ldk + h * g.hd, d, ROPE, g.rope_dim, csd + tok * half, x);
-              if (a.k_out) kv8_store(a.k_out, a.otype, (row0 + tok) * a.ldko + h * g.hd + d, x);
-            }
+        for (int j = 0; j < 4; ++j) {
+          const int tok = 2 * t + (j & 1) + 8 * (j >> 1) - kept;
+          float v[4] = {0, 0, 0, 0};
+          if (tok >= 0 && tok < nt) ka_at4<TYPE>(vrows + tok * stride, h * g.hd + n * 32 + 4 * gq, v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) val[8 * j + i] = x[i];
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {  // tokens 2t, 2t + 1, 2t + 8, 2t + 9
-            const int tok = 2 * t + (j & 1) + 8 * (j >> 1), d = tile * 32 + 4 * gq;
-            float x[4] = {0, 0, 0, 0};
-            if (tok >= kept && tok < end) {
-              kv8_load(a.v, TYPE, (row0 + tok) * a.ldv + h * g.hd + d, x);
-              if (a.v_out) kv8_store(a.v_out, a.otype, (row0 + tok) * a.ldvo + h * g.hd + d, x);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) val[4 * i + j] = x[i];
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(val[i]) & 0x7FFFFFFFu);
-      }
-      m = __reduce_max_sync(0xffffffffu, m);
-      __syncthreads();  // the round before has read amax
-      if (lane == 0) amax[warp] = m;
-      __syncthreads();  // and every warp of a head has read its exponent before one writes it
-      if (on) {
-        for (int w = 0; w < tiles; ++w) m = max(m, amax[grp * tiles + w]);
-        const int need = kv8_need(m, g.code), e = max(e_old, need);
-        if (tile == 0 && lane == 0) *ep = (int8_t)e;
-        const bool down = e_old != KV8_E_ZERO && e_old < e && e != KV8_E_NAN;
-        const bool none = e == KV8_E_ZERO || e == KV8_E_NAN;
-        const float inv = none ? 0.0f : kv8_pow2(-e), shift = down ? kv8_pow2(e_old - e) : 1.0f;
-        uint32_t nw[4];
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          nw[w] = none ? 0u : kv8_encode4(val[4 * w] * inv, val[4 * w + 1] * inv, val[4 * w + 2] * inv, val[4 * w + 3] * inv, g.code);
-        if (kept > 0) {  // beside the block's older tokens
-          const uint32_t ow[4] = {old.x, old.y, old.z, old.w};
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            uint32_t r = 0;
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-              const int tok = is_v ? 2 * t + (b & 1) + 8 * (b >> 1) : gq + 8 * (w >> 1);
-              uint32_t c = (ow[w] >> (8 * b)) & 0xFFu;
-              if (tok >= kept && tok < end) c = (nw[w] >> (8 * b)) & 0xFFu;
-              else if (tok >= end) c = 0u;
-              else if (down) c = kv8_encode(kv8_decode(c, g.code) * shift, g.code);
-              r |= c << (8 * b);
-            }
-            nw[w] = r;
-          }
-        }
-        *word = make_uint4(nw[0], nw[1], nw[2], nw[3]);
-      }
-    }
-  } else {
-    const int y = blockIdx.y - y_kv, ny = gridDim.y - y_kv;
-    const int h0 = (int)((int64_t)a.n_heads * y / ny), h1 = (int)((int64_t)a.n_heads * (y + 1) / ny);
-    // a thread's item: 8 values of a head, or 8 and their partners, for all of the block's tokens, two at a time
-    const bool paired = ROPE == PB_ROPE_HALF && (half & 7) == 0;
-    const int np = paired ? half / 8 : 0, per_head = np + (g.hd - (paired ? g.rope_dim : 0)) / 8;
-    for (int r = tid; r < (h1 - h0) * per_head; r += KA_THREADS) {
-      const int h = h0 + r / per_head, c = r % per_head;
-      const bool pair = c < np;
-      const int d = paired ? (pair ? 8 * c : g.rope_dim + 8 * (c - np)) : 8 * c;
-      const int64_t qi = row0 * a.ldq + h * g.hd + d, oi = row0 * a.ldqo + h * g.hd + d;
-      for (int t0 = kept; t0 < end; t0 += 2) {
-        float x[2][8], z[2][8];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int tok = t0 + u;
-          if (tok >= end) break;
-          if (paired) {
-            kv8_load(a.q, TYPE, qi + tok * (int64_t)a.ldq, x[u]);
-            if (pair) kv8_load(a.q, TYPE, qi + tok * (int64_t)a.ldq + half, z[u]);
-          } else {
-            ka_load_rotated<float>(a.q, TYPE, qi + tok * (int64_t)a.ldq - d, d, ROPE, g.rope_dim, csf + tok * half, x[u]);
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int tok = t0 + u;
-          if (tok >= end) break;
-          if (pair) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float2 cs = csf[tok * half + d + i];
-              const float x0 = x[u][i], x1 = z[u][i];
-              x[u][i] = x0 * cs.x - x1 * cs.y;
-              z[u][i] = x0 * cs.y + x1 * cs.x;
-            }
-            kv8_store(a.q_out, a.otype, oi + tok * (int64_t)a.ldqo + half, z[u]);
-          }
-          kv8_store(a.q_out, a.otype, oi + tok * (int64_t)a.ldqo, x[u]);
+          for (int w = 0; w < 4; ++w) val[w][j] = v[w];
         }
       }
+      uint32_t nw[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        nw[w] = none ? 0u : kv8_encode4(val[w][0] * inv, val[w][1] * inv, val[w][2] * inv, val[w][3] * inv, g.code);
+      if (kept > 0) {  // beside the block's older tokens
+        const uint32_t ow[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t r = 0;
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const int tok = is_v ? 2 * t + (b & 1) + 8 * (b >> 1) : gq + 8 * (w >> 1);
+            uint32_t c = (ow[w] >> (8 * b)) & 0xFFu;
+            if (tok >= kept) c = (nw[w] >> (8 * b)) & 0xFFu;  // 0 past the new tokens
+            else if (down) c = kv8_encode(kv8_decode(c, g.code) * shift, g.code);
+            r |= c << (8 * b);
+          }
+          nw[w] = r;
+        }
+      }
+      word[32 * n] = make_uint4(nw[0], nw[1], nw[2], nw[3]);
     }
   }
 }
@@ -957,6 +1012,10 @@ static kt_kernel kt_kernel_of(int hd, int code, int tr) {
 }
 
 int pb_setup_kv8_kernels(void) {
+  for (int type : {PB_TYPE_F32, PB_TYPE_F16, PB_TYPE_BF16})
+    for (int rope = PB_ROPE_NONE; rope <= PB_ROPE_HALF; ++rope)
+      if (cudaFuncSetAttribute(ka_kernel_of(type, rope), cudaFuncAttributeMaxDynamicSharedMemorySize, 112 << 10) != cudaSuccess)
+        return PB_ERR_CUDA;
   for (int hd = 32; hd <= 256; hd += 32)
     for (int code = 0; code < 2; ++code)
       for (int tr = 8; tr <= 16; tr += 8)
@@ -1009,10 +1068,11 @@ extern "C" int pb_kv8_create(pb_ctx* ctx, const pb_kv8_config* c, pb_kv8** out) 
   *out = nullptr;
   kv8_geo g;
   PB_TRY(kv8_check(ctx, c, &g));
-  double freqs[128];
+  double freqs[3 * 128] = {};  // by pair: its frequency f, then cos f, then sin f
   if (g.rope != PB_ROPE_NONE && pb_rope_freqs(c->rope_theta, g.rope_dim, c->rope_factor, c->low_freq_factor,
                                               c->high_freq_factor, c->original_max_pos, freqs) != PB_OK)
     return pb_set_error(ctx, PB_ERR_ARG, "pb_kv8: bad rotary base or frequency scaling");
+  for (int j = 0; j < g.rope_dim / 2; ++j) freqs[128 + j] = cos(freqs[j]), freqs[256 + j] = sin(freqs[j]);
   pb_device_scope dev(ctx->device);
   pb_kv8* kv = new pb_kv8();
   kv->ctx = ctx;
@@ -1023,7 +1083,7 @@ extern "C" int pb_kv8_create(pb_ctx* ctx, const pb_kv8_config* c, pb_kv8** out) 
   if (e == cudaSuccess) e = cudaMalloc(&kv->ws, parts * 16 * (g.hd + 4) * sizeof(float));
   if (e == cudaSuccess) e = cudaMalloc(&kv->cnt, parts * sizeof(unsigned int));
   if (e == cudaSuccess) e = cudaMemset(kv->cnt, 0, parts * sizeof(unsigned int));
-  if (e == cudaSuccess && g.rope_dim) e = cudaMemcpy(kv->freqs, freqs, g.rope_dim / 2 * sizeof(double), cudaMemcpyHostToDevice);
+  if (e == cudaSuccess && g.rope_dim) e = cudaMemcpy(kv->freqs, freqs, sizeof freqs, cudaMemcpyHostToDevice);
   if (e != cudaSuccess) {
     cudaFree(kv->freqs);
     cudaFree(kv->ws);
@@ -1090,13 +1150,19 @@ extern "C" int pb_kv8_append(pb_kv8* kv, void* pages_dev, int type, const void* 
                        n_seqs, n_rows, otype, ldqo, ldko, ldvo, q_out_dev, k_out_dev, v_out_dev, kv->freqs,
                        static_cast<uint8_t*>(pages_dev), ctx->d_err};
   const int64_t units = kv8_units(n_rows, n_seqs);
-  // Shares of the heads: CTAs for two waves or so (3 fit on an SM), as each computes its block's angles; no finer than a kv
-  // head, or 512 values of q a token
-  const int64_t want = 6 * ctx->sm_count / units + 1;
-  const int y_kv = (int)(want / 2 < 1 ? 1 : want / 2 > g.n_kv ? g.n_kv : want / 2);
-  const int q_most = pb_cdiv((int64_t)n_heads * g.hd, 1024);
-  const int y_q = !q_dev ? 0 : (int)(want / 2 < 1 ? 1 : want / 2 > q_most ? q_most : want / 2);
-  const size_t smem = (size_t)PB_KV8_BLOCK * (g.rope_dim / 2) * sizeof(double2);
+  // Shares of the heads: as many as KA_ROWS holds, fewer where that leaves SMs without a CTA
+  // (at head_dim 256 in f32 one head's K and V fill it)
+  const int kv_most = KA_ROWS / (2 * PB_KV8_BLOCK * g.hd * ts), q_most = KA_ROWS / (PB_KV8_BLOCK * g.hd * ts);
+  const int64_t want = 4 * ctx->sm_count / units / 2 + 1;
+  auto shares = [&](int heads, int most) {
+    const int y = pb_cdiv(heads, most < 1 ? 1 : most);
+    return y > want ? y : want < heads ? (int)want : heads;
+  };
+  const int y_kv = shares(g.n_kv, kv_most), y_q = q_dev ? shares(n_heads, q_most) : 0;
+  const int kv_heads = pb_cdiv(g.n_kv, y_kv), q_heads = y_q ? pb_cdiv(n_heads, y_q) : 0;
+  const size_t kv_rows = (size_t)PB_KV8_BLOCK * (2 * (kv_heads * g.hd * ts + 16) + (ts == 4 ? 0 : kv_heads * g.hd * 4 + 16));
+  const size_t q_rows = (size_t)PB_KV8_BLOCK * (q_heads * g.hd * ts + 16);
+  const size_t smem = (size_t)PB_KV8_BLOCK * (g.rope_dim / 2) * sizeof(double2) + (kv_rows > q_rows ? kv_rows : q_rows);
   return pb_launch(ctx, "k_kv8_append", true, ka_kernel_of(type, g.rope), dim3((unsigned)units, y_kv + y_q), dim3(KA_THREADS), smem, g,
                    a, y_kv);
 }

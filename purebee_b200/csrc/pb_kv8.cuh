@@ -44,7 +44,7 @@ struct kv8_geo {
 struct pb_kv8 {
   pb_ctx* ctx = nullptr;
   kv8_geo g;
-  double* freqs = nullptr;  // [rope_dim / 2] pair frequencies
+  double* freqs = nullptr;  // [3][128] by pair: frequency f, cos f, sin f
   // parts of the groups that pb_kv8_attn splits and their arrival counters (zero
   // between calls); fixed, so recorded graphs stay valid
   float* ws = nullptr;
@@ -114,6 +114,11 @@ __device__ __forceinline__ void kv8_store(void* p, int type, int64_t i, const fl
     if constexpr (NV == 8) *reinterpret_cast<uint4*>(s) = make_uint4(w[0], w[1], w[2], w[3]);
     else *reinterpret_cast<uint2*>(s) = make_uint2(w[0], w[1]);
   }
+}
+
+__device__ __forceinline__ void kv8_store1(void* p, int type, int64_t i, float v) {
+  if (type == PB_TYPE_F32) static_cast<float*>(p)[i] = v;
+  else static_cast<uint16_t*>(p)[i] = (uint16_t)kv8_to16(v, type);
 }
 
 // The exponent that values with the largest magnitude `bits` (of an f32) need.
