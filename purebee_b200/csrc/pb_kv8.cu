@@ -24,7 +24,7 @@ struct kv8_append_args {
 };
 
 constexpr int KA_THREADS = 128;
-constexpr int KA_ROWS = 32 << 10;  // bytes of a CTA's rows (16 tokens of its heads)
+constexpr int KA_ROWS = 32 << 10;  // bytes of a CTA's rows (16 tokens of its heads, k in f32 too): 4 CTAs fit on an SM
 
 template <int TYPE>
 __device__ __forceinline__ float ka_at(const unsigned char* row, int d) {
@@ -146,8 +146,6 @@ __global__ void __launch_bounds__(KA_THREADS, 4) k_kv8_append(kv8_geo g, kv8_app
   pb_pdl_wait();
   kv8_unit un;
   if (!kv8_find_unit(a.starts, a.first, a.n_seqs, a.n_rows, blockIdx.x, &found, un, a.err)) return;
-  uint8_t* block0 = kv8_block(a.pages, g, a.table, a.ld_table, un.seq, un.blk, a.err);
-  if (!block0) return;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
   const int pos0 = un.blk * PB_KV8_BLOCK, kept = un.lo - pos0, nt = un.hi - un.lo, end = kept + nt;  // new tokens: [kept, end)
   const int64_t row0 = (int64_t)un.row0 + un.lo - un.first;  // the first one's row
@@ -172,6 +170,7 @@ __global__ void __launch_bounds__(KA_THREADS, 4) k_kv8_append(kv8_geo g, kv8_app
       pb_bulk_g2s(rows + tid * stride, static_cast<const char*>(a.q) + ((row0 + tid) * a.ldq + h0 * g.hd) * ES, bytes, &bar);
     }
   }
+  uint8_t* block0 = kv_part ? kv8_block(a.pages, g, a.table, a.ld_table, un.seq, un.blk, a.err) : nullptr;
   double2* csd = reinterpret_cast<double2*>(ka_raw);  // [token][half], for k
   float2* csf = reinterpret_cast<float2*>(ka_raw);    // for q
   for (int j = tid; j < half; j += KA_THREADS) {
@@ -189,7 +188,7 @@ __global__ void __launch_bounds__(KA_THREADS, 4) k_kv8_append(kv8_geo g, kv8_app
   if (kv_part)
     for (int i = tid; i < 2 * heads; i += KA_THREADS) amax[i] = 0;
   const bool ok = pb_mbar_wait(&bar, 0, a.err);
-  if (!__syncthreads_and(ok)) return;
+  if (!__syncthreads_and(ok && (block0 || !kv_part))) return;
   if (!kv_part) {
     auto out = [&](auto ot) {
       constexpr int OT = decltype(ot)::value;
@@ -302,72 +301,100 @@ static ka_kernel ka_kernel_of(int type, int rope) {
 // read: rows of the cache as values
 // ============================================================================
 
-constexpr int KR_THREADS = 256, KR_TILES = 2;
+constexpr int KR_THREADS = 128;
+constexpr int KR_BYTES = 24 << 10;  // of a CTA's blocks
 
-// A CTA has one 16-token block of one sequence, a warp the K or V of a head, up
-// to KR_TILES tiles loaded at once.  Memory bound: the codes are read once, the
-// rows written in pieces of 64 bytes and more.
-template <int CODE>
-__global__ void __launch_bounds__(KR_THREADS, 3)
-k_kv8_read(kv8_geo g, uint8_t* pages, const int* __restrict__ starts, const int* __restrict__ first,
-           const int* __restrict__ table, int ld_table, int n_seqs, int n_rows, int otype, void* k_out, int ldk,
-           void* v_out, int ldv, int* err) {
+// A CTA has one 16-token block of one sequence and a share of the heads, whose
+// blocks come by bulk copies, all at once.  Memory bound: the codes are read
+// once, and a warp writes whole rows of a head (lanes along the values).
+template <int CODE, int OT>
+__global__ void __launch_bounds__(KR_THREADS)
+k_kv8_read(kv8_geo g, const uint8_t* pages, const int* __restrict__ starts, const int* __restrict__ first,
+           const int* __restrict__ table, int ld_table, int n_seqs, int n_rows, void* k_out, int ldk, void* v_out, int ldv,
+           int* err) {
+  extern __shared__ __align__(16) unsigned char kr_raw[];
   __shared__ kv8_found found;
+  __shared__ uint64_t bar;
+  const int tid = threadIdx.x;
+  if (tid == 0) {
+    pb_mbar_init(&bar, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   pb_pdl_trigger();
   pb_pdl_wait();
   kv8_unit un;
   if (!kv8_find_unit(starts, first, n_seqs, n_rows, blockIdx.x, &found, un, err)) return;
-  const uint8_t* block0 = kv8_block(pages, g, table, ld_table, un.seq, un.blk, err);
+  const uint8_t* block0 = kv8_block(const_cast<uint8_t*>(pages), g, table, ld_table, un.seq, un.blk, err);
   if (!block0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, t = lane & 3;
-  const int pos0 = un.blk * PB_KV8_BLOCK, kept = un.lo - pos0, end = un.hi - pos0, tiles = g.hd / 32;
+  const int h0 = (int)((int64_t)g.n_kv * blockIdx.y / gridDim.y), heads = (int)((int64_t)g.n_kv * (blockIdx.y + 1) / gridDim.y) - h0;
+  if (tid == 0) {
+    pb_mbar_arrive_tx(&bar, heads * g.block_bytes);
+    for (int h = 0; h < heads; ++h)
+      pb_bulk_g2s(kr_raw + h * g.block_bytes, block0 + (int64_t)(h0 + h) * g.nblk * g.block_bytes, g.block_bytes, &bar);
+  }
+  const int pos0 = un.blk * PB_KV8_BLOCK, kept = un.lo - pos0, end = un.hi - pos0;
   const int64_t row0 = (int64_t)un.row0 + pos0 - un.first;
-  for (int i = warp + blockIdx.y * (KR_THREADS / 32); i < 2 * g.n_kv; i += gridDim.y * (KR_THREADS / 32)) {
-    const bool is_v = i & 1;
-    const int h = i >> 1;
-    if (is_v ? !v_out : !k_out) continue;
-    const uint8_t* blk = block0 + (int64_t)h * g.nblk * g.block_bytes;
-    const uint4* word = reinterpret_cast<const uint4*>(blk + (is_v ? 16 * g.hd : 0)) + lane;
-    const int e = reinterpret_cast<const int8_t*>(blk + 32 * g.hd)[is_v ? 1 : 0];
-    for (int n0 = 0; n0 < tiles; n0 += KR_TILES) {
-      uint4 w4[KR_TILES];
+  if (!__syncthreads_and(pb_mbar_wait(&bar, 0, err))) return;
+  auto decode = [&](const uint4& w4, float sc, float (&val)[16]) {
+    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-      for (int n = 0; n < KR_TILES; ++n)
-        if (n0 + n < tiles) w4[n] = word[32 * (n0 + n)];
-      const float sc = kv8_scale(e);
-#pragma unroll
-      for (int n = 0; n < KR_TILES; ++n) {
-        if (n0 + n >= tiles) break;
-        const uint32_t w[4] = {w4[n].x, w4[n].y, w4[n].z, w4[n].w};
+    for (int j = 0; j < 4; ++j) {
+      uint32_t p01, p23;
+      kv8_codes<CODE>(w[j], p01, p23);
+      const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&p01));
+      const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&p23));
+      val[4 * j] = lo.x * sc, val[4 * j + 1] = lo.y * sc, val[4 * j + 2] = hi.x * sc, val[4 * j + 3] = hi.y * sc;
+    }
+  };
+  auto scale = [&](int h, int which) { return kv8_scale(reinterpret_cast<const int8_t*>(kr_raw + h * g.block_bytes + 32 * g.hd)[which]); };
+  if (k_out) {
+    const int chunks = g.hd / 8;
+    for (int x = tid; x < 8 * chunks; x += KR_THREADS) {  // tokens q and q + 8 at values 8c ..
+      const int q = x / chunks, c = x % chunks;
+      const unsigned char* word = kr_raw + (c >> 2) * 512 + q * 64 + (c & 3) * 16;
+      const int64_t at = (row0 + q) * ldk + h0 * g.hd + 8 * c;
+      for (int h = 0; h < heads; ++h) {
         float val[16];
+        decode(*reinterpret_cast<const uint4*>(word + h * g.block_bytes), scale(h, 0), val);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t p01, p23;
-          kv8_codes<CODE>(w[j], p01, p23);
-          const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&p01));
-          const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&p23));
-          val[4 * j] = lo.x * sc, val[4 * j + 1] = lo.y * sc, val[4 * j + 2] = hi.x * sc, val[4 * j + 3] = hi.y * sc;
-        }
-        if (!is_v) {
+        for (int j = 0; j < 2; ++j) {
+          float v[8];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int tok = gq + 8 * j;
-            float x[8];
-#pragma unroll
-            for (int b = 0; b < 8; ++b) x[b] = val[8 * j + b];
-            if (tok >= kept && tok < end) kv8_store(k_out, otype, (row0 + tok) * ldk + h * g.hd + (n0 + n) * 32 + 8 * t, x);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int tok = 2 * t + (j & 1) + 8 * (j >> 1);
-            const float x[4] = {val[j], val[4 + j], val[8 + j], val[12 + j]};
-            if (tok >= kept && tok < end) kv8_store(v_out, otype, (row0 + tok) * ldv + h * g.hd + (n0 + n) * 32 + 4 * gq, x);
-          }
+          for (int b = 0; b < 8; ++b) v[b] = val[8 * j + b];
+          if (q + 8 * j >= kept && q + 8 * j < end) kv8_store(k_out, OT, at + (int64_t)8 * j * ldk + h * g.hd, v);
         }
       }
     }
   }
+  if (v_out) {
+    const int chunks = g.hd / 4;
+    for (int x = tid; x < 4 * chunks; x += KR_THREADS) {  // tokens 2t, 2t + 1, 2t + 8, 2t + 9 at values 4c ..
+      const int t = x / chunks, c = x % chunks;
+      const unsigned char* word = kr_raw + 16 * g.hd + (c >> 3) * 512 + (c & 7) * 64 + t * 16;
+      const int64_t at = (row0 + 2 * t) * ldv + h0 * g.hd + 4 * c;
+      for (int h = 0; h < heads; ++h) {
+        float val[16];
+        decode(*reinterpret_cast<const uint4*>(word + h * g.block_bytes), scale(h, 1), val);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int o = (j & 1) + 8 * (j >> 1);
+          const float v[4] = {val[j], val[4 + j], val[8 + j], val[12 + j]};
+          if (2 * t + o >= kept && 2 * t + o < end) kv8_store(v_out, OT, at + (int64_t)o * ldv + h * g.hd, v);
+        }
+      }
+    }
+  }
+}
+
+typedef void (*kr_kernel)(kv8_geo, const uint8_t*, const int*, const int*, const int*, int, int, int, void*, int, void*, int, int*);
+static kr_kernel kr_kernel_of(int code, int otype) {
+  if (code == PB_KV8_INT8)
+    return otype == PB_TYPE_F32   ? k_kv8_read<PB_KV8_INT8, PB_TYPE_F32>
+           : otype == PB_TYPE_F16 ? k_kv8_read<PB_KV8_INT8, PB_TYPE_F16>
+                                  : k_kv8_read<PB_KV8_INT8, PB_TYPE_BF16>;
+  return otype == PB_TYPE_F32   ? k_kv8_read<PB_KV8_E4M3, PB_TYPE_F32>
+         : otype == PB_TYPE_F16 ? k_kv8_read<PB_KV8_E4M3, PB_TYPE_F16>
+                                : k_kv8_read<PB_KV8_E4M3, PB_TYPE_BF16>;
 }
 
 // ============================================================================
@@ -1152,7 +1179,7 @@ extern "C" int pb_kv8_append(pb_kv8* kv, void* pages_dev, int type, const void* 
   const int64_t units = kv8_units(n_rows, n_seqs);
   // Shares of the heads: as many as KA_ROWS holds, fewer where that leaves SMs without a CTA
   // (at head_dim 256 in f32 one head's K and V fill it)
-  const int kv_most = KA_ROWS / (2 * PB_KV8_BLOCK * g.hd * ts), q_most = KA_ROWS / (PB_KV8_BLOCK * g.hd * ts);
+  const int kv_most = KA_ROWS / (8 * PB_KV8_BLOCK * g.hd), q_most = KA_ROWS / (PB_KV8_BLOCK * g.hd * ts);
   const int64_t want = 4 * ctx->sm_count / units / 2 + 1;
   auto shares = [&](int heads, int most) {
     const int y = pb_cdiv(heads, most < 1 ? 1 : most);
@@ -1183,11 +1210,12 @@ extern "C" int pb_kv8_read(pb_kv8* kv, const void* pages_dev, const int* starts_
                                          "and no narrower than the heads");
   pb_device_scope dev(ctx->device);
   const int64_t units = kv8_units(n_rows, n_seqs);
-  const int ny = units >= 4 * ctx->sm_count ? 1 : pb_cdiv(2 * g.n_kv, KR_THREADS / 32);
-  return pb_launch(ctx, "k_kv8_read", true, g.code == PB_KV8_INT8 ? k_kv8_read<PB_KV8_INT8> : k_kv8_read<PB_KV8_E4M3>,
-                   dim3((unsigned)units, ny), dim3(KR_THREADS), 0, g,
-                   static_cast<uint8_t*>(const_cast<void*>(pages_dev)), starts_dev, first_dev, table_dev, ld_table, n_seqs,
-                   n_rows, otype, k_out_dev, ldk, v_out_dev, ldv, ctx->d_err);
+  const int most = KR_BYTES / g.block_bytes, least = pb_cdiv(g.n_kv, most < 1 ? 1 : most);
+  const int64_t want = 4 * ctx->sm_count / units + 1;  // shares, where the blocks alone would leave SMs without a CTA
+  const int ny = want <= least ? least : want < g.n_kv ? (int)want : g.n_kv;
+  return pb_launch(ctx, "k_kv8_read", true, kr_kernel_of(g.code, otype), dim3((unsigned)units, ny), dim3(KR_THREADS),
+                   (size_t)pb_cdiv(g.n_kv, ny) * g.block_bytes, g, static_cast<const uint8_t*>(pages_dev), starts_dev, first_dev,
+                   table_dev, ld_table, n_seqs, n_rows, k_out_dev, ldk, v_out_dev, ldv, ctx->d_err);
 }
 
 extern "C" int pb_kv8_attn(pb_kv8* kv, const void* pages_dev, int type, const void* q_dev, int ldq, int n_heads,
