@@ -2,8 +2,8 @@
 // tcgen05 tensor cores.
 //
 // out = softmax(scale Q K^T) V per sequence and head, rows of different
-// sequences packed one after the other.  One pass over the keys in tiles of
-// 128 with a running maximum m and sum l per row (the online softmax):
+// sequences packed one after the other.  One pass over the keys in tiles of 128
+// with a running maximum m and sum l per row (the online softmax):
 //   S = Q K^T;  p = 2^(c S - m), c = scale log2(e);  l += sum p;  O += P V.
 // m is a reference near the maximum, not the maximum itself: it moves (and O
 // and l are scaled down) only when a row's maximum has risen by more than 2^8
@@ -13,22 +13,26 @@
 // output's own rounding; the sum l takes p unrounded.  f16 holds p times 2^7,
 // so p is exact to the type's precision down to 2^-21 of the row's largest.
 //
-// A CTA holds two tiles of 128 query rows that share their keys: two heads of
-// a group at the same rows, or, where the group's size is odd, 256 rows of
-// one head.  While the tensor cores work for one, the other's softmax runs.
-// 12 warps:
-//   warps 0-3, 4-7: the softmax of tile 0 and 1, a thread per row (its TMEM
-//     lane): S from TMEM, p back over the same columns, O / l at the end;
-//   warp 8 lane 0: TMA loads of Q and of the K and V tiles;
-//   warp 9 lane 0: the MMAs.  S (128 columns a tile) and O stay in TMEM; the
-//     second product takes P from TMEM and V as the MN-major operand, so V
-//     needs no transpose;
-//   warps 10, 11: the V tiles that some row must not see whole: rows behind
-//     the sequence's keys become zero (0 * inf would be NaN), and a value that
-//     is not finite under the causal mask sends the CTA's rows, once the rest
-//     is done, through the plain form below, which touches no masked value.
-// The issue order PV(i, j), QK(i, j + 1) of a tile makes the arrival of S for
-// tile j + 1 say that PV(i, j) is complete: the softmax may then scale O.
+// A tile of 128 query rows is a chain: S(j), softmax, P(j), O += P(j) V(j); the
+// softmax goes by halves of 64 keys, and the product of the first half runs
+// beside the exponentials of the second.  (Products of 64 keys in place of 128
+// would shorten the chain, but cost 46 cycles for 32 of arithmetic: measured
+// slower.)  Heads of up to 64 values take one tile a CTA, two CTAs a SM: S, P and
+// O have TMEM columns of their own, S(j + 1) is computed while the softmax is
+// still at tile j's second half, and one CTA's start and end run beside the
+// other's work.  Heads of up to 128 values take two tiles a CTA, which share the
+// K and V tiles (two heads of a group at the same rows, or, where the group's
+// size is odd, 256 rows of one head); P lies over S, and one tile's products run
+// beside the other's softmax.  Warps:
+//   4 per tile: the softmax, a thread per row (its TMEM lane): S from TMEM, p
+//     back to TMEM, O / l at the end;
+//   one lane each for the TMA loads (Q, the K and V tiles) and for the MMAs
+//     (P comes from TMEM, V is the MN-major operand: no transpose);
+//   two: the V tiles that some row must not see whole: rows behind the
+//     sequence's keys become zero (0 * inf would be NaN), and a value that is not
+//     finite under the causal mask sends the CTA's rows, once the rest is done,
+//     through the plain form below, which touches no masked value.
+// A quarter of the exponentials run on the FMA pipe (pa_ex2_poly).
 #include <math.h>
 
 #include "pb_kv8.cuh"
@@ -37,9 +41,11 @@
 namespace {
 
 constexpr int PA_ROWS = 128, PA_KEYS = 128;
-constexpr int PA_THREADS = 384;
 constexpr int PA_PANEL = 128 * 128;  // 128 rows of 64 values, 128-byte swizzled
-constexpr int PA_TMEM = 512;         // S0, S1: columns 0, 128; O0, O1: 256, 256 + head columns
+constexpr int PA_POLY = 2, PA_POLY_OF = 8;  // of so many pairs of exponentials, those that the FMA pipe computes
+// minimax polynomials of 2^r, |r| <= 1/2: relative error 7.5e-5 (bf16's p: half a step is 2e-3) and 2.6e-6 (f16's: 2.4e-4)
+constexpr float PA_P30 = 0.999928057f, PA_P31 = 0.693261087f, PA_P32 = 0.242611334f, PA_P33 = 0.0551713221f;
+constexpr float PA_P40 = 0.999999285f, PA_P41 = 0.693121672f, PA_P42 = 0.240247354f, PA_P43 = 0.0559186637f, PA_P44 = 0.00957053155f;
 constexpr float PA_RISE = 8.0f;      // log2 of the rise that moves a row's reference
 
 struct pa_args {
@@ -47,8 +53,8 @@ struct pa_args {
   void* out;
   const int *qst, *kst;
   int type, ldq, ldk, ldv, ldo, n_seqs, q_rows, k_rows, n_heads, group, hd, causal;
-  int pairs;     // head pairs (or heads) of a row tile
-  int two_rows;  // the CTA's tiles: 0: heads 2i, 2i + 1 at the same rows; 1: rows r, r + 128 of one head
+  int pairs;     // CTAs of a row tile: head pairs, or heads
+  int two_rows;  // two tiles a CTA: 0: heads 2i, 2i + 1 at the same rows; 1: rows r, r + 128 of one head
   float scale;
   float c;       // |scale| * log2(e), not 0
   int neg;       // scale < 0: S = (-Q) K^T
@@ -101,21 +107,41 @@ __device__ __noinline__ void pa_row_plain(const pa_args& a, float* qs, int64_t r
 }
 
 // ---- tensor-core pieces -------------------------------------------------------
-__device__ __forceinline__ void pa_mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
+// The whole warp comes here and the one elected lane (`lead`) issues: values that
+// the warp shares stay in uniform registers, a few instructions an MMA.  Issued
+// from a branch of one lane, an MMA took some 40, and the warp, one of three on
+// its scheduler, could not keep the tensor cores fed beside two softmax warps
+// (with the scheduler saturated, half their rate).
+__device__ __forceinline__ void pa_mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc, uint32_t lead) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(da), "l"(db), "r"(idesc), "r"(acc)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(da), "l"(db), "r"(idesc), "r"(acc), "r"(lead)
       : "memory");
 }
-__device__ __forceinline__ void pa_mma_ts(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void pa_mma_ts(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, uint32_t acc, uint32_t lead) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(db), "r"(idesc), "r"(acc)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(db), "r"(idesc), "r"(acc), "r"(lead)
       : "memory");
+}
+__device__ __forceinline__ void pa_commit(uint64_t* bar, uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(pb_smem_addr(bar)),
+      "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t pa_elect() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
 }
 // MN-major, 128-byte swizzle: 64 values of N in a row of 128 bytes, 8 rows of
 // K in 1024 (stride byte offset), the next 64 values a panel further (leading
@@ -144,6 +170,16 @@ __device__ __forceinline__ void pa_st32(uint32_t taddr, const uint32_t* v) {
       "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void pa_ld8(uint32_t taddr, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(taddr));
+}
+__device__ __forceinline__ void pa_st8(uint32_t taddr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(taddr)
+               : "memory");
+}
 __device__ __forceinline__ void pa_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pa_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pa_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -156,6 +192,62 @@ __device__ __forceinline__ float pa_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// two f32 in one 64-bit register, and their arithmetic
+__device__ __forceinline__ uint64_t pa_two(uint32_t a, uint32_t b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t pa_two(float a, float b) { return pa_two(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ void pa_split(uint64_t x, float& a, float& b) {
+  uint32_t u, v;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(u), "=r"(v) : "l"(x));
+  a = __uint_as_float(u), b = __uint_as_float(v);
+}
+__device__ __forceinline__ uint64_t pa_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t pa_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float pa_max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^x of two values on the FMA pipe: x = n + r, |r| <= 1/2, n by adding 1.5 *
+// 2^23; 2^r by its minimax polynomial; n into the exponent.  Below 2^-126 the
+// result stays at about 2^-126, nothing beside a row's sum (at least 2^-8).
+template <bool BF>
+__device__ __forceinline__ void pa_ex2_poly(uint64_t x, float& y0, float& y1) {
+  float a, b;
+  pa_split(x, a, b);
+  // not fmaxf: a NaN stays one
+  x = pa_two(a < -126.0f ? -126.0f : a, b < -126.0f ? -126.0f : b);
+  const uint64_t n = pa_add2(x, pa_two(12582912.0f, 12582912.0f));
+  const uint64_t r = pa_fma2(pa_add2(n, pa_two(-12582912.0f, -12582912.0f)), pa_two(-1.0f, -1.0f), x);
+  auto c2 = [](float c) { return pa_two(c, c); };
+  uint64_t p;
+  if (BF) {
+    p = pa_fma2(r, c2(PA_P33), c2(PA_P32));
+    p = pa_fma2(r, p, c2(PA_P31));
+    p = pa_fma2(r, p, c2(PA_P30));
+  } else {
+    p = pa_fma2(r, c2(PA_P44), c2(PA_P43));
+    p = pa_fma2(r, p, c2(PA_P42));
+    p = pa_fma2(r, p, c2(PA_P41));
+    p = pa_fma2(r, p, c2(PA_P40));
+  }
+  float p0, p1, n0, n1;
+  pa_split(p, p0, p1);
+  pa_split(n, n0, n1);
+  y0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23));
+  y1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23));
+}
 template <bool BF>
 __device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
   uint32_t r;
@@ -164,35 +256,43 @@ __device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
   return r;
 }
 
-constexpr int pa_stages(int hdp) { return hdp == 128 ? 2 : 4; }
-constexpr size_t pa_smem(int hdp) { return 1024 + (size_t)(2 + 2 * pa_stages(hdp)) * (hdp / 64) * PA_PANEL; }
+constexpr int PA_STAGES = 2;  // of the K and of the V ring
+constexpr int pa_tiles(int hdp) { return hdp == 128 ? 2 : 1; }
+constexpr int pa_threads(int hdp) { return 128 * pa_tiles(hdp) + 128; }
+constexpr size_t pa_smem(int hdp) {
+  return 1024 + (size_t)(hdp / 64) * (pa_tiles(hdp) * PA_PANEL + 2 * PA_STAGES * PA_PANEL);
+}
 
 // HDP: head columns in shared memory and TMEM (64 or 128; TMA fills those past
 // head_dim with zeros), BF: bf16 rows.
 template <int HDP, bool BF>
-__global__ void __launch_bounds__(PA_THREADS, 1)
+__global__ void __launch_bounds__(pa_threads(HDP), HDP == 128 ? 1 : 2)
 k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
               const __grid_constant__ CUtensorMap map_v, const __grid_constant__ pa_args a) {
-  constexpr int NS = pa_stages(HDP), PN = HDP / 64, TILE = PN * PA_PANEL;
+  constexpr int NT = pa_tiles(HDP), T = pa_threads(HDP), NS = PA_STAGES, PN = HDP / 64;
+  constexpr int QT = PN * PA_PANEL, KT = PN * PA_PANEL;  // bytes of a Q tile, of a K or V tile
+  // TMEM columns: S at 128 i; P over S, or (NT == 1) behind it; O last
+  constexpr int TMEM = 256 * NT, P_COL = NT == 1 ? 128 : 0, O_COL = NT == 1 ? 192 : 256;
   constexpr uint32_t FMT = BF ? 1u : 0u;
   constexpr uint32_t IDESC = (1u << 4) | (FMT << 7) | (FMT << 10) | ((uint32_t)(PA_ROWS >> 4) << 24);
   constexpr uint32_t IDESC_QK = IDESC | ((uint32_t)(PA_KEYS >> 3) << 17);
   constexpr uint32_t IDESC_PV = IDESC | ((uint32_t)(HDP >> 3) << 17) | (1u << 16);
   extern __shared__ __align__(1024) unsigned char pa_raw[];
-  __shared__ uint64_t q_full, k_full[NS], k_empty[NS], v_full[NS], v_ready[NS], v_empty[NS], s_full[2], p_full[2], o_full[2];
+  __shared__ uint64_t q_full, k_full[NS], k_empty[NS], v_full[NS], v_mask[NS], v_ready[NS], v_empty[NS], s_full[NT], s_free, p_full[NT][2], o_half[NT][2];
   __shared__ uint32_t tmem_base;
   __shared__ int found, redo;
-  __shared__ float qrow[PA_THREADS / 32][128];
+  __shared__ float qrow[T / 32][128];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pb_pdl_trigger();
   pb_pdl_wait();
 
   // which rows: sequence s has the tile numbers from starts[s] / span + s on
-  const int span = a.two_rows ? 2 * PA_ROWS : PA_ROWS, unit = (int)(gridDim.x - 1 - blockIdx.x);
+  const bool two_rows = NT == 2 && a.two_rows;
+  const int span = two_rows ? 2 * PA_ROWS : PA_ROWS, unit = (int)(gridDim.x - 1 - blockIdx.x);
   const int rt = unit / a.pairs, pair = a.pairs - 1 - unit % a.pairs;
   if (tid == 0) found = -1, redo = 0;
   __syncthreads();
-  for (int s = tid; s < a.n_seqs; s += PA_THREADS) {
+  for (int s = tid; s < a.n_seqs; s += T) {
     const int lo = a.qst[s], hi = a.qst[s + 1];
     if (lo < 0 || hi < lo || hi > a.q_rows) pb_raise(a.err, PB_DEVERR_BOUNDS);
     else if (lo / span + s <= rt && rt < hi / span + s + 1) found = s;
@@ -208,39 +308,43 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
   const int r0 = (rt - (q0 / span + seq)) * span;  // the CTA's first row of the sequence
   if (r0 >= nq) return;
   // tile i: rows row_of(i) .., head head_of(i); row r sees see(r) keys
-  const int kvh = a.two_rows ? pair / a.group : pair / (a.group / 2);
-  auto row_of = [&](int i) { return a.two_rows ? r0 + i * PA_ROWS : r0; };
-  auto head_of = [&](int i) { return a.two_rows ? pair : 2 * pair + i; };
+  const int kvh = NT == 1 || two_rows ? pair / a.group : pair / (a.group / 2);
+  auto row_of = [&](int i) { return two_rows ? r0 + i * PA_ROWS : r0; };
+  auto head_of = [&](int i) { return NT == 1 || two_rows ? pair : 2 * pair + i; };
   auto see = [&](int r) { return a.causal ? max(0, min(nk, nk - nq + r + 1)) : nk; };
   auto tiles_of = [&](int i) {
     const int last = min(nq, row_of(i) + PA_ROWS) - 1;
     return last < row_of(i) ? 0 : (see(last) + PA_KEYS - 1) / PA_KEYS;
   };
-  const int n0 = tiles_of(0), n1 = tiles_of(1), nt = max(n0, n1);
+  const int n0 = tiles_of(0), n1 = NT == 2 ? tiles_of(1) : 0, nt = max(n0, n1);
   const int whole = see(r0) / PA_KEYS;  // key tiles that every row sees whole
 
   unsigned char* base = pa_raw + ((1024 - (pb_smem_addr(pa_raw) & 1023)) & 1023);
-  unsigned char *sQ = base, *sK = sQ + 2 * TILE, *sV = sK + NS * TILE;
-  if (warp == 9) {
+  unsigned char *sQ = base, *sK = sQ + NT * QT, *sV = sK + NS * KT;
+  if (warp == 4 * NT + 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pb_smem_addr(&tmem_base)),
-                 "r"(PA_TMEM)
+                 "r"(TMEM)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (tid == 256) {
+  if (tid == 128 * NT) {
     pb_mbar_init(&q_full, 1);
     for (int s = 0; s < NS; ++s) {
       pb_mbar_init(&k_full[s], 1);
       pb_mbar_init(&k_empty[s], 1);
       pb_mbar_init(&v_full[s], 1);
+      pb_mbar_init(&v_mask[s], 1);
       pb_mbar_init(&v_ready[s], 2);
       pb_mbar_init(&v_empty[s], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < NT; ++i) {
       pb_mbar_init(&s_full[i], 1);
-      pb_mbar_init(&p_full[i], 4);
-      pb_mbar_init(&o_full[i], 1);
+      for (int h = 0; h < 2; ++h) {
+        pb_mbar_init(&p_full[i][h], 4);
+        pb_mbar_init(&o_half[i][h], 1);
+      }
     }
+    pb_mbar_init(&s_free, 4);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   pa_fence_before();
@@ -248,162 +352,195 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
   pa_fence_after();
   const uint32_t tmem = tmem_base;
 
-  if (warp >= 8) {
-    if (warp == 8) {
-      if (lane == 0 && nt > 0) {  // TMA
-        pb_mbar_arrive_tx(&q_full, 2 * TILE);
-        for (int i = 0; i < 2; ++i)
-          for (int p = 0; p < PN; ++p)
-            pb_tma_load_3d(sQ + i * TILE + p * PA_PANEL, &map_q, p * 64, head_of(i), q0 + row_of(i), &q_full);
-        for (int j = 0; j < nt; ++j) {
-          const int s = j % NS, use = j / NS;
-          if (j >= NS && !pb_mbar_wait(&k_empty[s], (use - 1) & 1, a.err)) break;
-          pb_mbar_arrive_tx(&k_full[s], TILE);
-          for (int p = 0; p < PN; ++p)
-            pb_tma_load_3d(sK + s * TILE + p * PA_PANEL, &map_k, p * 64, kvh, k0 + j * PA_KEYS, &k_full[s]);
-          if (j >= NS && !pb_mbar_wait(&v_empty[s], (use - 1) & 1, a.err)) break;
-          pb_mbar_arrive_tx(&v_full[s], TILE);
-          for (int p = 0; p < PN; ++p)
-            pb_tma_load_3d(sV + s * TILE + p * PA_PANEL, &map_v, p * 64, kvh, k0 + j * PA_KEYS, &v_full[s]);
-        }
-      }
-    } else if (warp == 9) {
-      if (lane == 0 && nt > 0) {  // MMA
-        const uint32_t idesc_qk = IDESC_QK | (a.neg ? 1u << 13 : 0u);
-        auto qk = [&](int i, int s) {
-          const uint64_t da = pb_sw128_desc(pb_smem_addr(sQ + i * TILE)), db = pb_sw128_desc(pb_smem_addr(sK + s * TILE));
-#pragma unroll
-          for (int kk = 0; kk < HDP / 16; ++kk) {
-            const uint64_t o = (uint64_t)((kk >> 2) * (PA_PANEL >> 4) + 2 * (kk & 3));
-            pa_mma_ss(tmem + i * 128, da + o, db + o, idesc_qk, kk > 0 ? 1u : 0u);
-          }
-          pb_umma_commit(&s_full[i]);
-        };
-        bool ok = pb_mbar_wait(&q_full, 0, a.err) && pb_mbar_wait(&k_full[0], 0, a.err);
-        if (ok) {
-          if (n0 > 0) qk(0, 0);
-          if (n1 > 0) qk(1, 0);
-          pb_umma_commit(&k_empty[0]);
-        }
-        for (int j = 0; j < nt && ok; ++j) {
-          const int s = j % NS, s1 = (j + 1) % NS;
-          if (j + 1 < nt && !(ok = pb_mbar_wait(&k_full[s1], ((j + 1) / NS) & 1, a.err))) break;
-          if (!(ok = pb_mbar_wait(&v_ready[s], (j / NS) & 1, a.err))) break;
-          for (int i = 0; i < 2; ++i) {
-            const int ni = i ? n1 : n0;
-            if (j >= ni) continue;
-            if (!(ok = pb_mbar_wait(&p_full[i], j & 1, a.err))) break;
-            pa_fence_after();
-            const uint64_t db = pa_desc_mn(pb_smem_addr(sV + s * TILE));
-#pragma unroll
-            for (int kk = 0; kk < PA_KEYS / 16; ++kk)
-              pa_mma_ts(tmem + 256 + i * HDP, tmem + i * 128 + kk * 8, db + (uint64_t)(kk * (2048 >> 4)), IDESC_PV,
-                        (j > 0 || kk > 0) ? 1u : 0u);
-            if (j + 1 < ni) qk(i, s1);
-            else pb_umma_commit(&o_full[i]);
-          }
-          if (!ok) break;
-          pb_umma_commit(&v_empty[s]);
-          if (j + 1 < nt) pb_umma_commit(&k_empty[s1]);
-        }
-      }
-    } else {  // V tiles under a mask
-      const int u = tid - 320;
+  if (warp == 4 * NT) {
+    if (lane == 0 && nt > 0) {  // TMA
+      pb_mbar_arrive_tx(&q_full, NT * QT);
+      for (int i = 0; i < NT; ++i)
+        for (int p = 0; p < PN; ++p)
+          pb_tma_load_3d(sQ + i * QT + p * PA_PANEL, &map_q, p * 64, head_of(i), q0 + row_of(i), &q_full);
       for (int j = 0; j < nt; ++j) {
-        const int s = j % NS;
-        if (!__all_sync(0xffffffffu, pb_mbar_wait(&v_full[s], (j / NS) & 1, a.err))) break;
-        if (j >= whole) {
-          const int keys = nk - j * PA_KEYS;
-          bool bad = false;
-          for (int ch = u; ch < PA_KEYS * PN * 8; ch += 64) {
-            const int row = ch / (PN * 8), col = ch % (PN * 8);
-            uint4* w = reinterpret_cast<uint4*>(sV + s * TILE + (col >> 3) * PA_PANEL + pb_sw128(row, col & 7));
-            if (row >= keys) {
-              *w = make_uint4(0, 0, 0, 0);
-            } else if (a.causal) {
-              uint4 x = *w;
-              uint32_t* e = reinterpret_cast<uint32_t*>(&x);
-              constexpr uint32_t EXP = BF ? 0x7F80u : 0x7C00u;
-              bool hit = false;
-#pragma unroll
-              for (int b = 0; b < 4; ++b) {
-                if ((e[b] & EXP) == EXP) e[b] &= 0xFFFF0000u, hit = true;
-                if ((e[b] & (EXP << 16)) == EXP << 16) e[b] &= 0xFFFFu, hit = true;
-              }
-              if (hit) *w = x, bad = true;
-            }
-          }
-          if (bad) redo = 1;
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
-        __syncwarp();
-        if (lane == 0) pa_arrive(&v_ready[s]);
+        const int s = j % NS, use = j / NS;
+        if (j >= NS && !pb_mbar_wait_sleep(&k_empty[s], (use - 1) & 1, a.err)) break;
+        pb_mbar_arrive_tx(&k_full[s], KT);
+        for (int p = 0; p < PN; ++p)
+          pb_tma_load_3d(sK + s * KT + p * PA_PANEL, &map_k, p * 64, kvh, k0 + j * PA_KEYS, &k_full[s]);
+        if (j >= NS && !pb_mbar_wait_sleep(&v_empty[s], (use - 1) & 1, a.err)) break;
+        uint64_t* full = j < whole ? &v_full[s] : &v_mask[s];  // a tile under a mask goes to the helpers first
+        pb_mbar_arrive_tx(full, KT);
+        for (int p = 0; p < PN; ++p)
+          pb_tma_load_3d(sV + s * KT + p * PA_PANEL, &map_v, p * 64, kvh, k0 + j * PA_KEYS, full);
       }
+    }
+  } else if (warp == 4 * NT + 1) {
+    if (nt > 0) {  // MMA
+      const uint32_t lead = pa_elect(), tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t idesc_qk = IDESC_QK | (a.neg ? 1u << 13 : 0u);
+      auto arrived = [&](uint64_t* bar, int phase) { return __all_sync(0xffffffffu, pb_mbar_wait(bar, phase & 1, a.err)); };
+      bool ok = arrived(&q_full, 0);
+      auto qk = [&](int i, int j) {
+        const uint64_t da = pb_sw128_desc(pb_smem_addr(sQ + i * QT)), db = pb_sw128_desc(pb_smem_addr(sK + j % NS * KT));
+#pragma unroll
+        for (int kk = 0; kk < HDP / 16; ++kk) {
+          const uint64_t o = (uint64_t)((kk >> 2) * (PA_PANEL >> 4) + 2 * (kk & 3));
+          pa_mma_ss(tm + i * 128, da + o, db + o, idesc_qk, kk > 0 ? 1u : 0u, lead);
+        }
+        pa_commit(&s_full[i], lead);
+      };
+      auto pv = [&](int i, int j, int h) {  // half h of the keys
+        const uint64_t db = pa_desc_mn(pb_smem_addr(sV + j % NS * KT));
+#pragma unroll
+        for (int kk = 4 * h; kk < 4 * h + 4; ++kk)
+          pa_mma_ts(tm + O_COL + i * HDP, tm + i * 128 + P_COL + kk * 8, db + (uint64_t)(kk * (2048 >> 4)), IDESC_PV,
+                    (j > 0 || kk > 0) ? 1u : 0u, lead);
+        pa_commit(&o_half[i][h], lead);
+      };
+      ok = ok && arrived(&k_full[0], 0);
+      if (ok) {
+        for (int i = 0; i < NT; ++i)
+          if (0 < (i ? n1 : n0)) qk(i, 0);
+        pa_commit(&k_empty[0], lead);
+      }
+      for (int j = 0; j < nt && ok; ++j) {
+        const int s = j % NS, s1 = (j + 1) % NS;
+        if (j + 1 < nt && !(ok = arrived(&k_full[s1], (j + 1) / NS))) break;
+        // a tile under a mask has been through the helpers' hands
+        if (!(ok = j < whole ? arrived(&v_full[s], j / NS) : arrived(&v_ready[s], (j - whole) / NS))) break;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const int ni = i ? n1 : n0;
+          if (j >= ni) continue;
+          if (!(ok = arrived(&p_full[i][0], j))) break;
+          pa_fence_after();
+          pv(i, j, 0);
+          if (NT == 1 && j + 1 < ni) {  // the softmax has the whole of S(j) in registers
+            if (!(ok = arrived(&s_free, j))) break;
+            pa_fence_after();
+            qk(i, j + 1);
+          }
+          if (!(ok = arrived(&p_full[i][1], j))) break;
+          pa_fence_after();
+          pv(i, j, 1);
+          if (NT == 2 && j + 1 < ni) qk(i, j + 1);  // over P(j), after its product
+        }
+        if (!ok) break;
+        pa_commit(&v_empty[s], lead);
+        if (j + 1 < nt) pa_commit(&k_empty[s1], lead);
+      }
+    }
+  } else if (warp > 4 * NT + 1) {  // V tiles under a mask
+    const int u = tid - 128 * NT - 64;
+    for (int j = whole; j < nt; ++j) {
+      const int s = j % NS, keys = nk - j * PA_KEYS;
+      if (!__all_sync(0xffffffffu, pb_mbar_wait(&v_mask[s], ((j - whole) / NS) & 1, a.err))) break;
+      bool bad = false;
+      for (int ch = u; ch < PA_KEYS * PN * 8; ch += 64) {
+        const int row = ch / (PN * 8), col = ch % (PN * 8);
+        uint4* w = reinterpret_cast<uint4*>(sV + s * KT + (col >> 3) * PA_PANEL + pb_sw128(row, col & 7));
+        if (row >= keys) {
+          *w = make_uint4(0, 0, 0, 0);
+        } else if (a.causal) {
+          uint4 x = *w;
+          uint32_t* e = reinterpret_cast<uint32_t*>(&x);
+          constexpr uint32_t EXP = BF ? 0x7F80u : 0x7C00u;
+          bool hit = false;
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            if ((e[b] & EXP) == EXP) e[b] &= 0xFFFF0000u, hit = true;
+            if ((e[b] & (EXP << 16)) == EXP << 16) e[b] &= 0xFFFFu, hit = true;
+          }
+          if (hit) *w = x, bad = true;
+        }
+      }
+      if (bad) redo = 1;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) pa_arrive(&v_ready[s]);
     }
   } else {
     const int i = warp >> 2, ni = i ? n1 : n0;
     const int r = row_of(i) + (warp & 3) * 32 + lane;  // this thread's row of the sequence
-    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), tS = lanes + i * 128, tO = lanes + 256 + i * HDP;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t tS = lanes + i * 128, tP = tS + P_COL, tO = lanes + O_COL + i * HDP;
     const int sees = see(r), all_see = see(row_of(i));
     constexpr float BIAS = BF ? 0.0f : 7.0f;
     const float c = a.c;
     float m = 0.0f, l = 0.0f;
     bool ok = true;
-    for (int j = 0; j < ni; ++j) {
-      ok = __all_sync(0xffffffffu, pb_mbar_wait(&s_full[i], j & 1, a.err));
-      if (!ok) break;
+    auto arrived = [&](uint64_t* bar, int phase) { return __all_sync(0xffffffffu, pb_mbar_wait(bar, phase & 1, a.err)); };
+    for (int j = 0; j < ni && ok; ++j) {
+      if (!(ok = arrived(&s_full[i], j))) break;
       pa_fence_after();
-      uint32_t sv[128];
-      pa_ld32(tS, sv);
-      pa_ld32(tS + 32, sv + 32);
-      pa_ld32(tS + 64, sv + 64);
-      pa_ld32(tS + 96, sv + 96);
-      pa_wait_ld();
-      if ((j + 1) * PA_KEYS > all_see) {
-        const int lim = sees - j * PA_KEYS;
-#pragma unroll
-        for (int x = 0; x < 128; ++x) sv[x] = x < lim ? sv[x] : 0xFF800000u;
-      }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int x = 0; x < 128; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(sv[x]));
-      const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c, -1e38f);
-      if (j == 0) {
-        m = top;
-      } else {
-        const bool rise = top > m + PA_RISE;
-        if (__any_sync(0xffffffffu, rise)) {  // PV(i, j - 1) is complete: S of this tile was issued after it
-          const float f = rise ? pa_ex2(m - top) : 1.0f;
-          if (rise) m = top, l *= f;
 #pragma unroll 1
-          for (int x = 0; x < HDP; x += 32) {
-            uint32_t o[32];
-            pa_ld32(tO + x, o);
-            pa_wait_ld();
+      for (int h = 0; h < 2; ++h) {
+        uint32_t sv[64];
+        pa_ld32(tS + 64 * h, sv);
+        pa_ld32(tS + 64 * h + 32, sv + 32);
+        pa_wait_ld();
+        if (NT == 1 && h == 1) {
+          pa_fence_before();
+          __syncwarp();
+          if (lane == 0) pa_arrive(&s_free);
+        }
+        const int key0 = j * PA_KEYS + 64 * h;
+        if (key0 + 64 > all_see) {
+          const int lim = sees - key0;
 #pragma unroll
-            for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-            pa_st32(tO + x, o);
+          for (int x = 0; x < 64; ++x) sv[x] = x < lim ? sv[x] : 0xFF800000u;
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int x = 0; x < 64; x += 2)
+          mx[x / 2 & 3] = pa_max3(mx[x / 2 & 3], __uint_as_float(sv[x]), __uint_as_float(sv[x + 1]));
+        const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c, -1e38f);
+        // P(j - 1)'s half, which this one is written over, is used up (where P lies over S, S(j) has said so).  A wait is never
+        // for a phase that the barrier may have passed twice
+        if (NT == 1 && j > 0 && !(ok = arrived(&o_half[i][h], j - 1))) break;
+        if (j == 0 && h == 0) {
+          m = top;
+        } else {
+          const bool rise = top > m + PA_RISE;
+          if (__any_sync(0xffffffffu, rise)) {  // O stands still once the product before is done
+            if (!(ok = h == 0 ? arrived(&o_half[i][1], j - 1) : arrived(&o_half[i][0], j))) break;
+            pa_fence_after();
+            const float f = rise ? pa_ex2(m - top) : 1.0f;
+            if (rise) m = top, l *= f;
+#pragma unroll 1
+            for (int x = 0; x < HDP; x += 8) {  // few registers: the scores are live
+              uint32_t o[8];
+              pa_ld8(tO + x, o);
+              pa_wait_ld();
+#pragma unroll
+              for (int y = 0; y < 8; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+              pa_st8(tO + x, o);
+            }
           }
         }
-      }
-      const float off = BIAS - m;
-      float sum[4] = {0, 0, 0, 0};
+        const uint64_t c2 = pa_two(c, c), off2 = pa_two(BIAS - m, BIAS - m);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
-      for (int x = 0; x < 128; x += 2) {
-        const float p0 = pa_ex2(__fmaf_rn(__uint_as_float(sv[x]), c, off)), p1 = pa_ex2(__fmaf_rn(__uint_as_float(sv[x + 1]), c, off));
-        sum[x & 2] += p0;
-        sum[(x & 2) + 1] += p1;
-        sv[x >> 1] = pa_pack<BF>(p0, p1);
+        for (int x = 0; x < 64; x += 2) {
+          const uint64_t y = pa_fma2(pa_two(sv[x], sv[x + 1]), c2, off2);
+          float p0, p1;
+          if ((x >> 1) % PA_POLY_OF < PA_POLY) {
+            pa_ex2_poly<BF>(y, p0, p1);
+          } else {
+            pa_split(y, p0, p1);
+            p0 = pa_ex2(p0), p1 = pa_ex2(p1);
+          }
+          sum[x >> 1 & 1] = pa_add2(sum[x >> 1 & 1], pa_two(p0, p1));
+          sv[x >> 1] = pa_pack<BF>(p0, p1);
+        }
+        pa_st32(tP + 32 * h, sv);
+        pa_wait_st();
+        pa_fence_before();
+        __syncwarp();
+        if (lane == 0) pa_arrive(&p_full[i][h]);
+        float s0, s1;
+        pa_split(pa_add2(sum[0], sum[1]), s0, s1);
+        l += s0 + s1;
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      pa_st32(tS, sv);
-      pa_st32(tS + 32, sv + 32);
-      pa_wait_st();
-      pa_fence_before();
-      __syncwarp();
-      if (lane == 0) pa_arrive(&p_full[i]);
     }
-    if (ok && ni > 0) ok = pb_mbar_wait(&o_full[i], 0, a.err);
+    if (ok && ni > 0) ok = arrived(&o_half[i][0], ni - 1) && arrived(&o_half[i][1], ni - 1);
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       pa_fence_after();
@@ -433,26 +570,26 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
   }
   pa_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 4 * NT + 1) {
     __syncwarp();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(PA_TMEM) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM) : "memory");
   }
   if (redo) {
-    for (int x = warp; x < 2 * PA_ROWS; x += PA_THREADS / 32) {
+    for (int x = warp; x < NT * PA_ROWS; x += T / 32) {
       const int i = x / PA_ROWS, r = row_of(i) + x % PA_ROWS;
       if (r < nq) pa_row_plain(a, qrow[warp], q0 + r, head_of(i), k0, see(r));
     }
   }
 }
 
-// [rows][heads][hd] of 16-bit values with a row stride of ld, boxes of 128 rows
+// [rows][heads][hd] of 16-bit values with a row stride of ld, boxes of box_rows
 // x 64 values of one head
-int pa_map(pb_ctx* ctx, CUtensorMap* map, bool bf, const void* p, int rows, int heads, int hd, int ld) {
+int pa_map(pb_ctx* ctx, CUtensorMap* map, bool bf, const void* p, int rows, int heads, int hd, int ld, int box_rows) {
   auto enc = pb_tensor_map_encoder(ctx);
   if (!enc) return PB_ERR_CUDA;
   cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows};
   cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)ld * 2};
-  cuuint32_t box[3] = {64, 1, 128};
+  cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = enc(map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(p),
                    dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -496,8 +633,9 @@ extern "C" int pb_attn_packed(pb_ctx* ctx, int type, const void* q_dev, int ldq,
   a.q = q_dev, a.k = k_dev, a.v = v_dev, a.out = out_dev, a.qst = q_starts_dev, a.kst = k_starts_dev;
   a.type = type, a.ldq = ldq, a.ldk = ldk, a.ldv = ldv, a.ldo = ldo, a.n_seqs = n_seqs, a.q_rows = q_rows, a.k_rows = k_rows;
   a.n_heads = n_heads, a.group = n_heads / n_kv, a.hd = head_dim, a.causal = causal;
-  a.two_rows = a.group & 1;
-  a.pairs = a.two_rows ? n_heads : n_heads / 2;
+  const int hdp = head_dim <= 64 ? 64 : 128;
+  a.two_rows = hdp == 128 && (a.group & 1);
+  a.pairs = hdp == 64 || a.two_rows ? n_heads : n_heads / 2;
   a.scale = (float)scale;
   a.neg = scale < 0;
   // a scale of 0 keeps a positive factor: a masked score times it stays -inf
@@ -505,16 +643,16 @@ extern "C" int pb_attn_packed(pb_ctx* ctx, int type, const void* q_dev, int ldq,
   a.err = ctx->d_err;
   const bool bf = type == PB_TYPE_BF16;
   CUtensorMap mq, mk, mv;
-  PB_TRY(pa_map(ctx, &mq, bf, q_dev, q_rows, n_heads, head_dim, ldq));
+  PB_TRY(pa_map(ctx, &mq, bf, q_dev, q_rows, n_heads, head_dim, ldq, PA_ROWS));
   mk = mv = mq;
   if (k_rows > 0) {  // without keys no tile is loaded
-    PB_TRY(pa_map(ctx, &mk, bf, k_dev, k_rows, n_kv, head_dim, ldk));
-    PB_TRY(pa_map(ctx, &mv, bf, v_dev, k_rows, n_kv, head_dim, ldv));
+    PB_TRY(pa_map(ctx, &mk, bf, k_dev, k_rows, n_kv, head_dim, ldk, PA_KEYS));
+    PB_TRY(pa_map(ctx, &mv, bf, v_dev, k_rows, n_kv, head_dim, ldv, PA_KEYS));
   }
   const int64_t grid = ((int64_t)q_rows / (a.two_rows ? 2 * PA_ROWS : PA_ROWS) + n_seqs) * a.pairs;
   if (grid > 0x7FFFFFFF) return pb_set_error(ctx, PB_ERR_ARG, "pb_attn_packed: too many rows and heads for one call");
-  auto kern = head_dim <= 64 ? (bf ? k_attn_packed<64, true> : k_attn_packed<64, false>)
+  auto kern = hdp == 64 ? (bf ? k_attn_packed<64, true> : k_attn_packed<64, false>)
                              : (bf ? k_attn_packed<128, true> : k_attn_packed<128, false>);
-  return pb_launch(ctx, "k_attn_packed", true, kern, dim3((unsigned)grid), dim3(PA_THREADS), pa_smem(head_dim <= 64 ? 64 : 128),
+  return pb_launch(ctx, "k_attn_packed", true, kern, dim3((unsigned)grid), dim3(pa_threads(hdp)), pa_smem(hdp),
                    mq, mk, mv, a);
 }
