@@ -32,7 +32,7 @@
 //     sequence's keys become zero (0 * inf would be NaN), and a value that is not
 //     finite under the causal mask sends the CTA's rows, once the rest is done,
 //     through the plain form below, which touches no masked value.
-// A quarter of the exponentials run on the FMA pipe (pa_ex2_poly).
+// A part of the exponentials run on the FMA pipe (pa_ex2_poly).
 #include <math.h>
 
 #include "pb_kv8.cuh"
@@ -42,7 +42,10 @@ namespace {
 
 constexpr int PA_ROWS = 128, PA_KEYS = 128;
 constexpr int PA_PANEL = 128 * 128;  // 128 rows of 64 values, 128-byte swizzled
-constexpr int PA_POLY = 2, PA_POLY_OF = 8;  // of so many pairs of exponentials, those that the FMA pipe computes
+// Of PA_POLY_OF pairs of exponentials, those that the FMA pipe computes: measured best at 1 for heads up to 64 (whose
+// softmaxes run back to back and fill the issue slots), at 2 to 3 for heads up to 128.
+constexpr int pa_poly(int hdp) { return hdp == 128 ? 2 : 1; }
+constexpr int PA_POLY_OF = 8;
 // minimax polynomials of 2^r, |r| <= 1/2: relative error 7.5e-5 (bf16's p: half a step is 2e-3) and 2.6e-6 (f16's: 2.4e-4)
 constexpr float PA_P30 = 0.999928057f, PA_P31 = 0.693261087f, PA_P32 = 0.242611334f, PA_P33 = 0.0551713221f;
 constexpr float PA_P40 = 0.999999285f, PA_P41 = 0.693121672f, PA_P42 = 0.240247354f, PA_P43 = 0.0559186637f, PA_P44 = 0.00957053155f;
@@ -280,7 +283,10 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
   extern __shared__ __align__(1024) unsigned char pa_raw[];
   __shared__ uint64_t q_full, k_full[NS], k_empty[NS], v_full[NS], v_mask[NS], v_ready[NS], v_empty[NS], s_full[NT], s_free, p_full[NT][2], o_half[NT][2];
   __shared__ uint32_t tmem_base;
-  __shared__ int found, redo;
+  __shared__ int redo;
+  __shared__ struct {
+    int seq, q0, nq, k0, nk;
+  } found;
   __shared__ float qrow[T / 32][128];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pb_pdl_trigger();
@@ -290,17 +296,18 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
   const bool two_rows = NT == 2 && a.two_rows;
   const int span = two_rows ? 2 * PA_ROWS : PA_ROWS, unit = (int)(gridDim.x - 1 - blockIdx.x);
   const int rt = unit / a.pairs, pair = a.pairs - 1 - unit % a.pairs;
-  if (tid == 0) found = -1, redo = 0;
+  if (tid == 0) found.seq = -1, redo = 0;
+  if (warp == 4 * NT && lane < 3)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &map_q : lane == 1 ? &map_k : &map_v) : "memory");
   __syncthreads();
   for (int s = tid; s < a.n_seqs; s += T) {
-    const int lo = a.qst[s], hi = a.qst[s + 1];
+    const int lo = a.qst[s], hi = a.qst[s + 1], kl = a.kst[s], kh = a.kst[s + 1];
     if (lo < 0 || hi < lo || hi > a.q_rows) pb_raise(a.err, PB_DEVERR_BOUNDS);
-    else if (lo / span + s <= rt && rt < hi / span + s + 1) found = s;
+    else if (lo / span + s <= rt && rt < hi / span + s + 1) found = {s, lo, hi - lo, kl, kh - kl};
   }
   __syncthreads();
-  const int seq = found;
-  if (seq < 0) return;
-  const int q0 = a.qst[seq], nq = a.qst[seq + 1] - q0, k0 = a.kst[seq], nk = a.kst[seq + 1] - k0;
+  if (found.seq < 0) return;
+  const int seq = found.seq, q0 = found.q0, nq = found.nq, k0 = found.k0, nk = found.nk;
   if (k0 < 0 || nk < 0 || (int64_t)k0 + nk > a.k_rows) {
     if (tid == 0) pb_raise(a.err, PB_DEVERR_BOUNDS);
     return;
@@ -402,7 +409,6 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
       }
       for (int j = 0; j < nt && ok; ++j) {
         const int s = j % NS, s1 = (j + 1) % NS;
-        if (j + 1 < nt && !(ok = arrived(&k_full[s1], (j + 1) / NS))) break;
         // a tile under a mask has been through the helpers' hands
         if (!(ok = j < whole ? arrived(&v_full[s], j / NS) : arrived(&v_ready[s], (j - whole) / NS))) break;
 #pragma unroll
@@ -413,14 +419,17 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
           pa_fence_after();
           pv(i, j, 0);
           if (NT == 1 && j + 1 < ni) {  // the softmax has the whole of S(j) in registers
-            if (!(ok = arrived(&s_free, j))) break;
+            if (!(ok = arrived(&s_free, j) && arrived(&k_full[s1], (j + 1) / NS))) break;
             pa_fence_after();
             qk(i, j + 1);
           }
           if (!(ok = arrived(&p_full[i][1], j))) break;
           pa_fence_after();
           pv(i, j, 1);
-          if (NT == 2 && j + 1 < ni) qk(i, j + 1);  // over P(j), after its product
+          if (NT == 2 && j + 1 < ni) {  // over P(j), after its product
+            if (!(ok = arrived(&k_full[s1], (j + 1) / NS))) break;
+            qk(i, j + 1);
+          }
         }
         if (!ok) break;
         pa_commit(&v_empty[s], lead);
@@ -461,7 +470,8 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     const int r = row_of(i) + (warp & 3) * 32 + lane;  // this thread's row of the sequence
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t tS = lanes + i * 128, tP = tS + P_COL, tO = lanes + O_COL + i * HDP;
-    const int sees = see(r), all_see = see(row_of(i));
+    // keys that this row sees, and the fewest and most of the warp's rows (0 where none of them is the sequence's)
+    const int w0 = row_of(i) + (warp & 3) * 32, sees = see(r), w_least = see(w0), w_most = w0 < nq ? see(min(nq, w0 + 32) - 1) : 0;
     constexpr float BIAS = BF ? 0.0f : 7.0f;
     const float c = a.c;
     float m = 0.0f, l = 0.0f;
@@ -482,10 +492,23 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
           if (lane == 0) pa_arrive(&s_free);
         }
         const int key0 = j * PA_KEYS + 64 * h;
-        if (key0 + 64 > all_see) {
-          const int lim = sees - key0;
+        if (key0 >= w_most) {  // nothing of these keys for the whole warp
+          if (NT == 1 && j > 0 && !(ok = arrived(&o_half[i][h], j - 1))) break;
 #pragma unroll
-          for (int x = 0; x < 64; ++x) sv[x] = x < lim ? sv[x] : 0xFF800000u;
+          for (int x = 0; x < 32; ++x) sv[x] = 0;
+          pa_st32(tP + 32 * h, sv);
+          pa_wait_st();
+          pa_fence_before();
+          __syncwarp();
+          if (lane == 0) pa_arrive(&p_full[i][h]);
+          continue;
+        }
+        if (key0 + 64 > w_least) {
+          const int lim = sees - key0;  // as two words of bits, which test several scores an instruction
+          const uint32_t see0 = lim >= 32 ? 0xFFFFFFFFu : lim <= 0 ? 0u : (1u << lim) - 1u;
+          const uint32_t see1 = lim >= 64 ? 0xFFFFFFFFu : lim <= 32 ? 0u : (1u << (lim - 32)) - 1u;
+#pragma unroll
+          for (int x = 0; x < 64; ++x) sv[x] = ((x < 32 ? see0 : see1) >> (x & 31)) & 1u ? sv[x] : 0xFF800000u;
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -495,7 +518,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         // P(j - 1)'s half, which this one is written over, is used up (where P lies over S, S(j) has said so).  A wait is never
         // for a phase that the barrier may have passed twice
         if (NT == 1 && j > 0 && !(ok = arrived(&o_half[i][h], j - 1))) break;
-        if (j == 0 && h == 0) {
+        if (key0 == 0) {
           m = top;
         } else {
           const bool rise = top > m + PA_RISE;
@@ -521,7 +544,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         for (int x = 0; x < 64; x += 2) {
           const uint64_t y = pa_fma2(pa_two(sv[x], sv[x + 1]), c2, off2);
           float p0, p1;
-          if ((x >> 1) % PA_POLY_OF < PA_POLY) {
+          if ((x >> 1) % PA_POLY_OF < pa_poly(HDP)) {
             pa_ex2_poly<BF>(y, p0, p1);
           } else {
             pa_split(y, p0, p1);
