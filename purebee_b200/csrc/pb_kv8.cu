@@ -585,7 +585,7 @@ __device__ __forceinline__ bool kt_wait(uint64_t* bar, uint32_t parity, int* err
   return ok || pb_mbar_wait(bar, parity, err);
 }
 
-template <int HD, int CODE, int TR>
+template <int HD, int CODE, int TR, bool LO>
 __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 : 1) k_kv8_attn(kv8_geo g, kt_args a) {
   constexpr int NT = HD / 32, BB = 32 * HD + 16, STAGES = kt_stages(HD);
   constexpr bool HL = TR == 8;
@@ -667,7 +667,7 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
 
   // Q as A fragments in the tiles' order, scaled by the row's largest; qf undoes it
   constexpr bool DIGITS = CODE == PB_KV8_INT8;
-  constexpr int QN = DIGITS && HL ? 6 : 8;  // registers a tile
+  constexpr int QN = HL && !LO ? 4 : DIGITS && HL ? 6 : 8;  // registers a tile
   uint32_t qa[NT][QN];
   float qf[NR];
   int see[NR];  // keys the row sees
@@ -718,8 +718,14 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
             d1 |= (uint32_t)(i1 & 0xFF) << (8 * j);
             d2 |= (uint32_t)(i2 & 0xFF) << (8 * j);
           }
-          if (HL) qa[i][2 * s] = d0, qa[i][2 * s + 1] = d1, qa[i][4 + s] = d2;
+          if (HL) {
+            qa[i][2 * s] = d0, qa[i][2 * s + 1] = d1;
+            if (LO) qa[i][(QN == 6 ? 4 : 0) + s] = d2;
+          }
           else qa[i][2 * s + r] = d0, qa[i][(QN == 8 ? 4 : 0) + 2 * s + r] = d1;
+        } else if (HL && !LO) {
+          qa[i][2 * s] = kt_h2(y[0], y[1]);
+          qa[i][2 * s + 1] = kt_h2(y[2], y[3]);
         } else {
           uint32_t* q4 = &qa[i][(QN == 8 ? 4 : 0) * s];
           q4[r] = kt_h2(y[0], y[1]);
@@ -765,19 +771,21 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
           const uint32_t* q = qa[n];
           kt_mma_s8(ca[0], q[0], q[1], q[2], q[3], w.x, w.y);
           kt_mma_s8(ca[1], q[0], q[1], q[2], q[3], w.z, w.w);
-          if (HL) {
+          if constexpr (HL && LO) {
             kt_mma_s8(cb[0], q[4], 0u, q[5], 0u, w.x, w.y);
             kt_mma_s8(cb[1], q[4], 0u, q[5], 0u, w.z, w.w);
-          } else {
-            kt_mma_s8(cb[0], q[4], q[5], q[QN - 2], q[QN - 1], w.x, w.y);
-            kt_mma_s8(cb[1], q[4], q[5], q[QN - 2], q[QN - 1], w.z, w.w);
+          } else if constexpr (!HL) {
+            kt_mma_s8(cb[0], q[4], q[5], q[6], q[7], w.x, w.y);
+            kt_mma_s8(cb[1], q[4], q[5], q[6], q[7], w.z, w.w);
           }
         }
         const float f0 = qf[0] * ks, f1 = qf[NR - 1] * ks;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int *c = ca[j >> 1], *d = cb[j >> 1], z = j & 1;
-          if (HL) {  // |i1 sum| * 254 + |i2 sum| stays below 2^31 (256 * 127 * 127 * 255)
+          if (HL && !LO) {
+            x0[j] = __fmaf_rn((float)c[2 + z], f0 * (1.0f / 254.0f), (float)c[z] * f0);
+          } else if (HL) {  // |i1 sum| * 254 + |i2 sum| stays below 2^31 (256 * 127 * 127 * 255)
             x0[j] = __fmaf_rn((float)(c[2 + z] * 254 + d[z]), f0 * (1.0f / 64516.0f), (float)c[z] * f0);
           } else {
             x0[j] = __fmaf_rn((float)d[z], f0 * (1.0f / 254.0f), (float)c[z] * f0);
@@ -796,19 +804,20 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
           const uint32_t wa[2] = {w.x, w.y}, wb_[2] = {w.z, w.w};
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const uint32_t* q = &qa[n][(QN == 8 ? 4 : 0) * k];
+            const uint32_t* q = &qa[n][(QN == 8 ? 4 : 2) * k];
+            const uint32_t a0 = q[0], a1 = QN == 8 ? q[1] : 0u, a2 = QN == 8 ? q[QN == 8 ? 2 : 0] : q[1], a3 = QN == 8 ? q[QN == 8 ? 3 : 0] : 0u;
             uint32_t c0, c1;
             kv8_codes<CODE>(wa[k], c0, c1);
-            kt_mma(c[0], q[0], q[1], q[2], q[3], c0, c1);
+            kt_mma(c[0], a0, a1, a2, a3, c0, c1);
             kv8_codes<CODE>(wb_[k], c0, c1);
-            kt_mma(c[1], q[0], q[1], q[2], q[3], c0, c1);
+            kt_mma(c[1], a0, a1, a2, a3, c0, c1);
           }
         }
         const float f0 = qf[0] * ks, f1 = qf[NR - 1] * ks;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float* y = c[j >> 1];
-          x0[j] = (HL ? y[j & 1] + y[2 + (j & 1)] : y[j & 1]) * f0;
+          x0[j] = (HL && LO ? y[j & 1] + y[2 + (j & 1)] : y[j & 1]) * f0;
           if (!HL) x1[j] = y[2 + (j & 1)] * f1;
         }
       }
@@ -885,8 +894,8 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
         pa[h][r] = kt_h2(p[0], p[1]);
         pa[h][2 + r] = kt_h2(p[2], p[3]);
         if (HL) {
-          pa[h][1] = kt_lo2(p[0], p[1], pa[h][0]);
-          pa[h][3] = kt_lo2(p[2], p[3], pa[h][2]);
+          pa[h][1] = LO ? kt_lo2(p[0], p[1], pa[h][0]) : 0u;
+          pa[h][3] = LO ? kt_lo2(p[2], p[3], pa[h][2]) : 0u;
         }
       }
     }
@@ -896,7 +905,7 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) o[n][j][x] *= rescale[HL ? 0 : x >> 1];
+          for (int x = 0; x < (HL && !LO ? 2 : 4); ++x) o[n][j][x] *= rescale[HL ? 0 : x >> 1];
     }
     auto values = [&](const unsigned char* bk, const uint32_t (&p)[4]) {
 #pragma unroll
@@ -936,8 +945,8 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
       float y[8];  // accumulators (j, c0 / c1): values j and 4 + j of the lane's 8
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        y[j] = HL ? o[n][j][0] + o[n][j][2] : o[n][j][2 * r];
-        y[4 + j] = HL ? o[n][j][1] + o[n][j][3] : o[n][j][2 * r + 1];
+        y[j] = HL && LO ? o[n][j][0] + o[n][j][2] : o[n][j][2 * r];
+        y[4 + j] = HL && LO ? o[n][j][1] + o[n][j][3] : o[n][j][2 * r + 1];
       }
       *reinterpret_cast<float4*>(d + 32 * n) = make_float4(y[0], y[1], y[2], y[3]);
       *reinterpret_cast<float4*>(d + 32 * n + 4) = make_float4(y[4], y[5], y[6], y[7]);
@@ -1020,21 +1029,24 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
 }
 
 typedef void (*kt_kernel)(kv8_geo, kt_args);
-template <int HD>
-static kt_kernel kt_pick(int code, int tr) {
-  if (code == PB_KV8_INT8) return tr == 8 ? k_kv8_attn<HD, PB_KV8_INT8, 8> : k_kv8_attn<HD, PB_KV8_INT8, 16>;
-  return tr == 8 ? k_kv8_attn<HD, PB_KV8_E4M3, 8> : k_kv8_attn<HD, PB_KV8_E4M3, 16>;
+template <int HD, int CODE>
+static kt_kernel kt_pick(int tr, bool lo) {
+  return tr == 16 ? k_kv8_attn<HD, CODE, 16, false> : lo ? k_kv8_attn<HD, CODE, 8, true> : k_kv8_attn<HD, CODE, 8, false>;
 }
-static kt_kernel kt_kernel_of(int hd, int code, int tr) {
+template <int HD>
+static kt_kernel kt_pick_code(int code, int tr, bool lo) {
+  return code == PB_KV8_INT8 ? kt_pick<HD, PB_KV8_INT8>(tr, lo) : kt_pick<HD, PB_KV8_E4M3>(tr, lo);
+}
+static kt_kernel kt_kernel_of(int hd, int code, int tr, bool lo) {
   switch (hd) {
-    case 32: return kt_pick<32>(code, tr);
-    case 64: return kt_pick<64>(code, tr);
-    case 96: return kt_pick<96>(code, tr);
-    case 128: return kt_pick<128>(code, tr);
-    case 160: return kt_pick<160>(code, tr);
-    case 192: return kt_pick<192>(code, tr);
-    case 224: return kt_pick<224>(code, tr);
-    default: return kt_pick<256>(code, tr);
+    case 32: return kt_pick_code<32>(code, tr, lo);
+    case 64: return kt_pick_code<64>(code, tr, lo);
+    case 96: return kt_pick_code<96>(code, tr, lo);
+    case 128: return kt_pick_code<128>(code, tr, lo);
+    case 160: return kt_pick_code<160>(code, tr, lo);
+    case 192: return kt_pick_code<192>(code, tr, lo);
+    case 224: return kt_pick_code<224>(code, tr, lo);
+    default: return kt_pick_code<256>(code, tr, lo);
   }
 }
 
@@ -1045,9 +1057,8 @@ int pb_setup_kv8_kernels(void) {
         return PB_ERR_CUDA;
   for (int hd = 32; hd <= 256; hd += 32)
     for (int code = 0; code < 2; ++code)
-      for (int tr = 8; tr <= 16; tr += 8)
-        if (cudaFuncSetAttribute(kt_kernel_of(hd, code, tr), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)kt_smem(hd)) != cudaSuccess)
+      for (auto k : {kt_kernel_of(hd, code, 8, false), kt_kernel_of(hd, code, 8, true), kt_kernel_of(hd, code, 16, false)})
+        if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kt_smem(hd)) != cudaSuccess)
           return PB_ERR_CUDA;
   return PB_OK;
 }
@@ -1235,13 +1246,13 @@ extern "C" int pb_kv8_attn(pb_kv8* kv, const void* pages_dev, int type, const vo
     return pb_set_error(ctx, PB_ERR_ARG, "pb_kv8_attn: rows must be 16-byte aligned, their strides multiples of 16 bytes "
                                          "and no narrower than the heads");
   pb_device_scope dev(ctx->device);
-  // Row tiles of 8 rows with 22-bit queries and probabilities where the rows are f32, or where 8 rows hold a sequence's on
-  // average (the products cost the same); else 16 rows, half the passes over the codes.
+  // Row tiles of 8 rows where the rows are f32 (the products' other 8 rows hold what f16 leaves of them), or where 8 rows
+  // hold a sequence's on average; else 16 rows, half the passes over the codes.
   const int group = n_heads / g.n_kv, tr = type == PB_TYPE_F32 || (int64_t)n_rows * group <= 8 * (int64_t)n_seqs ? 8 : 16;
   kt_args a = {static_cast<const uint8_t*>(pages_dev), q_dev, out_dev, starts_dev, lens_dev, table_dev, type, ldq, ldo,
                n_heads, group, ld_table, n_seqs, n_rows, (float)(scale * 1.4426950408889634), kv->ws, kv->cnt, ctx->d_err};
   if ((int64_t)n_rows * n_heads > 0x7FFFFFFF)
     return pb_set_error(ctx, PB_ERR_ARG, "pb_kv8_attn: too many rows and heads for one call");
-  return pb_launch(ctx, "k_kv8_attn", true, kt_kernel_of(g.hd, g.code, tr), dim3(kv->ctas), dim3(KT_WARPS * 32),
+  return pb_launch(ctx, "k_kv8_attn", true, kt_kernel_of(g.hd, g.code, tr, type == PB_TYPE_F32), dim3(kv->ctas), dim3(KT_WARPS * 32),
                    kt_smem(g.hd), g, a);
 }

@@ -480,7 +480,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     for (int j = 0; j < ni && ok; ++j) {
       if (!(ok = arrived(&s_full[i], j))) break;
       pa_fence_after();
-#pragma unroll 1
+#pragma unroll(NT == 2 ? 2 : 1)
       for (int h = 0; h < 2; ++h) {
         uint32_t sv[64];
         pa_ld32(tS + 64 * h, sv);
