@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(KA_THREADS, 4) k_kv8_append(kv8_geo g, kv8_app
   kv8_unit un;
   if (!kv8_find_unit(a.starts, a.first, a.n_seqs, a.n_rows, blockIdx.x, &found, un, a.err)) return;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
-  const int pos0 = un.blk * PB_KV8_BLOCK, kept = un.lo - pos0, nt = un.hi - un.lo, end = kept + nt;  // new tokens: [kept, end)
+  const int pos0 = un.blk * PB_KV8_BLOCK, kept = un.lo - pos0, nt = un.hi - un.lo;  // new tokens: [kept, kept + nt)
   const int64_t row0 = (int64_t)un.row0 + un.lo - un.first;  // the first one's row
   const int half = ROPE == PB_ROPE_NONE ? 0 : g.rope_dim >> 1;
   const bool kv_part = (int)blockIdx.y < y_kv;
@@ -404,7 +404,9 @@ static kr_kernel kr_kernel_of(int code, int otype) {
 // The rows of a sequence that share a kv head (its new tokens x the head's
 // group) are taken TR at a time: a row tile.  A (sequence, kv head, row tile)
 // is a group; its work is counted in pairs of 16-token blocks, and KT_COST pairs
-// more for what a group costs by itself (measured 4 us against 0.6 us a pair).
+// more for what a group costs by itself (its queries, its pipeline's start, its
+// join: 64 ragged sequences 112.7 us with 6, 103.9 with 16, 106.3 with 30; two
+// long ones 100.3, 97.1, 93.3).
 // All groups, one after the other, are cut into equal ranges, one for each CTA
 // of a single wave, whatever the lengths: a CTA walks its range group by group,
 // finds its place from the lengths on the device (kt_plan; so a recorded graph
@@ -433,7 +435,7 @@ static kr_kernel kr_kernel_of(int code, int otype) {
 // own, so p' uses f16's range whatever V's scales; the sum l runs beside it
 // over 2^(s - m1).  out = O / l * 2^(m2 - m1).
 constexpr int KT_WARPS = 4;
-constexpr int KT_COST = 6;
+constexpr int KT_COST = 20;
 __host__ __device__ constexpr int kt_stages(int hd) { return hd <= 64 ? 4 : 2; }
 constexpr float KT_RISE = 8.0f, KT_BIAS = 6.0f;  // p' <= 2^(8 + 6)
 constexpr float KT_LOW = -1e30f;
@@ -538,16 +540,33 @@ __device__ __forceinline__ void kt_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// A part of a group that this CTA wrote: the group's first CTA and part, its parts and rows.
+struct kt_pend {
+  int c0, first_part, n_parts, row0, rows, len, kvh, rho0;
+};
 // Four values of a row's O under the reference m2, the row's sum l under m1.
 struct kt_sum {
   float4 o = {0, 0, 0, 0};
   float m1 = KT_LOW, m2 = KT_LOW, l = 0.0f;
-  __device__ __forceinline__ void add(const float4& v, const float4& m) {
-    const float n1 = fmaxf(m1, m.x), n2 = fmaxf(m2, m.y);
-    const float f1 = kt_ex2(m1 - n1), g1 = kt_ex2(m.x - n1), f2 = kt_ex2(m2 - n2), g2 = kt_ex2(m.y - n2);
-    l = l * f1 + m.z * g1;
-    o.x = o.x * f2 + v.x * g2, o.y = o.y * f2 + v.y * g2, o.z = o.z * f2 + v.z * g2, o.w = o.w * f2 + v.w * g2;
+  // n parts' values at p, p + stride, ..., their {m1, m2, l} `m` floats further: the references first, so that the sums
+  // depend on one another by an addition only
+  __device__ __forceinline__ void add(const float* p, int stride, int m, int n) {
+    float n1 = m1, n2 = m2;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float2 v = *reinterpret_cast<const float2*>(p + i * stride + m);
+      n1 = fmaxf(n1, v.x), n2 = fmaxf(n2, v.y);
+    }
+    const float f1 = kt_ex2(m1 - n1), f2 = kt_ex2(m2 - n2);
     m1 = n1, m2 = n2;
+    l *= f1, o.x *= f2, o.y *= f2, o.z *= f2, o.w *= f2;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float4 v = *reinterpret_cast<const float4*>(p + i * stride + m), x = *reinterpret_cast<const float4*>(p + i * stride);
+      const float w = kt_ex2(v.y - n2);
+      l = __fmaf_rn(v.z, kt_ex2(v.x - n1), l);
+      o.x = __fmaf_rn(x.x, w, o.x), o.y = __fmaf_rn(x.y, w, o.y), o.z = __fmaf_rn(x.z, w, o.z), o.w = __fmaf_rn(x.w, w, o.w);
+    }
   }
 };
 // out of a row's four values at d: O / l * 2^(m2 - m1)
@@ -594,6 +613,7 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
   extern __shared__ __align__(16) unsigned char kt_raw[];
   __shared__ uint64_t full[KT_WARPS][STAGES];
   __shared__ uint64_t part_bar;
+  __shared__ kt_pend pend[2];
   __shared__ unsigned int last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t = lane & 3;
   if (lane == 0) {
@@ -609,6 +629,7 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
   const int nblk_log2 = 31 - __clz(g.nblk);
   int used = 0;              // pairs that this warp has been through: its ring's place
   uint32_t part_phase = 0;   // of part_bar
+  int n_pend = 0;            // parts to announce
   for (long long u = rg.lo; u < rg.hi;) {
   {
     long long n;
@@ -962,9 +983,7 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
     for (int j = 0; j < J; ++j) {
       const int x = tid + T * j;
       if (x < live * COLS) {
-        const float* p = reinterpret_cast<const float*>(kt_raw) + 4 * x;
-        for (int i = 0; i < n; ++i, p += SLOT)
-          acc[j].add(*reinterpret_cast<const float4*>(p), *reinterpret_cast<const float4*>(p - 4 * x + TR * HD + x / COLS * 4));
+        acc[j].add(reinterpret_cast<const float*>(kt_raw) + 4 * x, SLOT, TR * HD + x / COLS * 4 - 4 * x, n);
       }
     }
   };
@@ -991,40 +1010,60 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
         if (x % COLS == 0) __stcg(reinterpret_cast<float4*>(part + TR * HD + x / COLS * 4), make_float4(acc[j].m1, acc[j].m2, acc[j].l, 0.0f));
       }
     }
-    const int first_part = 2 * c0 + (u0 == c0 * rg.per ? 0 : 1);
-    __threadfence();
-    __syncthreads();
+    // Announced at the range's end: a fence here, with the memory busy, took 8 to 11 us.  (A CTA that ends with the group it
+    // began with announces once.)
+    if (tid == 0) pend[n_pend] = {c0, 2 * c0 + (u0 == c0 * rg.per ? 0 : 1), n_parts, row0, rows, len, kvh, rho0};
+    ++n_pend;
+  }
+  // the ring, which the joins used, is free again
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncthreads();
+  }
+  // ---- the parts: the last CTA of a group to come adds them ------------------------
+  if (n_pend == 0) return;
+  __threadfence();
+  __syncthreads();
+  for (int k = 0; k < n_pend; ++k) {
+    const kt_pend& pd = pend[k];
     if (tid == 0) {
-      last = atomicAdd(a.cnt + first_part, 1u) == (unsigned)n_parts - 1 ? 1u : 0u;
-      if (last) a.cnt[first_part] = 0;  // for the next call
+      last = atomicAdd(a.cnt + pd.first_part, 1u) == (unsigned)pd.n_parts - 1 ? 1u : 0u;
+      if (last) a.cnt[pd.first_part] = 0;  // for the next call
     }
     __syncthreads();
-    if (last) {  // all parts, by bulk copies into the ring as many at a time as it holds
+    if (last) {  // by bulk copies into the ring, as many at a time as it holds
       constexpr int HOLD = (int)(KT_WARPS * STAGES * 2 * BB / (SLOT * sizeof(float)));
+      constexpr int T = KT_WARPS * 32, COLS = HD / 4, J = (TR * COLS + T - 1) / T;
+      const int live = min(TR, pd.rows - pd.rho0);
+      kt_sum acc[J];
       __threadfence();
-#pragma unroll
-      for (int j = 0; j < J; ++j) acc[j] = kt_sum();
-      for (int i0 = 0; i0 < n_parts; i0 += HOLD) {
-        const int n = min(HOLD, n_parts - i0);
-        if (tid == 0) {
+      for (int i0 = 0; i0 < pd.n_parts; i0 += HOLD) {
+        const int n = min(HOLD, pd.n_parts - i0);
+        if (warp == 0) {
           asm volatile("fence.proxy.async;" ::: "memory");
-          pb_mbar_arrive_tx(&part_bar, n * SLOT * 4);
-          for (int i = 0; i < n; ++i)
-            pb_bulk_g2s(kt_raw + (size_t)i * SLOT * 4, a.ws + (size_t)(i0 + i == 0 ? first_part : 2 * (c0 + i0 + i)) * SLOT,
-                        SLOT * 4, &part_bar);
+          if (lane == 0) pb_mbar_arrive_tx(&part_bar, n * SLOT * 4);
+          __syncwarp();
+          for (int i = lane; i < n; i += 32)
+            pb_bulk_g2s(kt_raw + (size_t)i * SLOT * 4,
+                        a.ws + (size_t)(i0 + i == 0 ? pd.first_part : 2 * (pd.c0 + i0 + i)) * SLOT, SLOT * 4, &part_bar);
         }
         pb_mbar_wait(&part_bar, part_phase, a.err);
         part_phase ^= 1;
-        add_parts(n);
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const int x = tid + T * j;
+          if (x < live * COLS)
+            acc[j].add(reinterpret_cast<const float*>(kt_raw) + 4 * x, SLOT, TR * HD + x / COLS * 4 - 4 * x, n);
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
       }
-      finish();
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int x = tid + T * j;
+        if (x < live * COLS) kt_finish(g, a, pd.row0, pd.rows, pd.len, pd.kvh, pd.rho0 + x / COLS, x % COLS * 4, acc[j]);
+      }
     }
-  }
-  // the ring, which the joins used, and `last` are free again
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  __syncthreads();
+    __syncthreads();  // `last` and the ring are free again
   }
 }
 
@@ -1239,12 +1278,14 @@ extern "C" int pb_kv8_attn(pb_kv8* kv, const void* pages_dev, int type, const vo
   PB_TRY(kv8_check_call(kv, "pb_kv8_attn", pages_dev, starts_dev, lens_dev, table_dev, ld_table, n_seqs, n_rows, &done));
   const int ts = pb_type_size(type);
   if (!ts) return pb_set_error(ctx, PB_ERR_ARG, "pb_kv8_attn: rows are f32, f16 or bf16");
-  if (n_heads <= 0 || n_heads % g.n_kv || n_heads > (1 << 15) || !isfinite(scale))
-    return pb_set_error(ctx, PB_ERR_ARG, "pb_kv8_attn: n_heads must be a multiple of the cache's %d kv heads, scale finite", g.n_kv);
+  if (n_heads <= 0 || n_heads % g.n_kv || n_heads > (1 << 15) || !(fabs(scale) <= 1e30))
+    return pb_set_error(ctx, PB_ERR_ARG, "pb_kv8_attn: n_heads must be a multiple of the cache's %d kv heads, scale at most "
+                                         "1e30 in size", g.n_kv);
   if (done) return PB_OK;
   if (!pb_rows_ok(q_dev, ldq, n_heads * g.hd, ts) || !pb_rows_ok(out_dev, ldo, n_heads * g.hd, ts))
     return pb_set_error(ctx, PB_ERR_ARG, "pb_kv8_attn: rows must be 16-byte aligned, their strides multiples of 16 bytes "
                                          "and no narrower than the heads");
+  if (out_dev == q_dev) return pb_set_error(ctx, PB_ERR_ARG, "pb_kv8_attn: the output is an array of its own");
   pb_device_scope dev(ctx->device);
   // Row tiles of 8 rows where the rows are f32 (the products' other 8 rows hold what f16 leaves of them), or where 8 rows
   // hold a sequence's on average; else 16 rows, half the passes over the codes.

@@ -640,7 +640,7 @@ extern "C" int pb_attn_packed(pb_ctx* ctx, int type, const void* q_dev, int ldq,
   if (type != PB_TYPE_F16 && type != PB_TYPE_BF16)
     return pb_set_error(ctx, PB_ERR_ARG, "pb_attn_packed: rows are f16 or bf16");
   if (n_seqs < 0 || n_seqs > (1 << 20) || q_rows < 0 || k_rows < 0 || q_rows > (1 << 30) || k_rows > (1 << 30) ||
-      n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || n_heads > 65535 || (causal != 0 && causal != 1) || !isfinite(scale))
+      n_heads <= 0 || n_kv <= 0 || n_heads % n_kv || n_heads > 65535 || (causal != 0 && causal != 1) || !(fabs(scale) <= 1e30))
     return pb_set_error(ctx, PB_ERR_ARG, "pb_attn_packed: bad sizes (%d sequences, %d and %d rows, %d heads over %d)", n_seqs,
                         q_rows, k_rows, n_heads, n_kv);
   if (head_dim <= 0 || head_dim % 8 || head_dim > 128)
@@ -651,6 +651,8 @@ extern "C" int pb_attn_packed(pb_ctx* ctx, int type, const void* q_dev, int ldq,
       (k_rows > 0 && (!pb_rows_ok(k_dev, ldk, n_kv * head_dim, 2) || !pb_rows_ok(v_dev, ldv, n_kv * head_dim, 2))))
     return pb_set_error(ctx, PB_ERR_ARG, "pb_attn_packed: rows must be 16-byte aligned, their strides multiples of 16 bytes "
                                          "and no narrower than the heads");
+  if (out_dev == q_dev || (k_rows > 0 && (out_dev == k_dev || out_dev == v_dev)))
+    return pb_set_error(ctx, PB_ERR_ARG, "pb_attn_packed: the output is an array of its own");
   pb_device_scope dev(ctx->device);
   pa_args a = {};
   a.q = q_dev, a.k = k_dev, a.v = v_dev, a.out = out_dev, a.qst = q_starts_dev, a.kst = k_starts_dev;

@@ -221,6 +221,22 @@ def test_attention_long_split(native, ctx, code, t, n, nh):
     assert np.array_equal(b, c) and np.isfinite(a).all()  # the same bits each time
 
 
+@pytest.mark.parametrize("t,nh", [("f32", 4), ("bf16", 24)])
+def test_attention_many_sequences(native, ctx, t, nh):
+    """More sequences than a CTA has threads, many without rows or without tokens, some with several rows."""
+    rng = np.random.default_rng(20)
+    n = 300
+    lens = rng.integers(0, 40, n)
+    lens[rng.random(n) < 0.2] = 0
+    lens[7], lens[299] = 900, 333
+    rows = rng.integers(0, 3, n)
+    p = Pool(native, ctx, 0, 2, 32, 16, n, 900, seed=21)
+    p.append(lens.tolist(), [0] * n, 2)
+    p.check_attn(nh, rows.tolist(), lens.tolist(), t)
+    p.append(rows.tolist(), lens.tolist(), 2)
+    p.check()
+
+
 @pytest.mark.parametrize("t", ["f32", "f16"])
 def test_attention_uneven_scales(native, ctx, t):
     """Blocks of V whose scales lie far apart, a peaked softmax on the small ones, large keys, scale 0 and negative."""
@@ -344,7 +360,7 @@ def test_refusals(native, ctx):
     ok = dict(pages=p.pages.ptr, type_=0, q=x.ptr, ldq=256, n_heads=4, starts=i.ptr, lens=i.ptr, table=p.table.ptr,
               ld_table=p.ld, n_seqs=1, n_rows=1, scale=1.0, out=o.ptr, ldo=256)
     for b in (dict(n_heads=3), dict(n_heads=0), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(ldq=129),
-              dict(out=o.ptr + 2), dict(type_=8), dict(lens=None), dict(ld_table=-1)):
+              dict(out=o.ptr + 2), dict(out=x.ptr), dict(scale=1e39), dict(type_=8), dict(lens=None), dict(ld_table=-1)):
         with pytest.raises(N.PureBeeError, match="PB_ERR_ARG"):
             p.kv.attn(**{**ok, **b})
     ok = dict(pages=p.pages.ptr, starts=i.ptr, first=i.ptr, table=p.table.ptr, ld_table=p.ld, n_seqs=1, n_rows=1, otype=0,

@@ -146,16 +146,61 @@ def test_packed_replayed(native, ctx):
             at += c
 
 
+def test_packed_many_sequences(native, ctx):
+    """More sequences than a CTA has threads, of a few rows each, some empty."""
+    rng = np.random.default_rng(14)
+    n = rng.integers(0, 5, 900)
+    check(native, ctx, "f16", n, n + rng.integers(0, 3, 900), 2, 1, 64, seed=15)
+    check(native, ctx, "bf16", n[:450], n[:450], 2, 1, 128, seed=16)
+
+
+def test_packed_same_bits(native, ctx):
+    rng = np.random.default_rng(17)
+    q, k, v = rng.standard_normal((700, 4, 128)), rng.standard_normal((700, 2, 128)), rng.standard_normal((700, 2, 128))
+    a = [run(native, ctx, "bf16", q, k, v, [300, 400], [300, 400], True, 0.2)[0] for _ in range(3)]
+    assert np.array_equal(a[0], a[1]) and np.array_equal(a[0], a[2])
+
+
+def test_packed_rows_past_31_bits(native, ctx):
+    """Rows whose elements lie past 2^31, behind unused ones."""
+    hd, nh, rows, n = 64, 2, 560000, 70
+    ld = 4096
+    rng = np.random.default_rng(18)
+    bufs = [ctx.alloc(rows * ld * 2) for _ in range(2)]  # q and k side by side in one, v in the other
+    x = rng.standard_normal((3, n, nh, hd)).astype(np.float16)
+    at = rows - n - 3
+    tail = np.zeros((n, ld), np.float16)
+    tail[:, :nh * hd], tail[:, 512:512 + nh * hd] = x[0].reshape(n, -1), x[1].reshape(n, -1)
+    L = native.lib()
+    ctx._check(L.pb_upload(ctx.h, bufs[0].ptr + at * ld * 2, native.ptr(tail), tail.nbytes))
+    tail2 = np.zeros((n, ld), np.float16)
+    tail2[:, :nh * hd] = x[2].reshape(n, -1)
+    ctx._check(L.pb_upload(ctx.h, bufs[1].ptr + at * ld * 2, native.ptr(tail2), tail2.nbytes))
+    st = ctx.to_device(np.array([at, at + n], np.int32))
+    o = 1024 * 2  # the output beside v
+    ctx.attn_packed(native.TYPE_F16, bufs[0].ptr, ld, bufs[0].ptr + 1024, ld, bufs[1].ptr, ld, st.ptr, st.ptr, 1, rows, rows, nh, nh,
+                    hd, 0.125, 1, bufs[1].ptr + o, ld)
+    ctx.sync()
+    out = np.empty((n, ld), np.float16)
+    ctx._check(L.pb_download(ctx.h, native.ptr(out), bufs[1].ptr + at * ld * 2, out.nbytes))
+    got = out[:, 1024:1024 + nh * hd].reshape(n, nh, hd).astype(np.float64)
+    a = [y.astype(np.float64) for y in x]
+    w, mag, dots = R.attention(*a, 0.125)
+    tol = R.attention_tolerance(w, mag, dots, hd, n, "f16", 2.0 ** -11) + 2.0 ** -25 * np.abs(a[2]).sum()
+    assert not R.differs(got, w, tol, "f16").any()
+
+
 def test_packed_refusals(native, ctx):
     N = native
     b, i = ctx.alloc(1 << 16), ctx.to_device(np.array([0, 4], np.int32))
+    o = ctx.alloc(1 << 16)
     ok = dict(type_=N.TYPE_F16, q=b.ptr, ldq=256, k=b.ptr, ldk=128, v=b.ptr, ldv=128, q_starts=i.ptr, k_starts=i.ptr, n_seqs=1,
-              q_rows=4, k_rows=4, n_heads=4, n_kv=2, head_dim=64, scale=1.0, causal=1, out=b.ptr, ldo=256)
+              q_rows=4, k_rows=4, n_heads=4, n_kv=2, head_dim=64, scale=1.0, causal=1, out=o.ptr, ldo=256)
     n0 = ctx.launches
     for bad in (dict(type_=0), dict(type_=2), dict(q=None), dict(k=b.ptr + 2), dict(v=None), dict(ldq=252), dict(ldk=132),
                 dict(ldv=64), dict(out=None), dict(ldo=128), dict(q_starts=None), dict(k_starts=None), dict(n_seqs=-1),
                 dict(q_rows=-1), dict(n_heads=3), dict(n_kv=0), dict(head_dim=136), dict(head_dim=60), dict(head_dim=0),
-                dict(scale=float("inf")), dict(causal=2)):
+                dict(scale=float("inf")), dict(scale=-1e31), dict(causal=2), dict(out=b.ptr)):
         with pytest.raises(N.PureBeeError, match="PB_ERR_ARG"):
             ctx.attn_packed(**{**ok, **bad})
     for none in (dict(n_seqs=0), dict(q_rows=0)):
