@@ -500,8 +500,9 @@ int pb_batch_set_precision(pb_batch* b, int terms);
  * (ld*) count elements; row arrays are 16-byte aligned with strides of a
  * multiple of 16 bytes.  Types: PB_TYPE_F32, PB_TYPE_F16, PB_TYPE_BF16.
  *
- * A table entry or a length that does not fit the pool raises the device
- * error word (index out of bounds): what it covers is not read or written. */
+ * A table entry, a length or a start that does not fit raises the device error
+ * word (index out of bounds): no page is written for it, and nothing outside
+ * the pool and the row arrays is touched; the rows it covers are unspecified. */
 #define PB_KV8_INT8 0 /* codes -127 .. 127 */
 #define PB_KV8_E4M3 1 /* 8-bit floats, 448 the largest */
 #define PB_KV8_BLOCK 16
@@ -524,8 +525,10 @@ typedef struct pb_kv8_config {
 /* Bytes of one layer's pool, -1 for a bad configuration.  Host only.  A pool's
  * bytes need no initialisation: a block is written whole before it is read. */
 int64_t pb_kv8_pool_bytes(const pb_kv8_config* c);
-/* The handle: geometry, frequencies and a workspace; it serves any number of
- * pools.  Its calls run on ctx's stream; free it before the context. */
+/* The handle: geometry and frequencies; it serves any number of pools.  Its
+ * calls run on ctx's stream, and so do graphs that hold them: pb_kv8_attn's
+ * workspace is the context's.  Not while recording; free it after the graphs
+ * that use it and before the context. */
 int pb_kv8_create(pb_ctx* ctx, const pb_kv8_config* c, pb_kv8** out);
 int pb_kv8_free(pb_kv8* kv);
 /* Append: rows k_dev, v_dev [n_kv_heads * head_dim] of sequence s become its
@@ -539,8 +542,8 @@ int pb_kv8_free(pb_kv8* kv);
  * q_dev [n_heads * head_dim] (optional, with q_out_dev) is rotated into
  * q_out_dev; k_out_dev, v_out_dev (optional) get the rotated k and v without
  * the coding, for pb_attn_packed.  Outputs are of type otype and may not
- * overlap the inputs.  A page that two sequences share is read by both, but
- * appended to by none. */
+ * overlap the inputs or each other.  A page that two sequences share (or that
+ * is twice in a table) is read by both, but appended to by none. */
 int pb_kv8_append(pb_kv8* kv, void* pages_dev, int type, const void* q_dev, int ldq, const void* k_dev, int ldk,
                   const void* v_dev, int ldv, int n_heads, const int* starts_dev, const int* past_dev,
                   const int* table_dev, int ld_table, int n_seqs, int n_rows, int otype, void* q_out_dev, int ldqo,
@@ -557,7 +560,8 @@ int pb_kv8_read(pb_kv8* kv, const void* pages_dev, const int* starts_dev, const 
  * being cached with them; each sees the tokens up to its own, kv head h /
  * (n_heads / n_kv_heads) for head h.  out = sum_j softmax_j(scale q.k_j) v_j
  * with f32 sums; a row that sees no token (lens_dev[s] less than its rows)
- * gets zeros.  q_dev and out_dev [n_rows][n_heads * head_dim] are of one type. */
+ * gets zeros.  q_dev and out_dev [n_rows][n_heads * head_dim] are of one type
+ * and do not overlap. */
 int pb_kv8_attn(pb_kv8* kv, const void* pages_dev, int type, const void* q_dev, int ldq, int n_heads,
                 const int* starts_dev, const int* lens_dev, const int* table_dev, int ld_table, int n_seqs, int n_rows,
                 double scale, void* out_dev, int ldo);
@@ -568,7 +572,8 @@ int pb_kv8_attn(pb_kv8* kv, const void* pages_dev, int type, const void* q_dev, 
  * tokens, query i of nq sees keys up to nk - nq + i; 0: all of them.  A query
  * that sees no key gets zeros.  f16 or bf16 rows and output, f32 scores and
  * sums, the probabilities rounded to the rows' type; head_dim a multiple of 8,
- * up to 128.  q_starts_dev and k_starts_dev may be one array. */
+ * up to 128.  q_starts_dev and k_starts_dev may be one array; out_dev overlaps
+ * no input. */
 int pb_attn_packed(pb_ctx* ctx, int type, const void* q_dev, int ldq, const void* k_dev, int ldk, const void* v_dev,
                    int ldv, const int* q_starts_dev, const int* k_starts_dev, int n_seqs, int q_rows, int k_rows,
                    int n_heads, int n_kv, int head_dim, double scale, int causal, void* out_dev, int ldo);

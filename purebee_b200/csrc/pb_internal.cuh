@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include <string>
+#include <vector>
 
 #include "../../include/purebee_cuda.h"
 
@@ -31,6 +32,10 @@ struct pb_ctx {
   size_t gemm_scratch_bytes = 0;
   // fixed per-device array of pb_attention_noalloc (looked up in pb_init)
   void* noalloc_attn = nullptr;
+  // workspaces of pb_kv8_attn, the last one the largest (pb_kv8_create adds one where a handle needs more; none is freed
+  // before the context, so recorded graphs stay valid)
+  std::vector<void*> kv8_ws;
+  size_t kv8_ws_bytes = 0;
 };
 
 // Device layouts of a quantized matrix (payload and scales split apart, so

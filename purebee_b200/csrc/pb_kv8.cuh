@@ -46,7 +46,7 @@ struct pb_kv8 {
   kv8_geo g;
   double* freqs = nullptr;  // [3][128] by pair: frequency f, cos f, sin f
   // parts of the groups that pb_kv8_attn splits and their arrival counters (zero
-  // between calls); fixed, so recorded graphs stay valid
+  // between calls): the context's, whose calls come one after the other
   float* ws = nullptr;
   unsigned int* cnt = nullptr;
   int ctas = 0;  // of pb_kv8_attn

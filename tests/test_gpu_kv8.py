@@ -371,6 +371,51 @@ def test_refusals(native, ctx):
     assert ctx.launches == n0
 
 
+def test_refusals_of_outputs_that_are_other_arrays_too(native, ctx):
+    p = Pool(native, ctx, 0, 2, 64, 16, 1, 32)
+    q, k, v, o, o2 = (ctx.alloc(1 << 12) for _ in range(5))
+    i = p.ints([0, 1])
+    ok = dict(pages=p.pages.ptr, type_=0, q=q.ptr, ldq=256, k=k.ptr, ldk=128, v=v.ptr, ldv=128, n_heads=4, starts=i.ptr,
+              past=i.ptr, table=p.table.ptr, ld_table=p.ld, n_seqs=1, n_rows=1, otype=1, q_out=o.ptr, ldqo=256)
+    n0 = ctx.launches
+    for b in (dict(q_out=k.ptr), dict(q_out=v.ptr), dict(k_out=q.ptr), dict(k_out=v.ptr), dict(k_out=o.ptr), dict(v_out=v.ptr),
+              dict(v_out=k.ptr), dict(v_out=o.ptr), dict(k_out=o2.ptr, v_out=o2.ptr)):
+        with pytest.raises(native.PureBeeError, match="PB_ERR_ARG"):
+            p.kv.append(**{**ok, "ldko": 128, "ldvo": 128, **b})
+    with pytest.raises(native.PureBeeError, match="PB_ERR_ARG"):
+        p.kv.read(p.pages.ptr, i.ptr, i.ptr, p.table.ptr, p.ld, 1, 1, 0, o.ptr, 128, o.ptr, 128)
+    assert ctx.launches == n0
+
+
+def test_handles_share_the_workspace(native, ctx):
+    """Handles of several head sizes, made and used in turn on one context, and recorded into one graph: the same bits."""
+    lens, pools = [900, 40], []
+    for hd in (64, 256, 32):
+        p = Pool(native, ctx, 0, 2, hd, 16, 2, 900, seed=hd)
+        p.append(lens, [0, 0], 2)
+        p.check_attn(4, [3, 1], lens, "f32")
+        p.q, p.out = ctx.to_device(p.rng.standard_normal((4, 4 * hd)).astype(np.float32)), ctx.alloc(4 * 4 * 4 * hd)
+        p.st, p.ln = p.ints([0, 3, 4]), p.ints(lens)
+        pools.append(p)
+
+    def step():
+        for p in pools:
+            p.kv.attn(p.pages.ptr, 0, p.q.ptr, 4 * p.hd, 4, p.st.ptr, p.ln.ptr, p.table.ptr, p.ld, 2, 4, 0.1, p.out.ptr, 4 * p.hd)
+
+    step()
+    want = [p.out.download().copy() for p in pools]
+    graph = ctx.capture(step)
+    for _ in range(2):
+        for p in pools:
+            p.out.upload(np.full(16 * p.hd, 9, np.float32))
+        graph.launch()
+        step()
+        graph.launch()
+        for p, w in zip(pools, want):
+            np.testing.assert_array_equal(p.out.download(), w)
+    graph.free()
+
+
 @pytest.mark.parametrize("what", ["page", "negative page", "length", "rows", "past"])
 def test_bad_device_state_raises_the_error_word(native, what):
     """Tables, lengths and row bounds that do not fit: an error word, nothing written outside."""
