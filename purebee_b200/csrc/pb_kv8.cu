@@ -405,8 +405,8 @@ static kr_kernel kr_kernel_of(int code, int otype) {
 // group) are taken TR at a time: a row tile.  A (sequence, kv head, row tile)
 // is a group; its work is counted in pairs of 16-token blocks, and KT_COST pairs
 // more for what a group costs by itself (its queries, its pipeline's start, its
-// join: 64 ragged sequences 112.7 us with 6, 103.9 with 16, 106.3 with 30; two
-// long ones 100.3, 97.1, 93.3).
+// join: 64 ragged sequences 111.2 us with 10, 108 with 20 to 36, 116 with 96; two
+// long ones 97.6, 93.2, 94.7; drafted tokens 80.8, 77.9 (74.7 with 36), 80.4).
 // All groups, one after the other, are cut into equal ranges, one for each CTA
 // of a single wave, whatever the lengths: a CTA walks its range group by group,
 // finds its place from the lengths on the device (kt_plan; so a recorded graph
@@ -415,7 +415,9 @@ static kr_kernel kr_kernel_of(int code, int otype) {
 // A warp takes every KT_WARPS-th pair through a ring of its own, one bulk copy
 // a pair (a block's K codes, V codes and scales are contiguous, and so are a
 // page's blocks of a head), and keeps running maximum, sum and output of its
-// rows; the warps join in shared memory.
+// rows; the warps join in shared memory.  A pair without a mask and with plain
+// scales takes a way without branches, both blocks' products side by side
+// (drafted tokens 82 -> 78 us, 64 ragged with heads of 64 values 72 -> 62).
 //
 // Rows of the products' M = 16 that a tile of 8 rows (TR = 8) leaves free hold
 // more bits of the same 8 rows; the accumulators of a row meet in one thread.
@@ -435,7 +437,7 @@ static kr_kernel kr_kernel_of(int code, int otype) {
 // own, so p' uses f16's range whatever V's scales; the sum l runs beside it
 // over 2^(s - m1).  out = O / l * 2^(m2 - m1).
 constexpr int KT_WARPS = 4;
-constexpr int KT_COST = 20;
+constexpr int KT_COST = 32;
 __host__ __device__ constexpr int kt_stages(int hd) { return hd <= 64 ? 4 : 2; }
 constexpr float KT_RISE = 8.0f, KT_BIAS = 6.0f;  // p' <= 2^(8 + 6)
 constexpr float KT_LOW = -1e30f;
@@ -717,8 +719,11 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
     // 2^-e brings the largest into [1/2, 1); a row below 2^-118 counts as zeros, one that is not finite as NaN
     const int e = (int)(m >> 23) - 126;
     const bool nan = m >= 0x7F800000u, tiny = e < -118;
-    const float inv = nan || tiny ? 0.0f : e > 126 ? kv8_pow2(-126) * kv8_pow2(126 - e) : kv8_pow2(-e), up = nan ? __int_as_float(0x7fc00000) : tiny ? 0.0f : 1.0f;
-    qf[r] = a.scale * (up * kv8_pow2(max(-126, min(127, e)))) * (DIGITS ? 1.0f / 127.0f : 1.0f);
+    float inv = nan || tiny ? 0.0f : e > 126 ? kv8_pow2(-126) * kv8_pow2(126 - e) : kv8_pow2(-e);
+    const float up = nan ? __int_as_float(0x7fc00000) : tiny ? 0.0f : 1.0f;
+    if (a.scale < 0.0f) inv = -inv;  // the factor stays positive
+    if (DIGITS) inv *= 127.0f;
+    qf[r] = fabsf(a.scale) * (up * kv8_pow2(max(-126, min(127, e)))) * (DIGITS ? LO ? 1.0f / 127.0f : 1.0f / (127.0f * 254.0f) : 1.0f);
     if (e == 128) qf[r] *= 2.0f;  // 2^128 in two steps
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -726,19 +731,21 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
       for (int s = 0; s < 2; ++s) {  // values 4s .. 4s + 3 of the lane's 8
         float y[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = inv == 0.0f ? 0.0f : x[i][4 * s + j] * inv;
+        for (int j = 0; j < 4; ++j) y[j] = x[i][4 * s + j] * inv;  // of a row that is not finite: anything, times NaN
         if constexpr (DIGITS) {
-          uint32_t d0 = 0, d1 = 0, d2 = 0;
+          // adding 1.5 * 2^23 rounds to an integer, whose low byte is the digit
+          const float big = 12582912.0f;
+          uint32_t b0[4], b1[4], b2[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float v = y[j] * 127.0f;
-            const int i0 = __float2int_rn(v);
-            const float r1 = (v - (float)i0) * 254.0f;
-            const int i1 = __float2int_rn(r1), i2 = __float2int_rn((r1 - (float)i1) * 254.0f);
-            d0 |= (uint32_t)(i0 & 0xFF) << (8 * j);
-            d1 |= (uint32_t)(i1 & 0xFF) << (8 * j);
-            d2 |= (uint32_t)(i2 & 0xFF) << (8 * j);
+            const float t0 = __fadd_rn(y[j], big), r0 = __fsub_rn(y[j], __fsub_rn(t0, big));
+            const float t1 = __fmaf_rn(r0, 254.0f, big), r1 = __fmaf_rn(r0, 254.0f, -__fsub_rn(t1, big));
+            b0[j] = __float_as_uint(t0), b1[j] = __float_as_uint(t1), b2[j] = __float_as_uint(__fmaf_rn(r1, 254.0f, big));
           }
+          auto bytes = [](const uint32_t (&b)[4]) {
+            return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+          };
+          const uint32_t d0 = bytes(b0), d1 = bytes(b1), d2 = LO ? bytes(b2) : 0u;
           if (HL) {
             qa[i][2 * s] = d0, qa[i][2 * s + 1] = d1;
             if (LO) qa[i][(QN == 6 ? 4 : 0) + s] = d2;
@@ -778,8 +785,8 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
     const unsigned char* blk = ring + st * 2 * BB;
     const int b = first_block(i), tok0 = b * PB_KV8_BLOCK;
     const bool one = b < blocks, two = b + 1 < blocks;
-    // x: scores times log2(e), tokens 2t, 2t + 1, 2t + 8, 2t + 9 of a block
-    auto scores = [&](const unsigned char* bk, float ks, float (&x0)[4], float (&x1)[4]) {
+    // x times qf and the block's scale: scores times log2(e), tokens 2t, 2t + 1, 2t + 8, 2t + 9 of a block
+    auto scores = [&](const unsigned char* bk, float (&x0)[4], float (&x1)[4]) {
       if constexpr (DIGITS) {
         int ca[2][4], cb[2][4];
 #pragma unroll
@@ -800,17 +807,16 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
             kt_mma_s8(cb[1], q[4], q[5], q[6], q[7], w.z, w.w);
           }
         }
-        const float f0 = qf[0] * ks, f1 = qf[NR - 1] * ks;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 4; ++j) {  // |sums of a digit| <= 256 * 127 * 127: times 254 they and the next digit's stay below 2^31
           const int *c = ca[j >> 1], *d = cb[j >> 1], z = j & 1;
           if (HL && !LO) {
-            x0[j] = __fmaf_rn((float)c[2 + z], f0 * (1.0f / 254.0f), (float)c[z] * f0);
-          } else if (HL) {  // |i1 sum| * 254 + |i2 sum| stays below 2^31 (256 * 127 * 127 * 255)
-            x0[j] = __fmaf_rn((float)(c[2 + z] * 254 + d[z]), f0 * (1.0f / 64516.0f), (float)c[z] * f0);
+            x0[j] = (float)(c[z] * 254 + c[2 + z]);
+          } else if (HL) {
+            x0[j] = __fmaf_rn((float)(c[2 + z] * 254 + d[z]), 1.0f / 64516.0f, (float)c[z]);
           } else {
-            x0[j] = __fmaf_rn((float)d[z], f0 * (1.0f / 254.0f), (float)c[z] * f0);
-            x1[j] = __fmaf_rn((float)d[2 + z], f1 * (1.0f / 254.0f), (float)c[2 + z] * f1);
+            x0[j] = (float)(c[z] * 254 + d[z]);
+            x1[j] = (float)(c[2 + z] * 254 + d[2 + z]);
           }
         }
       } else {
@@ -834,45 +840,58 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
             kt_mma(c[1], a0, a1, a2, a3, c0, c1);
           }
         }
-        const float f0 = qf[0] * ks, f1 = qf[NR - 1] * ks;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float* y = c[j >> 1];
-          x0[j] = (HL && LO ? y[j & 1] + y[2 + (j & 1)] : y[j & 1]) * f0;
-          if (!HL) x1[j] = y[2 + (j & 1)] * f1;
+          x0[j] = HL && LO ? y[j & 1] + y[2 + (j & 1)] : y[j & 1];
+          if (!HL) x1[j] = y[2 + (j & 1)];
         }
       }
     };
-    float x[2][2][4];  // [block][row]
-    int ve[2] = {KV8_E_ZERO, KV8_E_ZERO};
+    // the scales' exponents, K's and V's
+    const unsigned char* tail = blk + 32 * HD;
+    const int es0 = *reinterpret_cast<const int16_t*>(tail), es1 = two ? *reinterpret_cast<const int16_t*>(tail + BB) : KV8_E_ZERO << 8;
+    auto odd = [](int es) { const int e = es >> 8; return e == KV8_E_ZERO || e == KV8_E_NAN; };
+    const bool mask = tok0 + 2 * PB_KV8_BLOCK > see_min;
+    auto pair = [&](auto kind) {
+    constexpr bool PLAIN = decltype(kind)::value;  // two blocks, no mask, values to count
+    float x[2][2][4], fx[2][NR];  // [block][row], a score is x * fx
     // log2 of V's scale where the block's values count in f16's way; the others (no values, not finite) take a way of their own
-    float vadd[2] = {-INFINITY, -INFINITY};
+    float vadd[2];
+    const int es[2] = {es0, es1};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const unsigned char* bk = blk + h * BB;
-      if (h == 0 ? one : two) {
-        const int es = *reinterpret_cast<const uint16_t*>(bk + 32 * HD);
-        ve[h] = (int8_t)(es >> 8);
-        vadd[h] = ve[h] == KV8_E_ZERO ? -INFINITY : ve[h] == KV8_E_NAN ? __int_as_float(0x7fc00000) : (float)ve[h];
-        scores(bk, kv8_scale((int8_t)(es & 0xFF)), x[h][0], x[h][1]);
+      const int ve = es[h] >> 8;
+      vadd[h] = PLAIN || !odd(es[h]) ? (float)ve : ve == KV8_E_ZERO ? -INFINITY : __int_as_float(0x7fc00000);
+      if (PLAIN || (h == 0 ? one : two)) {
+        const float ks = kv8_scale((int8_t)(es[h] & 0xFF));
+#pragma unroll
+        for (int r = 0; r < NR; ++r) fx[h][r] = qf[r] * ks;
+        scores(bk, x[h][0], x[h][1]);
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[h][0][j] = x[h][1][j] = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) fx[h][r] = 1.0f;
       }
     }
-    const bool mask = tok0 + 2 * PB_KV8_BLOCK > see_min;
     uint32_t pa[2][4];
     float rescale[NR];
     bool any = false;
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-      if (mask) {
+      if (!PLAIN && mask) {  // -inf, whatever the factor
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (tok0 + 2 * t + (j & 1) + 8 * (j >> 1) >= see[r]) x[j >> 2][r][j & 3] = -INFINITY;
+        for (int j = 0; j < 8; ++j) {
+          float& y = x[j >> 2][r][j & 3];
+          y = tok0 + 2 * t + (j & 1) + 8 * (j >> 1) >= see[r] ? -INFINITY : y * fx[j >> 2][r];
+        }
+        fx[0][r] = fx[1][r] = 1.0f;
       }
       const float *xa = x[0][r], *xb = x[1][r];
-      const float ba = fmaxf(fmaxf(xa[0], xa[1]), fmaxf(xa[2], xa[3])), bb = fmaxf(fmaxf(xb[0], xb[1]), fmaxf(xb[2], xb[3]));
+      const float ba = fmaxf(fmaxf(xa[0], xa[1]), fmaxf(xa[2], xa[3])) * fx[0][r];
+      const float bb = fmaxf(fmaxf(xb[0], xb[1]), fmaxf(xb[2], xb[3])) * fx[1][r];
       float bm = fmaxf(ba, bb), bv = fmaxf(ba + vadd[0], bb + vadd[1]);
       // the references move when a score passes them by 2^8: looked at by the quad only where a lane of the warp saw one
       rescale[r] = 1.0f;
@@ -895,11 +914,11 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float p[4], sum = 0.0f;
-        if (ve[h] == KV8_E_ZERO || ve[h] == KV8_E_NAN) {  // p' is 0 or NaN there: the sum by itself
+        if (!PLAIN && odd(es[h])) {  // p' is 0 or NaN there: the sum by itself
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            sum += kt_ex2(x[h][r][j] - m1[r]);
-            p[j] = x[h][r][j] == -INFINITY ? 0.0f : kt_ex2(x[h][r][j] + (vadd[h] + top));  // -inf: masked
+            sum += kt_ex2(__fmaf_rn(x[h][r][j], fx[h][r], -m1[r]));
+            p[j] = x[h][r][j] == -INFINITY ? 0.0f : kt_ex2(__fmaf_rn(x[h][r][j], fx[h][r], vadd[h] + top));  // -inf: masked
           }
           l[r] += sum;
         } else {
@@ -907,7 +926,7 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
           // its f32 precision wherever 2^(x - m1) counts
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            p[j] = kt_ex2(x[h][r][j] + (vadd[h] + top));
+            p[j] = kt_ex2(__fmaf_rn(x[h][r][j], fx[h][r], vadd[h] + top));
             sum += p[j];
           }
           l[r] = __fmaf_rn(sum, kt_ex2(-(vadd[h] + top) - m1[r]), l[r]);
@@ -941,8 +960,11 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
         }
       }
     };
-    if (one) values(blk, pa[0]);
-    if (two) values(blk + BB, pa[1]);
+    if (PLAIN || one) values(blk, pa[0]);
+    if (PLAIN || two) values(blk + BB, pa[1]);
+    };
+    if (two && !mask && !odd(es0) && !odd(es1)) pair(std::true_type());
+    else pair(std::false_type());
     // every lane's reads of the stage come before the copy that refills it
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
