@@ -131,6 +131,10 @@ __device__ __forceinline__ void ka_rotate(const unsigned char* rows, int stride,
 // memory, and a warp then codes a head's K or V, tile by tile in the layout's
 // order.  Many small CTAs keep about 128 KB a SM in flight.  k is rotated in
 // double, so that its codes are those of the exact values; q in f32.
+// 9 prompts of 37 to 3001 f32 rows (32 heads over 8 of 128 values, half of them
+// rotated; 9.4 thousand rows, about 340 MB): about 79 us, 4.3 TB/s; a step of 96
+// bf16 rows 13 us and of 4 f32 rows 9.5 us with the read that follows, the
+// latency of one block's chain (starts, rows, rotation, codes).
 template <int TYPE, int ROPE>
 __global__ void __launch_bounds__(KA_THREADS, 4) k_kv8_append(kv8_geo g, kv8_append_args a, int y_kv) {
   constexpr int ES = TYPE == PB_TYPE_F32 ? 4 : 2;
@@ -307,6 +311,7 @@ constexpr int KR_BYTES = 24 << 10;  // of a CTA's blocks
 // A CTA has one 16-token block of one sequence and a share of the heads, whose
 // blocks come by bulk copies, all at once.  Memory bound: the codes are read
 // once, and a warp writes whole rows of a head (lanes along the values).
+// 73756 tokens of 8 heads of 128 values, e4m3 to bf16: 78 us, 5.8 TB/s.
 template <int CODE, int OT>
 __global__ void __launch_bounds__(KR_THREADS)
 k_kv8_read(kv8_geo g, const uint8_t* pages, const int* __restrict__ starts, const int* __restrict__ first,
@@ -436,6 +441,13 @@ static kr_kernel kr_kernel_of(int code, int otype) {
 // exponent, p' = 2^(s + ve - m2), with a running reference m2 of s + ve of its
 // own, so p' uses f16's range whatever V's scales; the sum l runs beside it
 // over 2^(s - m1).  out = O / l * 2^(m2 - m1).
+//
+// Measured (8 kv heads of 128 values): 2 x 131072 tokens, int8, 64 f16 heads: 93
+// us, 5.4 TB/s of codes; 64 ragged sequences up to 9000 tokens, e4m3, 32 bf16
+// heads: 105 to 108 us, 5.5 TB/s; memory bound.  12 sequences of 1 to 5 drafted
+// tokens, int8, f16: 75 us, 3.9 TB/s, bound by the work on two rows a thread and
+// by the second pass over the codes where 20 rows need two tiles.  One sequence
+// of 640 tokens, f32: 8.5 us, latency.
 constexpr int KT_WARPS = 4;
 constexpr int KT_COST = 32;
 __host__ __device__ constexpr int kt_stages(int hd) { return hd <= 64 ? 4 : 2; }

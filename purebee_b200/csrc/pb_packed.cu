@@ -26,13 +26,22 @@
 // beside the other's softmax.  Warps:
 //   4 per tile: the softmax, a thread per row (its TMEM lane): S from TMEM, p
 //     back to TMEM, O / l at the end;
-//   one lane each for the TMA loads (Q, the K and V tiles) and for the MMAs
-//     (P comes from TMEM, V is the MN-major operand: no transpose);
+//   one lane each for the TMA loads (Q, the K and V tiles; its warp finds the
+//     CTA's sequence and has Q and the first keys coming before the others are
+//     ready: short prompts 11.0 -> 10.0 us) and for the MMAs (P comes from TMEM,
+//     V is the MN-major operand: no transpose);
 //   two: the V tiles that some row must not see whole: rows behind the
 //     sequence's keys become zero (0 * inf would be NaN), and a value that is not
 //     finite under the causal mask sends the CTA's rows, once the rest is done,
 //     through the plain form below, which touches no masked value.
 // A part of the exponentials run on the FMA pipe (pa_ex2_poly).
+//
+// Bound by the chain of a tile (S, maximum, exponentials, P) and its issue slots,
+// not by the products: 8192 causal rows, 32 heads over 8, in bf16 take 455 us with
+// 128 values a head (1.21 PFLOP/s; about 540 us, 1.02 PFLOP/s, where the power
+// limit holds the clock at 1.45 GHz) and 425 us with 64 (the exponentials alone
+// 250 us); 24 ragged f16 prompts of 65 to 1024 rows with 64 values 162 us, of
+// which a third is the CTAs' starts and ends.
 #include <math.h>
 
 #include "pb_kv8.cuh"
@@ -266,6 +275,51 @@ constexpr size_t pa_smem(int hdp) {
   return 1024 + (size_t)(hdp / 64) * (pa_tiles(hdp) * PA_PANEL + 2 * PA_STAGES * PA_PANEL);
 }
 
+// A CTA's rows: rows r0 .. of the nq from q0 on (two_rows: 256 of them, else 128), the nk keys from k0 on, the key tiles that
+// its tiles see, and those that every row sees whole.
+struct pa_place {
+  int q0, nq, k0, nk, r0, n0, n1, whole;
+  bool ok;
+};
+__device__ __forceinline__ int pa_see(const pa_args& a, int nq, int nk, int r) {
+  return a.causal ? max(0, min(nk, nk - nq + r + 1)) : nk;
+}
+// Sequence s has the tile numbers from starts[s] / span + s on: the last s whose first is at most rt, by a warp, 32 looks a
+// step.  Starts that do not rise end it at some sequence, whose numbers are then looked at.
+__device__ __forceinline__ pa_place pa_find(const pa_args& a, bool two_rows, int rt, int lane) {
+  const int span = two_rows ? 2 * PA_ROWS : PA_ROWS;
+  pa_place pl = {};
+  int s0 = 0, n = a.n_seqs, lo = 0, hi = 0, kl = 0, kh = 0, at;
+  for (;;) {
+    const int step = (n + 31) / 32, s = s0 + lane * step;
+    const bool in = lane * step < n;
+    if (in) lo = a.qst[s];
+    if (in && step == 1) hi = a.qst[s + 1], kl = a.kst[s], kh = a.kst[s + 1];
+    at = __popc(__ballot_sync(0xffffffffu, in && lo / span + s <= rt)) - 1;
+    if (at < 0) return pl;
+    if (step == 1) break;
+    s0 += at * step;
+    n = min(step, n - at * step);
+  }
+  lo = __shfl_sync(0xffffffffu, lo, at), hi = __shfl_sync(0xffffffffu, hi, at);
+  kl = __shfl_sync(0xffffffffu, kl, at), kh = __shfl_sync(0xffffffffu, kh, at);
+  if (lo < 0 || hi < lo || hi > a.q_rows) return pl;
+  pl.q0 = lo, pl.nq = hi - lo, pl.k0 = kl, pl.nk = kh - kl;
+  const int64_t r0 = (int64_t)(rt - (lo / span + s0 + at)) * span;
+  if (r0 < 0 || r0 >= pl.nq) return pl;
+  if (kl < 0 || kh < kl || kh > a.k_rows) {
+    if (lane == 0) pb_raise(a.err, PB_DEVERR_BOUNDS);
+    return pl;
+  }
+  pl.r0 = (int)r0;
+  auto tiles = [&](int row) { return row >= pl.nq ? 0 : (pa_see(a, pl.nq, pl.nk, min(pl.nq, row + PA_ROWS) - 1) + PA_KEYS - 1) / PA_KEYS; };
+  pl.n0 = tiles(pl.r0);
+  pl.n1 = two_rows ? tiles(pl.r0 + PA_ROWS) : pl.n0;
+  pl.whole = pa_see(a, pl.nq, pl.nk, pl.r0) / PA_KEYS;
+  pl.ok = true;
+  return pl;
+}
+
 // HDP: head columns in shared memory and TMEM (64 or 128; TMA fills those past
 // head_dim with zeros), BF: bf16 rows.
 template <int HDP, bool BF>
@@ -284,56 +338,14 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
   __shared__ uint64_t q_full, k_full[NS], k_empty[NS], v_full[NS], v_mask[NS], v_ready[NS], v_empty[NS], s_full[NT], s_free, p_full[NT][2], o_half[NT][2];
   __shared__ uint32_t tmem_base;
   __shared__ int redo;
-  __shared__ struct {
-    int seq, q0, nq, k0, nk;
-  } found;
+  __shared__ pa_place place;
   __shared__ float qrow[T / 32][128];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  pb_pdl_trigger();
-  pb_pdl_wait();
-
-  // which rows: sequence s has the tile numbers from starts[s] / span + s on
-  const bool two_rows = NT == 2 && a.two_rows;
-  const int span = two_rows ? 2 * PA_ROWS : PA_ROWS, unit = (int)(gridDim.x - 1 - blockIdx.x);
-  const int rt = unit / a.pairs, pair = a.pairs - 1 - unit % a.pairs;
-  if (tid == 0) found.seq = -1, redo = 0;
-  if (warp == 4 * NT && lane < 3)
-    asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &map_q : lane == 1 ? &map_k : &map_v) : "memory");
-  __syncthreads();
-  for (int s = tid; s < a.n_seqs; s += T) {
-    const int lo = a.qst[s], hi = a.qst[s + 1], kl = a.kst[s], kh = a.kst[s + 1];
-    if (lo < 0 || hi < lo || hi > a.q_rows) pb_raise(a.err, PB_DEVERR_BOUNDS);
-    else if (lo / span + s <= rt && rt < hi / span + s + 1) found = {s, lo, hi - lo, kl, kh - kl};
-  }
-  __syncthreads();
-  if (found.seq < 0) return;
-  const int seq = found.seq, q0 = found.q0, nq = found.nq, k0 = found.k0, nk = found.nk;
-  if (k0 < 0 || nk < 0 || (int64_t)k0 + nk > a.k_rows) {
-    if (tid == 0) pb_raise(a.err, PB_DEVERR_BOUNDS);
-    return;
-  }
-  const int r0 = (rt - (q0 / span + seq)) * span;  // the CTA's first row of the sequence
-  if (r0 >= nq) return;
-  // tile i: rows row_of(i) .., head head_of(i); row r sees see(r) keys
-  const int kvh = NT == 1 || two_rows ? pair / a.group : pair / (a.group / 2);
-  auto row_of = [&](int i) { return two_rows ? r0 + i * PA_ROWS : r0; };
-  auto head_of = [&](int i) { return NT == 1 || two_rows ? pair : 2 * pair + i; };
-  auto see = [&](int r) { return a.causal ? max(0, min(nk, nk - nq + r + 1)) : nk; };
-  auto tiles_of = [&](int i) {
-    const int last = min(nq, row_of(i) + PA_ROWS) - 1;
-    return last < row_of(i) ? 0 : (see(last) + PA_KEYS - 1) / PA_KEYS;
-  };
-  const int n0 = tiles_of(0), n1 = NT == 2 ? tiles_of(1) : 0, nt = max(n0, n1);
-  const int whole = see(r0) / PA_KEYS;  // key tiles that every row sees whole
-
   unsigned char* base = pa_raw + ((1024 - (pb_smem_addr(pa_raw) & 1023)) & 1023);
   unsigned char *sQ = base, *sK = sQ + NT * QT, *sV = sK + NS * KT;
-  if (warp == 4 * NT + 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pb_smem_addr(&tmem_base)),
-                 "r"(TMEM)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
+  pb_pdl_trigger();
+  if (warp == 4 * NT && lane < 3)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &map_q : lane == 1 ? &map_k : &map_v) : "memory");
   if (tid == 128 * NT) {
     pb_mbar_init(&q_full, 1);
     for (int s = 0; s < NS; ++s) {
@@ -353,24 +365,67 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     }
     pb_mbar_init(&s_free, 4);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  pb_pdl_wait();
+
+  const bool two_rows = NT == 2 && a.two_rows;
+  const int unit = (int)(gridDim.x - 1 - blockIdx.x), rt = unit / a.pairs, pair = a.pairs - 1 - unit % a.pairs;
+  const int kvh = NT == 1 || two_rows ? pair / a.group : pair / (a.group / 2);
+  auto head_of = [&](int i) { return NT == 1 || two_rows ? pair : 2 * pair + i; };
+  if (warp == 4 * NT) {  // finds the place and has the first tiles on their way while the others get ready
+    const pa_place pl = pa_find(a, two_rows, rt, lane);
+    __syncwarp();
+    if (lane == 0) {
+      place = pl;
+      if (pl.ok && max(pl.n0, pl.n1) > 0) {
+        pb_mbar_arrive_tx(&q_full, NT * QT);
+        for (int i = 0; i < NT; ++i)
+          for (int p = 0; p < PN; ++p)
+            pb_tma_load_3d(sQ + i * QT + p * PA_PANEL, &map_q, p * 64, head_of(i), pl.q0 + pl.r0 + (two_rows ? i * PA_ROWS : 0), &q_full);
+        pb_mbar_arrive_tx(&k_full[0], KT);
+        for (int p = 0; p < PN; ++p) pb_tma_load_3d(sK + p * PA_PANEL, &map_k, p * 64, kvh, pl.k0, &k_full[0]);
+      }
+    }
+  } else if (warp == 4 * NT + 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pb_smem_addr(&tmem_base)),
+                 "r"(TMEM)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else if (tid < 128) {
+    if (tid == 0) redo = 0;
+    if (blockIdx.x == 0)  // what the search may pass by
+      for (int s = tid; s < a.n_seqs; s += 128) {
+        const int lo = a.qst[s], hi = a.qst[s + 1];
+        if (lo < 0 || hi < lo || hi > a.q_rows) pb_raise(a.err, PB_DEVERR_BOUNDS);
+      }
   }
   pa_fence_before();
   __syncthreads();
   pa_fence_after();
   const uint32_t tmem = tmem_base;
+  const pa_place pl = place;
+  if (!pl.ok) {
+    if (warp == 4 * NT + 1)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM) : "memory");
+    return;
+  }
+  const int q0 = pl.q0, nq = pl.nq, k0 = pl.k0, nk = pl.nk, r0 = pl.r0, n0 = pl.n0, n1 = NT == 2 ? pl.n1 : 0, nt = max(n0, n1);
+  const int whole = pl.whole;
+  // tile i: rows row_of(i) .., head head_of(i); row r sees see(r) keys
+  auto row_of = [&](int i) { return two_rows ? r0 + i * PA_ROWS : r0; };
+  auto see = [&](int r) { return pa_see(a, nq, nk, r); };
 
   if (warp == 4 * NT) {
     if (lane == 0 && nt > 0) {  // TMA
-      pb_mbar_arrive_tx(&q_full, NT * QT);
-      for (int i = 0; i < NT; ++i)
-        for (int p = 0; p < PN; ++p)
-          pb_tma_load_3d(sQ + i * QT + p * PA_PANEL, &map_q, p * 64, head_of(i), q0 + row_of(i), &q_full);
       for (int j = 0; j < nt; ++j) {
         const int s = j % NS, use = j / NS;
         if (j >= NS && !pb_mbar_wait_sleep(&k_empty[s], (use - 1) & 1, a.err)) break;
-        pb_mbar_arrive_tx(&k_full[s], KT);
-        for (int p = 0; p < PN; ++p)
-          pb_tma_load_3d(sK + s * KT + p * PA_PANEL, &map_k, p * 64, kvh, k0 + j * PA_KEYS, &k_full[s]);
+        if (j > 0) {
+          pb_mbar_arrive_tx(&k_full[s], KT);
+          for (int p = 0; p < PN; ++p)
+            pb_tma_load_3d(sK + s * KT + p * PA_PANEL, &map_k, p * 64, kvh, k0 + j * PA_KEYS, &k_full[s]);
+        }
         if (j >= NS && !pb_mbar_wait_sleep(&v_empty[s], (use - 1) & 1, a.err)) break;
         uint64_t* full = j < whole ? &v_full[s] : &v_mask[s];  // a tile under a mask goes to the helpers first
         pb_mbar_arrive_tx(full, KT);
