@@ -132,7 +132,7 @@ __device__ __forceinline__ void ka_rotate(const unsigned char* rows, int stride,
 // order.  Many small CTAs keep about 128 KB a SM in flight.  k is rotated in
 // double, so that its codes are those of the exact values; q in f32.
 // 9 prompts of 37 to 3001 f32 rows (32 heads over 8 of 128 values, half of them
-// rotated; 9.4 thousand rows, about 340 MB): about 79 us, 4.3 TB/s; a step of 96
+// rotated; 9776 rows, 340 MB): about 79 us, 4.3 TB/s; a step of 96
 // bf16 rows 13 us and of 4 f32 rows 9.5 us with the read that follows, the
 // latency of one block's chain (starts, rows, rotation, codes).
 template <int TYPE, int ROPE>
