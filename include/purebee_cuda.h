@@ -560,7 +560,7 @@ int pb_kv8_read(pb_kv8* kv, const void* pages_dev, const int* starts_dev, const 
  * being cached with them; each sees the tokens up to its own, kv head h /
  * (n_heads / n_kv_heads) for head h.  out = sum_j softmax_j(scale q.k_j) v_j
  * with f32 sums; a row that sees no token (lens_dev[s] less than its rows)
- * gets zeros.  q_dev and out_dev [n_rows][n_heads * head_dim] are of one type
+ * gets zeros, and a query whose values all lie below 2^-118 counts as zeros.  q_dev and out_dev [n_rows][n_heads * head_dim] are of one type
  * and do not overlap. */
 int pb_kv8_attn(pb_kv8* kv, const void* pages_dev, int type, const void* q_dev, int ldq, int n_heads,
                 const int* starts_dev, const int* lens_dev, const int* table_dev, int ld_table, int n_seqs, int n_rows,

@@ -439,7 +439,8 @@ static kr_kernel kr_kernel_of(int code, int otype) {
 //
 // Scales: S's columns times 2^ke of the block.  V's 2^ve is put into the
 // exponent, p' = 2^(s + ve - m2), with a running reference m2 of s + ve of its
-// own, so p' uses f16's range whatever V's scales; the sum l runs beside it
+// own, so p' uses f16's range whatever V's scales (below 2^-14 its last bit is
+// 2^-24, which is 2^-30 of the row's largest p 2^ve); the sum l runs beside it
 // over 2^(s - m1).  out = O / l * 2^(m2 - m1).
 //
 // Measured (8 kv heads of 128 values): 2 x 131072 tokens, int8, 64 f16 heads: 93
@@ -728,7 +729,7 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
     }
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    // 2^-e brings the largest into [1/2, 1); a row below 2^-118 counts as zeros, one that is not finite as NaN
+    // 2^-e brings the largest into [1/2, 1); a row below 2^-118 counts as zeros (its scores would be below 2^-40 for scales up to 1), one that is not finite as NaN
     const int e = (int)(m >> 23) - 126;
     const bool nan = m >= 0x7F800000u, tiny = e < -118;
     float inv = nan || tiny ? 0.0f : e > 126 ? kv8_pow2(-126) * kv8_pow2(126 - e) : kv8_pow2(-e);

@@ -255,6 +255,75 @@ def test_attention_uneven_scales(native, ctx, t):
         p.check_attn(4, [3], [190], t, scale=scale, q=q)
 
 
+def below_f16(q, k, v, scale, limit):
+    """What the tolerance of p's relative rounding leaves out: p' = p 2^e / 2^m2 * 2^6 (e the exponent of the block's V, m2 at
+    most the largest log2(p 2^e) so far) is held in f16, alone or as the second of two, and f16 has no step below 2^-24: off by
+    at most 2^-25, whatever p' is.  A key's term p v is p' code 2^(m2 - 6), so the output is off by at most
+    2^-31 max_j(p_j 2^e_j) sum_j |code_j|.  It counts where the keys of large p have the code 0."""
+    n, nkv, hd = v.shape
+    nq, nh = q.shape[:2]
+    tol = np.zeros((nq, nh, hd))
+    for h in range(nh):
+        kh, vh = k[:, h // (nh // nkv)], np.abs(v[:, h // (nh // nkv)])
+        most = np.array([vh[j // 16 * 16:j // 16 * 16 + 16].max() for j in range(n)])
+        unit = np.where(most > 0, 2.0 ** np.maximum(np.ceil(np.log2(np.maximum(most, 1e-300) / limit)), -40), 1.0)
+        for i in range(nq):
+            see = max(0, n - nq + i + 1)
+            if see:
+                s = kh[:see] @ q[i, h] * scale
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                tol[i, h] = 2.0 ** -31 * (p * unit[:see])[most[:see] > 0].max(initial=0) * (vh[:see] / unit[:see, None]).sum(0)
+    return tol
+
+
+@pytest.mark.parametrize("code,t,group", [(0, "f32", 4), (0, "bf16", 8), (0, "f16", 2), (1, "f32", 4), (1, "bf16", 8), (1, "f16", 2)])
+def test_attention_zero_rows_and_signs(native, ctx, code, t, group):
+    """Queries of zeros, keys of zeros (a block's K scale unset), scale 0 and negative, masks that end inside a pair of blocks."""
+    p = Pool(native, ctx, code, 2, 96, 16, 2, 150, seed=40 + code)
+
+    def edit(kv):
+        kv[16:48, 0] = 0
+        kv[64:80, 1] = 0
+        kv[130:, 0] *= 3.0
+    p.append([137, 34], [0, 0], 2, edit=edit)
+    n = [5, 3]
+    for scale in (0.1, 0.0, -0.4):
+        q = p.rng.standard_normal((sum(n), 2 * group, 96))
+        q[1], q[6, 0] = 0, 0
+        got, q = p.attn(q, n, [137, 34], t, scale)
+        at = 0
+        for s, (rows, ln) in enumerate(zip(n, [137, 34])):
+            k, v = p.ref[s].values(0, ln), p.ref[s].values(1, ln)
+            w, mag, dots = R.attention(q[at:at + rows], k, v, scale)
+            tol = R.attention_tolerance(w, mag, dots, 96, ln, t, 2.0 ** -22 if t == "f32" else 2.0 ** -11)
+            tol = tol + below_f16(q[at:at + rows], k, v, scale, 448 if code else 127)
+            bad = R.differs(got[at:at + rows], w, tol, t)
+            assert not bad.any(), (s, scale, np.argwhere(bad)[:4], got[at:at + rows][bad][:4], w[bad][:4], tol[bad][:4])
+            at += rows
+
+
+def test_first_rows_that_belong_to_nobody(native, ctx):
+    """starts[0] above 0: the rows before it are neither read nor written."""
+    p = Pool(native, ctx, 0, 2, 64, 16, 2, 64, seed=50)
+    p.append([40, 21], [0, 0], 2)
+    st, le = p.ints([5, 7, 8]), p.ints([40, 21])
+    x = p.rng.standard_normal((8, 4, 64)).astype(np.float32)
+    x[:5] = np.nan
+    dx, o = ctx.to_device(x), ctx.to_device(np.full((8, 4, 64), 3, np.float32))
+    p.kv.attn(p.pages.ptr, 0, dx.ptr, 256, 4, st.ptr, le.ptr, p.table.ptr, p.ld, 2, 8, 0.125, o.ptr, 256)
+    got = o.download().reshape(8, 4, 64)
+    want = p.check_attn(4, [2, 1], [40, 21], "f32", scale=0.125, q=x[5:].astype(np.float64))
+    assert np.all(got[:5] == 3) and np.array_equal(got[5:], want.astype(np.float32))
+    k, v = (ctx.to_device(np.full((8, 128), 5, np.float32)) for _ in range(2))
+    fi = p.ints([10, 20])
+    p.kv.read(p.pages.ptr, st.ptr, fi.ptr, p.table.ptr, p.ld, 2, 8, 0, k.ptr, 128, v.ptr, 128)
+    for i, d in ((0, k), (1, v)):
+        g = d.download().reshape(8, 2, 64)
+        assert np.all(g[:5] == 5)
+        np.testing.assert_array_equal(g[5:], np.concatenate([p.ref[0].values(i, 12)[10:], p.ref[1].values(i, 21)[20:]]))
+
+
 def test_attention_not_finite(native, ctx):
     """A query with a NaN, blocks that read as NaN: what sees them is NaN, what does not is not touched."""
     p = Pool(native, ctx, 1, 1, 64, 16, 3, 64, seed=13)

@@ -190,6 +190,28 @@ def test_packed_rows_past_31_bits(native, ctx):
     assert not R.differs(got, w, tol, "f16").any()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_packed_first_rows_that_belong_to_nobody(native, ctx, hd):
+    """starts[0] above 0 and above a tile: the same rows and bits as without the rows before them, which stay."""
+    n, off = [3, 130, 40], 300
+    got = check(native, ctx, "bf16", n, n, 2, 1, hd, seed=30, same=True)
+    rng = np.random.default_rng(30)
+    rows = sum(n)
+    q = rng.standard_normal((rows, 2, hd))
+    k, v = rng.standard_normal((2, rows, 1, hd))
+
+    def put(x):
+        return ctx.to_device(R.to_bits(np.concatenate([np.full((off, x[0].size), np.nan), x.reshape(rows, -1)]), "bf16"))
+    dq, dk, dv = put(q), put(k), put(v)
+    o = ctx.to_device(np.full((off + rows, 2 * hd), 3, np.uint16))
+    st = ctx.to_device((off + np.concatenate([[0], np.cumsum(n)])).astype(np.int32))
+    ctx.attn_packed(native.TYPE_BF16, dq.ptr, 2 * hd, dk.ptr, hd, dv.ptr, hd, st.ptr, st.ptr, 3, off + rows, off + rows, 2, 1, hd,
+                    hd ** -0.5, 1, o.ptr, 2 * hd)
+    raw = o.download(np.uint16).reshape(off + rows, 2 * hd)
+    assert np.all(raw[:off] == 3)
+    np.testing.assert_array_equal(R.from_bits(raw[off:], "bf16").reshape(rows, 2, hd), got)
+
+
 def test_packed_refusals(native, ctx):
     N = native
     b, i = ctx.alloc(1 << 16), ctx.to_device(np.array([0, 4], np.int32))
