@@ -47,7 +47,7 @@ __device__ __forceinline__ void ka_at4(const unsigned char* row, int d, float (&
 // a token), the pair (2i, 2i + 1) or (i, i + rope_dim / 2) by the angle of index
 // i; cs: {cos, sin} [token][half].  A thread has an item (4 values of a head at
 // d, and their partners in the half layout) for tokens tok0, tok0 + share, ...:
-// put(tok, h, d, values, largest) stores 4 rotated values, put1 one;
+// put(tok, h, d, values) stores 4 rotated values, put1 one;
 // most(h, largest) gets the largest magnitude of the item.  A thread gives both
 // values of a pair, so put may write in place.
 template <int TYPE, int ROPE, typename R, typename R2, typename Put, typename Put1, typename Most>
@@ -424,18 +424,20 @@ static kr_kernel kr_kernel_of(int code, int otype) {
 // scales takes a way without branches, both blocks' products side by side
 // (drafted tokens 82 -> 78 us, 64 ragged with heads of 64 values 72 -> 62).
 //
-// Rows of the products' M = 16 that a tile of 8 rows (TR = 8) leaves free hold
-// more bits of the same 8 rows; the accumulators of a row meet in one thread.
+// Rows of the products' M = 16 that a tile of 8 rows (TR = 8) leaves free can
+// hold more bits of the same 8 rows; the accumulators of a row meet in one thread.
 // O = P V: m16n8k16 in f16 straight from the codes (every code is exact in
 // f16); S's accumulators, rows = queries and columns = tokens, are its A
-// operand.  TR = 8: rows 0-7 hold hi = f16(p), rows 8-15 lo = f16(p - hi), 22
-// bits at no extra product; TR = 16 rounds p once, half a step of f16.
+// operand.  f32 rows (LO, TR = 8): rows 0-7 hold hi = f16(p), rows 8-15 lo =
+// f16(p - hi), 22 bits at no extra product; 16-bit rows, whose output has no more
+// than f16's bits, round p once, half a step of f16.
 // S = Q K^T with int8 codes: m16n8k32 on the codes as they are, q in signed
 // byte digits q = f (i0 + i1 / 254 + i2 / 254^2), f from the row's largest, so
-// the products and sums are exact: three digits (24 bits) for TR = 8, two (16
-// bits below the row's largest) for TR = 16, whose rows have 16-bit queries.
-// With e4m3 codes: m16n8k16 in f16 with q = hi + lo (TR = 8), or q in f16 after
-// a power of two (TR = 16, exact).
+// the products and sums are exact: three digits (24 bits) for f32 rows, two (16
+// bits below the row's largest) for 16-bit rows.
+// With e4m3 codes: m16n8k16 in f16 with q = hi + lo for f32 rows, or q in f16
+// after a power of two for 16-bit rows (what f16 cannot hold of them lies 2^-25
+// or more below the row's largest).
 //
 // Scales: S's columns times 2^ke of the block.  V's 2^ve is put into the
 // exponent, p' = 2^(s + ve - m2), with a running reference m2 of s + ve of its
@@ -1186,6 +1188,9 @@ extern "C" int pb_kv8_create(pb_ctx* ctx, const pb_kv8_config* c, pb_kv8** out) 
     return pb_set_error(ctx, PB_ERR_ARG, "pb_kv8: bad rotary base or frequency scaling");
   for (int j = 0; j < g.rope_dim / 2; ++j) freqs[128 + j] = cos(freqs[j]), freqs[256 + j] = sin(freqs[j]);
   pb_device_scope dev(ctx->device);
+  cudaStreamCaptureStatus recording = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(ctx->stream, &recording) != cudaSuccess || recording != cudaStreamCaptureStatusNone)
+    return pb_set_error(ctx, PB_ERR_STATE, "pb_kv8_create: not while recording");
   pb_kv8* kv = new pb_kv8();
   kv->ctx = ctx;
   kv->g = g;

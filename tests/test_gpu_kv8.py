@@ -456,6 +456,27 @@ def test_refusals_of_outputs_that_are_other_arrays_too(native, ctx):
     assert ctx.launches == n0
 
 
+def test_no_handle_while_recording(native, ctx):
+    """The refusal leaves the recording as it was."""
+    p = Pool(native, ctx, 0, 1, 32, 16, 1, 40)
+    p.append([20], [0], 1)
+    q, out = ctx.to_device(np.ones((1, 64), np.float32)), ctx.to_device(np.zeros((1, 64), np.float32))
+    st, le = p.ints([0, 1]), p.ints([20])
+
+    def step():
+        with pytest.raises(native.PureBeeError, match="PB_ERR_STATE"):
+            native.KV8(ctx, 0, 1, 256, 16, 4)
+        p.kv.attn(p.pages.ptr, 0, q.ptr, 64, 2, st.ptr, le.ptr, p.table.ptr, p.ld, 1, 1, 0.1, out.ptr, 64)
+
+    graph = ctx.capture(step)
+    graph.launch()
+    got = out.download().copy()
+    assert np.any(got != 0)
+    p.kv.attn(p.pages.ptr, 0, q.ptr, 64, 2, st.ptr, le.ptr, p.table.ptr, p.ld, 1, 1, 0.1, out.ptr, 64)
+    np.testing.assert_array_equal(out.download(), got)
+    graph.free()
+
+
 def test_handles_share_the_workspace(native, ctx):
     """Handles of several head sizes, made and used in turn on one context, and recorded into one graph: the same bits."""
     lens, pools = [900, 40], []
