@@ -233,7 +233,8 @@ __device__ __forceinline__ float pa_max3(float a, float b, float c) {
 }
 // 2^x of two values on the FMA pipe: x = n + r, |r| <= 1/2, n by adding 1.5 *
 // 2^23; 2^r by its minimax polynomial; n into the exponent.  Below 2^-126 the
-// result stays at about 2^-126, nothing beside a row's sum (at least 2^-8).
+// result is 0, as pa_ex2's: a masked key (-inf) must leave no part of its value
+// in O, and 2^-126 times a bf16 value near the largest is 3.5.
 template <bool BF>
 __device__ __forceinline__ void pa_ex2_poly(uint64_t x, float& y0, float& y1) {
   float a, b;
@@ -257,8 +258,8 @@ __device__ __forceinline__ void pa_ex2_poly(uint64_t x, float& y0, float& y1) {
   float p0, p1, n0, n1;
   pa_split(p, p0, p1);
   pa_split(n, n0, n1);
-  y0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23));
-  y1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23));
+  y0 = a < -126.0f ? 0.0f : __uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23));
+  y1 = b < -126.0f ? 0.0f : __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23));
 }
 template <bool BF>
 __device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {

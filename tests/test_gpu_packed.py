@@ -239,3 +239,17 @@ def test_packed_bad_rows_raise_the_error_word(native):
     with pytest.raises(native.PureBeeError, match="PB_ERR_DEVICE.*bounds"):
         c.sync()
     c.close()
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 96, 128])
+def test_packed_hidden_values_do_not_count(native, ctx, t, hd):
+    """Finite values near the type's largest behind the causal mask: the rows before them are what they are without them."""
+    rng = np.random.default_rng(31)
+    q, k, v = (rng.standard_normal((64, h, hd)) for h in (2, 1, 1))
+    big = 3e38 if t == "bf16" else 6e4
+    v[40:] = big * np.sign(v[40:])  # every place of 16 keys; the rows below 40 see none of them
+    got, q, k, v = run(native, ctx, t, q, k, v, [64], [64], True, hd ** -0.5, same=True)
+    w, mag, dots = R.attention(q[:40], k[:40], v[:40], hd ** -0.5)
+    tol = R.attention_tolerance(w, mag, dots, hd, 40, t, R.EPS[t] / 2) + (2.0 ** -25 * np.abs(v[:40]).sum(0) if t == "f16" else 0)
+    assert not R.differs(got[:40], w, tol, t).any()
