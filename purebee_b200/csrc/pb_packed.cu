@@ -226,21 +226,28 @@ __device__ __forceinline__ uint64_t pa_add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ uint64_t pa_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ float pa_max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 // 2^x of two values on the FMA pipe: x = n + r, |r| <= 1/2, n by adding 1.5 *
-// 2^23; 2^r by its minimax polynomial; n into the exponent.  Below 2^-126 the
-// result is 0, as pa_ex2's: a masked key (-inf) must leave no part of its value
-// in O, and 2^-126 times a bf16 value near the largest is 3.5.
+// 2^23; 2^r by its minimax polynomial, times 2^n, which n's low bits in the place
+// of an exponent are from 2^-126 on, and 0 at the clamp, n = -127.  So a masked
+// key (-inf) leaves no part of its value in O (2^-126 times a bf16 value near the
+// largest is 3.5), and a NaN, which a sum of bits would turn into a number, stays
+// one in the product.
 template <bool BF>
 __device__ __forceinline__ void pa_ex2_poly(uint64_t x, float& y0, float& y1) {
   float a, b;
   pa_split(x, a, b);
   // not fmaxf: a NaN stays one
-  x = pa_two(a < -126.0f ? -126.0f : a, b < -126.0f ? -126.0f : b);
+  x = pa_two(a < -127.0f ? -127.0f : a, b < -127.0f ? -127.0f : b);
   const uint64_t n = pa_add2(x, pa_two(12582912.0f, 12582912.0f));
   const uint64_t r = pa_fma2(pa_add2(n, pa_two(-12582912.0f, -12582912.0f)), pa_two(-1.0f, -1.0f), x);
   auto c2 = [](float c) { return pa_two(c, c); };
@@ -255,11 +262,9 @@ __device__ __forceinline__ void pa_ex2_poly(uint64_t x, float& y0, float& y1) {
     p = pa_fma2(r, p, c2(PA_P41));
     p = pa_fma2(r, p, c2(PA_P40));
   }
-  float p0, p1, n0, n1;
-  pa_split(p, p0, p1);
+  float n0, n1;
   pa_split(n, n0, n1);
-  y0 = a < -126.0f ? 0.0f : __uint_as_float(__float_as_uint(p0) + (__float_as_uint(n0) << 23));
-  y1 = b < -126.0f ? 0.0f : __uint_as_float(__float_as_uint(p1) + (__float_as_uint(n1) << 23));
+  pa_split(pa_mul2(p, pa_two((__float_as_uint(n0) << 23) + 0x3F800000u, (__float_as_uint(n1) << 23) + 0x3F800000u)), y0, y1);
 }
 template <bool BF>
 __device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {

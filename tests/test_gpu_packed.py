@@ -253,3 +253,19 @@ def test_packed_hidden_values_do_not_count(native, ctx, t, hd):
     w, mag, dots = R.attention(q[:40], k[:40], v[:40], hd ** -0.5)
     tol = R.attention_tolerance(w, mag, dots, hd, 40, t, R.EPS[t] / 2) + (2.0 ** -25 * np.abs(v[:40]).sum(0) if t == "f16" else 0)
     assert not R.differs(got[:40], w, tol, t).any()
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("what", ["key", "score"])
+def test_packed_not_finite_at_every_place(native, ctx, t, hd, what):
+    """A NaN key, or a score of +inf (inf - inf in the softmax), at every place of 16 keys: NaN for the rows that see it."""
+    def edit(q, k, v):
+        q[:, :, 3] = np.abs(q[:, :, 3]) + 0.5
+        for s in range(16):
+            k[40 * s + s, 0, 3] = np.nan if what == "key" else np.inf
+
+    with np.errstate(invalid="ignore"):
+        got = check(native, ctx, t, [40] * 16, [40] * 16, 2, 1, hd, seed=32, edit=edit, same=True).reshape(16, 40, 2, hd)
+    for s in range(16):
+        assert np.isfinite(got[s, :s]).all() and np.isnan(got[s, s:]).all(), s
