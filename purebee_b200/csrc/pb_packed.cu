@@ -33,7 +33,8 @@
 //   two: the V tiles that some row must not see whole: rows behind the
 //     sequence's keys become zero (0 * inf would be NaN), and a value that is not
 //     finite under the causal mask sends the CTA's rows, once the rest is done,
-//     through the plain form below, which touches no masked value.
+//     through the plain form below, which touches no masked value.  So does a row
+//     whose scores are of 2^24 and more (PA_FAR).
 // A part of the exponentials run on the FMA pipe (pa_ex2_poly).
 //
 // Bound by the chain of a tile (S, maximum, exponentials, P) and its issue slots,
@@ -59,6 +60,11 @@ constexpr int PA_POLY_OF = 8;
 constexpr float PA_P30 = 0.999928057f, PA_P31 = 0.693261087f, PA_P32 = 0.242611334f, PA_P33 = 0.0551713221f;
 constexpr float PA_P40 = 0.999999285f, PA_P41 = 0.693121672f, PA_P42 = 0.240247354f, PA_P43 = 0.0559186637f, PA_P44 = 0.00957053155f;
 constexpr float PA_RISE = 8.0f;      // log2 of the rise that moves a row's reference
+constexpr float PA_LOW = -3e38f;     // the reference where a row sees nothing
+// From a reference of this size on, a score's product with c and its rounded form, which the reference is, may lie whole
+// numbers apart, and BIAS is lost beside it: p would be 2 to some number.  The CTA's rows then go through the plain form.
+// (Rounding the products of such rows in the loop instead: ragged prompts 162 -> 175 us, 8192 rows 527 -> 560.)
+constexpr float PA_FAR = 16777216.0f;
 
 struct pa_args {
   const void *q, *k, *v;  // the plain form reads them directly
@@ -536,7 +542,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     constexpr float BIAS = BF ? 0.0f : 7.0f;
     const float c = a.c;
     float m = 0.0f, l = 0.0f;
-    bool ok = true;
+    bool ok = true, far = false;
     auto arrived = [&](uint64_t* bar, int phase) { return __all_sync(0xffffffffu, pb_mbar_wait(bar, phase & 1, a.err)); };
     for (int j = 0; j < ni && ok; ++j) {
       if (!(ok = arrived(&s_full[i], j))) break;
@@ -575,19 +581,20 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
 #pragma unroll
         for (int x = 0; x < 64; x += 2)
           mx[x / 2 & 3] = pa_max3(mx[x / 2 & 3], __uint_as_float(sv[x]), __uint_as_float(sv[x + 1]));
-        const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c, -1e38f);
+        const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c, PA_LOW);
         // P(j - 1)'s half, which this one is written over, is used up (where P lies over S, S(j) has said so).  A wait is never
         // for a phase that the barrier may have passed twice
         if (NT == 1 && j > 0 && !(ok = arrived(&o_half[i][h], j - 1))) break;
         if (key0 == 0) {
           m = top;
+          far = fabsf(top) >= PA_FAR && top > PA_LOW;
         } else {
           const bool rise = top > m + PA_RISE;
           if (__any_sync(0xffffffffu, rise)) {  // O stands still once the product before is done
             if (!(ok = h == 0 ? arrived(&o_half[i][1], j - 1) : arrived(&o_half[i][0], j))) break;
             pa_fence_after();
             const float f = rise ? pa_ex2(m - top) : 1.0f;
-            if (rise) m = top, l *= f;
+            if (rise) m = top, l *= f, far = far || fabsf(top) >= PA_FAR;
 #pragma unroll 1
             for (int x = 0; x < HDP; x += 8) {  // few registers: the scores are live
               uint32_t o[8];
@@ -629,6 +636,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     if (ok) {
       pa_fence_after();
       const bool live = r < nq;
+      if (live && far) redo = 1;
       const float inv = sees > 0 ? 1.0f / l : 0.0f;
       uint16_t* dst = static_cast<uint16_t*>(a.out) + (int64_t)(q0 + r) * a.ldo + head_of(i) * a.hd;
 #pragma unroll 1

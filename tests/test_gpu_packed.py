@@ -269,3 +269,25 @@ def test_packed_not_finite_at_every_place(native, ctx, t, hd, what):
         got = check(native, ctx, t, [40] * 16, [40] * 16, 2, 1, hd, seed=32, edit=edit, same=True).reshape(16, 40, 2, hd)
     for s in range(16):
         assert np.isfinite(got[s, :s]).all() and np.isnan(got[s, s:]).all(), s
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("scale", [3.0, 1e4, -1e4, 1e7, -1e7, 1.5e27, -1.5e27])
+def test_packed_scores_of_any_size(native, ctx, t, hd, scale):
+    """Scores that lie a fifteenth of their size apart, up to 1e30 and more: the softmax is one key, and the output its value."""
+    n = [150, 300]
+    rng = np.random.default_rng(33)
+    q, k, v = np.ones((450, 2, hd)), np.zeros((450, 1, hd)), rng.standard_normal((450, 1, hd))
+    best = []
+    for at, c in ((0, 150), (150, 300)):
+        j = np.arange(c)
+        k[at:at + c] = -(2.0 + j % 13)[:, None, None]
+        k[at + 5], k[at + 9] = -1.0, -15.0  # the only ones of their size
+        best += [at + (5 if scale > 0 else 9)] * c
+    got, _, _, v = run(native, ctx, t, q, k, v, n, n, True, scale, same=True)
+    want = v[best, :1]
+    rows = np.r_[9:150, 159:450]  # those that see both
+    # p = 1 for the one key, exactly; the others' sum to less than 450 2^(-64 * 3 * log2(e)); 1 / l and its product: two roundings
+    tol = np.abs(want) * (R.EPS[t] / 2 * 1.01 + 2.0 ** -22)
+    assert np.all(np.abs(got - want)[rows] <= tol[rows])
