@@ -141,7 +141,7 @@ template <int TYPE, int ROPE>
 __global__ void __launch_bounds__(KA_THREADS, 4) k_kv8_append(kv8_geo g, kv8_append_args a, int y_kv) {
   constexpr int ES = TYPE == PB_TYPE_F32 ? 4 : 2;
   extern __shared__ __align__(16) unsigned char ka_raw[];
-  __shared__ kv8_found found;
+  __shared__ int found;
   __shared__ uint64_t bar;
   __shared__ uint32_t amax[KA_ROWS / (PB_KV8_BLOCK * 32 * ES)];  // by head: of k, of v
   if (threadIdx.x == 0) {
@@ -320,7 +320,7 @@ k_kv8_read(kv8_geo g, const uint8_t* pages, const int* __restrict__ starts, cons
            const int* __restrict__ table, int ld_table, int n_seqs, int n_rows, void* k_out, int ldk, void* v_out, int ldv,
            int* err) {
   extern __shared__ __align__(16) unsigned char kr_raw[];
-  __shared__ kv8_found found;
+  __shared__ int found;
   __shared__ uint64_t bar;
   const int tid = threadIdx.x;
   if (tid == 0) {

@@ -178,38 +178,36 @@ __device__ __forceinline__ float kv8_decode(uint32_t b, int code) {
 
 // Packed rows: rows starts[s] .. starts[s + 1] - 1 belong to sequence s, row
 // starts[s] + i to its token first[s] + i.  The blocks that they touch are
-// numbered so that a CTA finds its own without a scan over the sequences:
-// sequence s has the numbers from starts[s] / 16 + 2 s on, of which it uses
-// at most (tokens + 14) / 16 + 1.  A bound of the count, known to the host:
+// numbered: sequence s has the numbers from starts[s] / 16 + 2 s on, of which it
+// uses at most (tokens + 14) / 16 + 1.  A CTA looks at all sequences for the one
+// that has its number.  A bound of the count, known to the host:
 static inline int64_t kv8_units(int n_rows, int n_seqs) { return (int64_t)(n_rows / 16) + 2 * (int64_t)n_seqs; }
 struct kv8_unit {
   int seq, row0, first, n;  // the sequence, its first row, first token and token count
   int blk, lo, hi;          // the block and the tokens of it that the rows hold, as positions
 };
-struct kv8_found {
-  int seq, row0, n, first;
-};
 // Every thread of the block calls it; `sh` is shared.  False: nothing to do.
-// Row bounds that do not rise, or leave [0, n_rows], raise the error word.
+// Row bounds that do not rise, or leave [0, n_rows], raise the error word; of
+// sequences that claim the same number then, each of them within [0, n_rows], the
+// first has it, and only its index is handed over, so that its bounds stay together.
 __device__ __forceinline__ bool kv8_find_unit(const int* __restrict__ starts, const int* __restrict__ first, int n_seqs,
-                                              int n_rows, int u, kv8_found* sh, kv8_unit& un, int* err) {
-  if (threadIdx.x == 0) sh->seq = -1;
+                                              int n_rows, int u, int* sh, kv8_unit& un, int* err) {
+  if (threadIdx.x == 0) *sh = n_seqs;
   __syncthreads();
   for (int s = threadIdx.x; s < n_seqs; s += blockDim.x) {
-    const int a = starts[s], b = starts[s + 1], f = first[s];
+    const int a = starts[s], b = starts[s + 1];
     if (a < 0 || b < a || b > n_rows) {
       pb_raise(err, PB_DEVERR_BOUNDS);
     } else if ((a >> 4) + 2 * s <= u && u < (b >> 4) + 2 * s + 2) {
-      *sh = {s, a, b - a, f};
+      atomicMin(sh, s);
     }
   }
   __syncthreads();
-  const kv8_found f = *sh;
-  if (f.seq < 0) return false;
-  un.seq = f.seq;
-  un.row0 = f.row0;
-  un.n = f.n;
-  un.first = f.first;
+  un.seq = *sh;
+  if (un.seq >= n_seqs) return false;
+  un.row0 = starts[un.seq];
+  un.n = starts[un.seq + 1] - un.row0;
+  un.first = first[un.seq];
   if (un.first < 0 || un.first > 0x7FFFFFF0 - un.n) {
     if (threadIdx.x == 0) pb_raise(err, PB_DEVERR_BOUNDS);
     return false;

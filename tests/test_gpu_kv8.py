@@ -533,3 +533,41 @@ def test_bad_device_state_raises_the_error_word(native, what):
     assert c.device_error() == 1
     p.kv.free()
     c.close()
+
+
+def falling(n_rows, low):
+    """Starts of 33 sequences that fall: 0 .. n_rows, empty ones, then low .. n_rows again."""
+    return [0] + [n_rows] * 31 + [low, n_rows]
+
+
+@pytest.mark.parametrize("low", [900, 1999, 16])
+def test_starts_that_fall(native, low):
+    """Two sequences that claim the same rows, each of them within n_rows: an error word, the rows behind n_rows stay."""
+    c = native.Context(0)
+    n, guard, nkv, hd, nh = 2000, 600, 1, 32, 2
+    kv = native.KV8(c, 0, nkv, hd, 16, 33 * 130)
+    pages = c.alloc(kv.pool_bytes)
+    c._check(native.lib().pb_memset(c.h, pages.ptr, 0, kv.pool_bytes))
+    table = c.to_device(np.arange(33 * 130, dtype=np.int32).reshape(33, 130))
+    st, zero = c.to_device(np.array(falling(n, low), np.int32)), c.to_device(np.zeros(33, np.int32))
+    rows = n + guard
+    x = c.to_device(np.ones((rows, (nh + 2 * nkv) * hd), np.float32))
+    w = (nh + 2 * nkv) * hd
+    o = [c.to_device(np.full((rows, k * hd), 7, np.float32)) for k in (nh, nkv, nkv)]
+    kv.append(pages.ptr, 0, x.ptr, w, x.ptr + 4 * nh * hd, w, x.ptr + 4 * (nh + nkv) * hd, w, nh, st.ptr, zero.ptr, table.ptr, 130, 33,
+              n, 0, o[0].ptr, nh * hd, o[1].ptr, nkv * hd, o[2].ptr, nkv * hd)
+    with pytest.raises(native.PureBeeError, match="PB_ERR_DEVICE.*bounds"):
+        c.sync()
+
+    def values(b):  # downloads report the raised word
+        a = np.empty(b.nbytes // 4, np.float32)
+        assert native.lib().pb_download(c.h, native.ptr(a), b.ptr, a.nbytes) == native.PB_ERR_DEVICE
+        return a.reshape(rows, -1)
+
+    for b in o:
+        assert np.all(values(b)[n:] == 7)
+    kv.read(pages.ptr, st.ptr, zero.ptr, table.ptr, 130, 33, n, 0, o[1].ptr, nkv * hd, o[2].ptr, nkv * hd)
+    for b in o[1:]:
+        assert np.all(values(b)[n:] == 7)
+    kv.free()
+    c.close()
