@@ -437,9 +437,10 @@ static kr_kernel kr_kernel_of(int code, int otype) {
 // byte digits q = f (i0 + i1 / 254 + i2 / 254^2), f from the row's largest, so
 // the products and sums are exact: three digits (24 bits) for f32 rows, two (16
 // bits below the row's largest) for 16-bit rows.
-// With e4m3 codes: m16n8k16 in f16 with q = hi + lo for f32 rows, or q in f16
-// after a power of two for 16-bit rows (what f16 cannot hold of them lies 2^-25
-// or more below the row's largest).
+// With e4m3 codes: m16n8k16 in f16 with q = hi + lo for f32 rows, or q in f16 for
+// 16-bit rows, after a power of two that brings the row's largest to 2^14 .. 2^15,
+// f16's top: what f16's smallest step, 2^-24, takes from the other values lies 2^-39
+// or more below the largest, so channels far below a loud one keep their bits.
 //
 // Scales: S's columns times 2^ke of the block.  V's 2^ve is put into the
 // exponent, p' = 2^(s + ve - m2), with a running reference m2 of s + ve of its
@@ -458,6 +459,7 @@ constexpr int KT_COST = 32;
 __host__ __device__ constexpr int kt_stages(int hd) { return hd <= 64 ? 4 : 2; }
 constexpr float KT_RISE = 8.0f, KT_BIAS = 6.0f;  // p' <= 2^(8 + 6)
 constexpr float KT_LOW = -1e30f;
+constexpr float KT_QTOP = 32768.0f;  // queries in f16 lie below it
 
 struct kt_args {
   const uint8_t* pages;
@@ -740,7 +742,7 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
     const float up = nan ? __int_as_float(0x7fc00000) : tiny ? 0.0f : 1.0f;
     if (a.scale < 0.0f) inv = -inv;  // the factor stays positive
     if (DIGITS) inv *= 127.0f;
-    qf[r] = fabsf(a.scale) * (up * kv8_pow2(max(-126, min(127, e)))) * (DIGITS ? LO ? 1.0f / 127.0f : 1.0f / (127.0f * 254.0f) : 1.0f);
+    qf[r] = fabsf(a.scale) * (up * kv8_pow2(max(-126, min(127, e)))) * (DIGITS ? LO ? 1.0f / 127.0f : 1.0f / (127.0f * 254.0f) : 1.0f / KT_QTOP);
     if (e == 128) qf[r] *= 2.0f;  // 2^128 in two steps
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -748,7 +750,7 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
       for (int s = 0; s < 2; ++s) {  // values 4s .. 4s + 3 of the lane's 8
         float y[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = x[i][4 * s + j] * inv;  // of a row that is not finite: anything, times NaN
+        for (int j = 0; j < 4; ++j) y[j] = x[i][4 * s + j] * inv * (DIGITS ? 1.0f : KT_QTOP);  // of a row that is not finite: anything, times NaN
         if constexpr (DIGITS) {
           // adding 1.5 * 2^23 rounds to an integer, whose low byte is the digit
           const float big = 12582912.0f;

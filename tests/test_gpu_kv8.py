@@ -571,3 +571,30 @@ def test_starts_that_fall(native, low):
         assert np.all(values(b)[n:] == 7)
     kv.free()
     c.close()
+
+
+LOUD = [(64, 4, 1), (128, 8, 2), (96, 5, 3), (160, 2, 1), (256, 8, 2)]
+
+
+def check_loud_query_channels(native, ctx, code, t, hd, group, n):
+    """Query channels far above the others, of keys that are zero or quiet there: the others keep their bits.  All rows, then
+    one row of a tile and some of another's channels."""
+    p = Pool(native, ctx, code, 1, hd, 32, 2, 150, seed=60 + code)
+
+    def edit(kv):
+        kv[:, 0, :, 5] = 0
+        kv[:, 0, :, 7:10] *= 2.0 ** -12
+    p.append([140, 35], [0, 0], 1, edit=edit)
+    for loud in (30.0, 300.0, 10000.0, 60000.0):
+        q = p.rng.standard_normal((2 * n, group, hd))
+        q[..., 5] = loud
+        p.check_attn(group, [n, n], [140, 35], t, q=q)
+        q = p.rng.standard_normal((2 * n, group, hd))
+        q[-1, 0, 5], q[0, -1, 7:10] = -loud, loud
+        p.check_attn(group, [n, n], [140, 35], t, q=q)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd,group,n", LOUD)
+def test_attention_loud_query_channels_e4m3(native, ctx, t, hd, group, n):
+    check_loud_query_channels(native, ctx, 1, t, hd, group, n)
