@@ -433,14 +433,20 @@ static kr_kernel kr_kernel_of(int code, int otype) {
 // operand.  f32 rows (LO, TR = 8): rows 0-7 hold hi = f16(p), rows 8-15 lo =
 // f16(p - hi), 22 bits at no extra product; 16-bit rows, whose output has no more
 // than f16's bits, round p once, half a step of f16.
-// S = Q K^T with int8 codes: m16n8k32 on the codes as they are, q in signed
-// byte digits q = f (i0 + i1 / 254 + i2 / 254^2), f from the row's largest, so
-// the products and sums are exact: three digits (24 bits) for f32 rows, two (16
-// bits below the row's largest) for 16-bit rows.
-// With e4m3 codes: m16n8k16 in f16 with q = hi + lo for f32 rows, or q in f16 for
-// 16-bit rows, after a power of two that brings the row's largest to 2^14 .. 2^15,
-// f16's top: what f16's smallest step, 2^-24, takes from the other values lies 2^-39
-// or more below the largest, so channels far below a loud one keep their bits.
+// S = Q K^T: m16n8k16 in f16, the codes made f16, with q = hi + lo for f32 rows (22
+// bits), q in f16 for 16-bit rows, after a power of two that brings the row's largest
+// to 2^14 .. 2^15, f16's top: what f16's smallest step, 2^-24, takes from the other
+// values lies 2^-39 or more below the largest, so channels far below a loud one keep
+// their bits.
+// 16-bit rows over int8 codes: m16n8k32 on the codes as they are, q in signed byte
+// digits q = f (i0 + i1 / 254), f from the row's largest, so the products and sums
+// are exact.  Digits have one step for the whole row: they are off by at most 2^-16
+// of the power of two above its largest value.  That is f16's own rounding of values
+// 32 times below (KT_EVEN), and 85 in 100 values of a normal distribution lie above
+// those.  Where more than half of a row lies below, a few loud channels over quiet
+// ones, the tile takes its queries in f16 as above (drafted tokens 75.7 us with even
+// rows, 95.8 with a channel 100 times the others; one f32 row a kv head takes f16
+// queries always: 2 x 131072 tokens 94.0 us with three digits, 88.0 so).
 //
 // Scales: S's columns times 2^ke of the block.  V's 2^ve is put into the
 // exponent, p' = 2^(s + ve - m2), with a running reference m2 of s + ve of its
@@ -460,6 +466,7 @@ __host__ __device__ constexpr int kt_stages(int hd) { return hd <= 64 ? 4 : 2; }
 constexpr float KT_RISE = 8.0f, KT_BIAS = 6.0f;  // p' <= 2^(8 + 6)
 constexpr float KT_LOW = -1e30f;
 constexpr float KT_QTOP = 32768.0f;  // queries in f16 lie below it
+constexpr float KT_EVEN = 32.0f;     // digits serve values down to this part of the power above the row's largest
 
 struct kt_args {
   const uint8_t* pages;
@@ -708,81 +715,97 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
   for (int i = 0; i < STAGES; ++i) fetch(i);
 
   // Q as A fragments in the tiles' order, scaled by the row's largest; qf undoes it
-  constexpr bool DIGITS = CODE == PB_KV8_INT8;
-  constexpr int QN = HL && !LO ? 4 : DIGITS && HL ? 6 : 8;  // registers a tile
+  constexpr bool DIGITS = CODE == PB_KV8_INT8 && !LO;
+  constexpr int QN = HL && !LO ? 4 : 8;  // registers a tile
   uint32_t qa[NT][QN];
   float qf[NR];
   int see[NR];  // keys the row sees
+  // As digits, or in f16; gives whether digits do not serve one of the lane's rows
+  auto queries = [&](auto kind) {
+    constexpr bool DIG = decltype(kind)::value;
+    bool spread = false;
 #pragma unroll
-  for (int r = 0; r < NR; ++r) {
-    const int rho = rho0 + gq + 8 * r;
-    const bool on = rho < rows;
-    const int tok = on ? rho / a.group : 0, h = kvh * a.group + (on ? rho % a.group : 0);
-    see[r] = on ? max(0, len - nq + tok + 1) : 0;
-    const int64_t at = (int64_t)(row0 + tok) * a.ldq + h * HD + 8 * t;
-    float x[NT][8];
-    uint32_t m = 0;
+    for (int r = 0; r < NR; ++r) {
+      const int rho = rho0 + gq + 8 * r;
+      const bool on = rho < rows;
+      const int tok = on ? rho / a.group : 0, h = kvh * a.group + (on ? rho % a.group : 0);
+      see[r] = on ? max(0, len - nq + tok + 1) : 0;
+      const int64_t at = (int64_t)(row0 + tok) * a.ldq + h * HD + 8 * t;
+      float x[NT][8];
+      uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      if (on) {
-        kv8_load(a.q, a.type, at + 32 * i, x[i]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[i][j] = 0.0f;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[i][j]) & 0x7FFFFFFFu);
-    }
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    // 2^-e brings the largest into [1/2, 1); a row below 2^-118 counts as zeros (its scores would be below 2^-40 for scales up to 1), one that is not finite as NaN
-    const int e = (int)(m >> 23) - 126;
-    const bool nan = m >= 0x7F800000u, tiny = e < -118;
-    float inv = nan || tiny ? 0.0f : e > 126 ? kv8_pow2(-126) * kv8_pow2(126 - e) : kv8_pow2(-e);
-    const float up = nan ? __int_as_float(0x7fc00000) : tiny ? 0.0f : 1.0f;
-    if (a.scale < 0.0f) inv = -inv;  // the factor stays positive
-    if (DIGITS) inv *= 127.0f;
-    qf[r] = fabsf(a.scale) * (up * kv8_pow2(max(-126, min(127, e)))) * (DIGITS ? LO ? 1.0f / 127.0f : 1.0f / (127.0f * 254.0f) : 1.0f / KT_QTOP);
-    if (e == 128) qf[r] *= 2.0f;  // 2^128 in two steps
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {  // values 4s .. 4s + 3 of the lane's 8
-        float y[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = x[i][4 * s + j] * inv * (DIGITS ? 1.0f : KT_QTOP);  // of a row that is not finite: anything, times NaN
-        if constexpr (DIGITS) {
-          // adding 1.5 * 2^23 rounds to an integer, whose low byte is the digit
-          const float big = 12582912.0f;
-          uint32_t b0[4], b1[4], b2[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float t0 = __fadd_rn(y[j], big), r0 = __fsub_rn(y[j], __fsub_rn(t0, big));
-            const float t1 = __fmaf_rn(r0, 254.0f, big), r1 = __fmaf_rn(r0, 254.0f, -__fsub_rn(t1, big));
-            b0[j] = __float_as_uint(t0), b1[j] = __float_as_uint(t1), b2[j] = __float_as_uint(__fmaf_rn(r1, 254.0f, big));
-          }
-          auto bytes = [](const uint32_t (&b)[4]) {
-            return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-          };
-          const uint32_t d0 = bytes(b0), d1 = bytes(b1), d2 = LO ? bytes(b2) : 0u;
-          if (HL) {
-            qa[i][2 * s] = d0, qa[i][2 * s + 1] = d1;
-            if (LO) qa[i][(QN == 6 ? 4 : 0) + s] = d2;
-          }
-          else qa[i][2 * s + r] = d0, qa[i][(QN == 8 ? 4 : 0) + 2 * s + r] = d1;
-        } else if (HL && !LO) {
-          qa[i][2 * s] = kt_h2(y[0], y[1]);
-          qa[i][2 * s + 1] = kt_h2(y[2], y[3]);
+      for (int i = 0; i < NT; ++i) {
+        if (on) {
+          kv8_load(a.q, a.type, at + 32 * i, x[i]);
         } else {
-          uint32_t* q4 = &qa[i][(QN == 8 ? 4 : 0) * s];
-          q4[r] = kt_h2(y[0], y[1]);
-          q4[2 + r] = kt_h2(y[2], y[3]);
-          if (HL) {
-            q4[1] = kt_lo2(y[0], y[1], q4[0]);
-            q4[3] = kt_lo2(y[2], y[3], q4[2]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[i][j] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[i][j]) & 0x7FFFFFFFu);
+      }
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      // 2^-e brings the largest into [1/2, 1); a row below 2^-118 counts as zeros (its scores would be below 2^-40 for scales up to 1), one that is not finite as NaN
+      const int e = (int)(m >> 23) - 126;
+      const bool nan = m >= 0x7F800000u, tiny = e < -118;
+      float inv = nan || tiny ? 0.0f : e > 126 ? kv8_pow2(-126) * kv8_pow2(126 - e) : kv8_pow2(-e);
+      const float up = nan ? __int_as_float(0x7fc00000) : tiny ? 0.0f : 1.0f;
+      if (a.scale < 0.0f) inv = -inv;  // the factor stays positive
+      if (DIG) inv *= 127.0f;
+      qf[r] = fabsf(a.scale) * (up * kv8_pow2(max(-126, min(127, e)))) * (DIG ? 1.0f / (127.0f * 254.0f) : 1.0f / KT_QTOP);
+      if (e == 128) qf[r] *= 2.0f;  // 2^128 in two steps
+      int low = 0;
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {  // values 4s .. 4s + 3 of the lane's 8
+          float y[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[j] = x[i][4 * s + j] * inv * (DIG ? 1.0f : KT_QTOP);  // of a row that is not finite: anything, times NaN
+          if constexpr (DIG) {
+            // adding 1.5 * 2^23 rounds to an integer, whose low byte is the digit
+            const float big = 12582912.0f;
+            uint32_t b0[4], b1[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              low += fabsf(y[j]) < 127.0f / KT_EVEN ? 1 : 0;
+              const float t0 = __fadd_rn(y[j], big), r0 = __fsub_rn(y[j], __fsub_rn(t0, big));
+              b0[j] = __float_as_uint(t0), b1[j] = __float_as_uint(__fmaf_rn(r0, 254.0f, big));
+            }
+            auto bytes = [](const uint32_t (&b)[4]) {
+              return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+            };
+            const uint32_t d0 = bytes(b0), d1 = bytes(b1);
+            if (HL) qa[i][2 * s] = d0, qa[i][2 * s + 1] = d1;
+            else qa[i][2 * s + r] = d0, qa[i][(QN == 8 ? 4 : 0) + 2 * s + r] = d1;
+          } else if (HL && !LO) {
+            qa[i][2 * s] = kt_h2(y[0], y[1]);
+            qa[i][2 * s + 1] = kt_h2(y[2], y[3]);
+          } else {
+            uint32_t* q4 = &qa[i][(QN == 8 ? 4 : 0) * s];
+            q4[r] = kt_h2(y[0], y[1]);
+            q4[2 + r] = kt_h2(y[2], y[3]);
+            if (HL) {
+              q4[1] = kt_lo2(y[0], y[1], q4[0]);
+              q4[3] = kt_lo2(y[2], y[3], q4[2]);
+            }
           }
         }
+      if (DIG) {
+        low += __shfl_xor_sync(0xffffffffu, low, 1);
+        low += __shfl_xor_sync(0xffffffffu, low, 2);
+        spread = spread || (2 * low > HD && !nan && !tiny);
       }
+    }
+    return spread;
+  };
+  bool wide = false;  // int8 codes, queries in f16: the same on every lane and warp, which hold the same rows
+  if constexpr (DIGITS) {
+    wide = __any_sync(0xffffffffu, queries(std::true_type()));
+    if (wide) queries(std::false_type());
+  } else {
+    queries(std::false_type());
   }
   // the fewest keys a live row of the tile sees: blocks up to there need no mask
   const int see_min = max(0, len - nq + rho0 / a.group + 1);
@@ -805,8 +828,8 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
     const int b = first_block(i), tok0 = b * PB_KV8_BLOCK;
     const bool one = b < blocks, two = b + 1 < blocks;
     // x times qf and the block's scale: scores times log2(e), tokens 2t, 2t + 1, 2t + 8, 2t + 9 of a block
-    auto scores = [&](const unsigned char* bk, float (&x0)[4], float (&x1)[4]) {
-      if constexpr (DIGITS) {
+    auto scores = [&](auto kind, const unsigned char* bk, float (&x0)[4], float (&x1)[4]) {
+      if constexpr (decltype(kind)::value) {  // digits
         int ca[2][4], cb[2][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -818,10 +841,7 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
           const uint32_t* q = qa[n];
           kt_mma_s8(ca[0], q[0], q[1], q[2], q[3], w.x, w.y);
           kt_mma_s8(ca[1], q[0], q[1], q[2], q[3], w.z, w.w);
-          if constexpr (HL && LO) {
-            kt_mma_s8(cb[0], q[4], 0u, q[5], 0u, w.x, w.y);
-            kt_mma_s8(cb[1], q[4], 0u, q[5], 0u, w.z, w.w);
-          } else if constexpr (!HL) {
+          if constexpr (!HL) {
             kt_mma_s8(cb[0], q[4], q[5], q[6], q[7], w.x, w.y);
             kt_mma_s8(cb[1], q[4], q[5], q[6], q[7], w.z, w.w);
           }
@@ -829,10 +849,8 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
 #pragma unroll
         for (int j = 0; j < 4; ++j) {  // |sums of a digit| <= 256 * 127 * 127: times 254 they and the next digit's stay below 2^31
           const int *c = ca[j >> 1], *d = cb[j >> 1], z = j & 1;
-          if (HL && !LO) {
+          if (HL) {
             x0[j] = (float)(c[z] * 254 + c[2 + z]);
-          } else if (HL) {
-            x0[j] = __fmaf_rn((float)(c[2 + z] * 254 + d[z]), 1.0f / 64516.0f, (float)c[z]);
           } else {
             x0[j] = (float)(c[z] * 254 + d[z]);
             x1[j] = (float)(c[2 + z] * 254 + d[2 + z]);
@@ -873,7 +891,7 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
     auto odd = [](int es) { const int e = es >> 8; return e == KV8_E_ZERO || e == KV8_E_NAN; };
     const bool mask = tok0 + 2 * PB_KV8_BLOCK > see_min;
     auto pair = [&](auto kind) {
-    constexpr bool PLAIN = decltype(kind)::value;  // two blocks, no mask, values to count
+    constexpr bool PLAIN = decltype(kind)::value;  // two blocks, no mask, values to count, queries as the code has them
     float x[2][2][4], fx[2][NR];  // [block][row], a score is x * fx
     // log2 of V's scale where the block's values count in f16's way; the others (no values, not finite) take a way of their own
     float vadd[2];
@@ -887,7 +905,8 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
         const float ks = kv8_scale((int8_t)(es[h] & 0xFF));
 #pragma unroll
         for (int r = 0; r < NR; ++r) fx[h][r] = qf[r] * ks;
-        scores(bk, x[h][0], x[h][1]);
+        if (DIGITS && (PLAIN || !wide)) scores(std::integral_constant<bool, DIGITS>(), bk, x[h][0], x[h][1]);
+        else scores(std::false_type(), bk, x[h][0], x[h][1]);
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[h][0][j] = x[h][1][j] = -INFINITY;
@@ -982,7 +1001,7 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
     if (PLAIN || one) values(blk, pa[0]);
     if (PLAIN || two) values(blk + BB, pa[1]);
     };
-    if (two && !mask && !odd(es0) && !odd(es1)) pair(std::true_type());
+    if (two && !mask && !odd(es0) && !odd(es1) && !wide) pair(std::true_type());
     else pair(std::false_type());
     // every lane's reads of the stage come before the copy that refills it
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

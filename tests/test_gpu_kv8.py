@@ -598,3 +598,9 @@ def check_loud_query_channels(native, ctx, code, t, hd, group, n):
 @pytest.mark.parametrize("hd,group,n", LOUD)
 def test_attention_loud_query_channels_e4m3(native, ctx, t, hd, group, n):
     check_loud_query_channels(native, ctx, 1, t, hd, group, n)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd,group,n", LOUD)
+def test_attention_loud_query_channels_int8(native, ctx, t, hd, group, n):
+    check_loud_query_channels(native, ctx, 0, t, hd, group, n)
