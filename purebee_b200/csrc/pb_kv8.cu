@@ -449,10 +449,14 @@ static kr_kernel kr_kernel_of(int code, int otype) {
 // queries always: 2 x 131072 tokens 94.0 us with three digits, 88.0 so).
 //
 // Scales: S's columns times 2^ke of the block.  V's 2^ve is put into the
-// exponent, p' = 2^(s + ve - m2), with a running reference m2 of s + ve of its
-// own, so p' uses f16's range whatever V's scales (below 2^-14 its last bit is
-// 2^-24, which is 2^-30 of the row's largest p 2^ve); the sum l runs beside it
-// over 2^(s - m1).  out = O / l * 2^(m2 - m1).
+// exponent, p' = 2^(s - m1 + ve - m2), with a running reference m1 of s and m2 of
+// s - m1 + ve, so p' uses f16's range whatever V's scales (below 2^-14 its last bit
+// is 2^-24, which is 2^-30 of the row's largest p 2^ve); the sum l runs beside it
+// over 2^(s - m1).  out = O / l * 2^m2.  m2 is counted from m1, so that ve and 2^m2
+// keep their bits beside scores of any size, and is a whole number, so that the key
+// whose score m1 is has a p' without rounding.  From 2^24 on (KT_FAR) a score's
+// product and its rounded form, which m1 is, may lie whole numbers apart: it is
+// rounded for all keys there.
 //
 // Measured (8 kv heads of 128 values): 2 x 131072 tokens, int8, 64 f16 heads: 93
 // us, 5.4 TB/s of codes; 64 ragged sequences up to 9000 tokens, e4m3, 32 bf16
@@ -465,6 +469,7 @@ constexpr int KT_COST = 32;
 __host__ __device__ constexpr int kt_stages(int hd) { return hd <= 64 ? 4 : 2; }
 constexpr float KT_RISE = 8.0f, KT_BIAS = 6.0f;  // p' <= 2^(8 + 6)
 constexpr float KT_LOW = -1e30f;
+constexpr float KT_FAR = 16777216.0f;
 constexpr float KT_QTOP = 32768.0f;  // queries in f16 lie below it
 constexpr float KT_EVEN = 32.0f;     // digits serve values down to this part of the power above the row's largest
 
@@ -572,40 +577,45 @@ __device__ __forceinline__ void kt_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
 struct kt_pend {
   int c0, first_part, n_parts, row0, rows, len, kvh, rho0;
 };
-// Four values of a row's O under the reference m2, the row's sum l under m1.
+// Four values of a row's O under the reference m1 + m2, the row's sum l under m1.
 struct kt_sum {
   float4 o = {0, 0, 0, 0};
   float m1 = KT_LOW, m2 = KT_LOW, l = 0.0f;
   // n parts' values at p, p + stride, ..., their {m1, m2, l} `m` floats further: the references first, so that the sums
   // depend on one another by an addition only
   __device__ __forceinline__ void add(const float* p, int stride, int m, int n) {
-    float n1 = m1, n2 = m2;
+    float n1 = m1;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) n1 = fmaxf(n1, p[i * stride + m]);
+    float n2 = m2 + (m1 - n1);
 #pragma unroll 4
     for (int i = 0; i < n; ++i) {
       const float2 v = *reinterpret_cast<const float2*>(p + i * stride + m);
-      n1 = fmaxf(n1, v.x), n2 = fmaxf(n2, v.y);
+      n2 = fmaxf(n2, v.y + (v.x - n1));
     }
-    const float f1 = kt_ex2(m1 - n1), f2 = kt_ex2(m2 - n2);
+    n2 = floorf(n2);
+    const float f1 = kt_ex2(m1 - n1), f2 = kt_ex2(m2 + (m1 - n1) - n2);
     m1 = n1, m2 = n2;
     l *= f1, o.x *= f2, o.y *= f2, o.z *= f2, o.w *= f2;
 #pragma unroll 4
     for (int i = 0; i < n; ++i) {
       const float4 v = *reinterpret_cast<const float4*>(p + i * stride + m), x = *reinterpret_cast<const float4*>(p + i * stride);
-      const float w = kt_ex2(v.y - n2);
+      const float w = kt_ex2(v.y + (v.x - n1) - n2);
       l = __fmaf_rn(v.z, kt_ex2(v.x - n1), l);
       o.x = __fmaf_rn(x.x, w, o.x), o.y = __fmaf_rn(x.y, w, o.y), o.z = __fmaf_rn(x.z, w, o.z), o.w = __fmaf_rn(x.w, w, o.w);
     }
   }
 };
-// out of a row's four values at d: O / l * 2^(m2 - m1)
+// out of a row's four values at d: O / l * 2^m2
 __device__ __forceinline__ void kt_finish(const kv8_geo& g, const kt_args& a, int row0, int rows, int len, int kvh, int rho,
                                           int d, const kt_sum& s) {
   const int tok = rho / a.group, h = kvh * a.group + rho % a.group;
   float y[4] = {0, 0, 0, 0};
   if (len - rows / a.group + tok >= 0) {  // the row sees a key
-    // 2^up in two halves: it may pass f32's range where the row's values do not
-    const float f = 1.0f / s.l, u0 = kt_ex2(0.5f * (s.m2 - s.m1 - KT_BIAS));
-    y[0] = s.o.x * f * u0 * u0, y[1] = s.o.y * f * u0 * u0, y[2] = s.o.z * f * u0 * u0, y[3] = s.o.w * f * u0 * u0;
+    // 2^m2 in two halves: it may pass f32's range where the row's values do not
+    const int e = (int)fmaxf(-252.0f, fminf(252.0f, s.m2 - KT_BIAS));
+    const float f = 1.0f / s.l, u0 = kv8_pow2(e >> 1), u1 = kv8_pow2(e - (e >> 1));
+    y[0] = s.o.x * f * u0 * u1, y[1] = s.o.y * f * u0 * u1, y[2] = s.o.z * f * u0 * u1, y[3] = s.o.w * f * u0 * u1;
   }
   kv8_store(a.out, a.type, (int64_t)(row0 + tok) * a.ldo + h * g.hd + d, y);
 }
@@ -820,6 +830,7 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
 #pragma unroll
   for (int r = 0; r < NR; ++r) m1[r] = m2[r] = KT_LOW, l[r] = 0.0f;
 
+  bool far = false;  // a reference of KT_FAR: the same on every lane
   int i = 0;
   for (; i < mine; ++i) {
     const int st = (used + i) % STAGES;
@@ -917,6 +928,11 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
     uint32_t pa[2][4];
     float rescale[NR];
     bool any = false;
+    auto rounded = [&](int r) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j >> 2][r][j & 3] *= fx[j >> 2][r];
+      fx[0][r] = fx[1][r] = 1.0f;
+    };
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       if (!PLAIN && mask) {  // -inf, whatever the factor
@@ -928,46 +944,56 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
         fx[0][r] = fx[1][r] = 1.0f;
       }
       const float *xa = x[0][r], *xb = x[1][r];
-      const float ba = fmaxf(fmaxf(xa[0], xa[1]), fmaxf(xa[2], xa[3])) * fx[0][r];
-      const float bb = fmaxf(fmaxf(xb[0], xb[1]), fmaxf(xb[2], xb[3])) * fx[1][r];
-      float bm = fmaxf(ba, bb), bv = fmaxf(ba + vadd[0], bb + vadd[1]);
+      const float ta = fmaxf(fmaxf(xa[0], xa[1]), fmaxf(xa[2], xa[3])), tb = fmaxf(fmaxf(xb[0], xb[1]), fmaxf(xb[2], xb[3]));
+      const float ya = __fmaf_rn(ta, fx[0][r], -m1[r]), yb = __fmaf_rn(tb, fx[1][r], -m1[r]);
       // the references move when a score passes them by 2^8: looked at by the quad only where a lane of the warp saw one
       rescale[r] = 1.0f;
-      if (__any_sync(0xffffffffu, bm > m1[r] + KT_RISE || bv > m2[r] + KT_RISE)) {
+      if (__any_sync(0xffffffffu, fmaxf(ya, yb) > KT_RISE || fmaxf(ya + vadd[0], yb + vadd[1]) > m2[r] + KT_RISE)) {
+        const float ba = ta * fx[0][r], bb = tb * fx[1][r];
+        float bm = fmaxf(ba, bb);
         bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 1));
         bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
-        bv = fmaxf(bv, __shfl_xor_sync(0xffffffffu, bv, 1));
-        bv = fmaxf(bv, __shfl_xor_sync(0xffffffffu, bv, 2));
-        if (bm > m1[r] + KT_RISE) {
-          l[r] *= kt_ex2(m1[r] - bm);
+        const bool rise = bm > m1[r] + KT_RISE;
+        if (rise) {
+          const float f = m1[r] - bm;
+          l[r] *= kt_ex2(f);
+          m2[r] = fmaxf(m2[r] + f, KT_LOW);
           m1[r] = bm;
         }
-        if (bv > m2[r] + KT_RISE) {
-          rescale[r] = kt_ex2(m2[r] - bv);
-          m2[r] = bv;
+        far = __any_sync(0xffffffffu, rise && fabsf(m1[r]) >= KT_FAR) || far;
+        float bv = fmaxf(ba - m1[r] + vadd[0], bb - m1[r] + vadd[1]);
+        bv = fmaxf(bv, __shfl_xor_sync(0xffffffffu, bv, 1));
+        bv = fmaxf(bv, __shfl_xor_sync(0xffffffffu, bv, 2));
+        if (rise || bv > m2[r] + KT_RISE) {
+          const float n2 = floorf(bv > m2[r] + KT_RISE ? bv : m2[r]);
+          rescale[r] = kt_ex2(m2[r] - n2);
+          m2[r] = n2;
         }
         any = true;
+        if (PLAIN && far) rounded(r);
       }
-      const float top = KT_BIAS - m2[r];
+      if (!PLAIN && far) rounded(r);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        const float c = vadd[h] + (KT_BIAS - m2[r]);
         float p[4], sum = 0.0f;
         if (!PLAIN && odd(es[h])) {  // p' is 0 or NaN there: the sum by itself
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            sum += kt_ex2(__fmaf_rn(x[h][r][j], fx[h][r], -m1[r]));
-            p[j] = x[h][r][j] == -INFINITY ? 0.0f : kt_ex2(__fmaf_rn(x[h][r][j], fx[h][r], vadd[h] + top));  // -inf: masked
+            const float y = __fmaf_rn(x[h][r][j], fx[h][r], -m1[r]);
+            sum += kt_ex2(y);
+            p[j] = x[h][r][j] == -INFINITY ? 0.0f : kt_ex2(y + c);  // -inf: masked
           }
           l[r] += sum;
         } else {
-          // l's 2^(x - m1) is p' times one factor a block: V's exponents lie within 100 of each other, so p' keeps
-          // its f32 precision wherever 2^(x - m1) counts
+          // l's 2^(s - m1) is p' times one factor a block: V's exponents lie within 100 of each other, so p' keeps
+          // its f32 precision wherever 2^(s - m1) counts
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            p[j] = kt_ex2(__fmaf_rn(x[h][r][j], fx[h][r], vadd[h] + top));
+            p[j] = kt_ex2(__fmaf_rn(x[h][r][j], fx[h][r], -m1[r]) + c);
             sum += p[j];
           }
-          l[r] = __fmaf_rn(sum, kt_ex2(-(vadd[h] + top) - m1[r]), l[r]);
+          l[r] = __fmaf_rn(sum, kt_ex2(-c), l[r]);
         }
         pa[h][r] = kt_h2(p[0], p[1]);
         pa[h][2 + r] = kt_h2(p[2], p[3]);
@@ -1001,7 +1027,7 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
     if (PLAIN || one) values(blk, pa[0]);
     if (PLAIN || two) values(blk + BB, pa[1]);
     };
-    if (two && !mask && !odd(es0) && !odd(es1) && !wide) pair(std::true_type());
+    if (two && !mask && !odd(es0) && !odd(es1) && !wide && !far) pair(std::true_type());
     else pair(std::false_type());
     // every lane's reads of the stage come before the copy that refills it
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

@@ -604,3 +604,34 @@ def test_attention_loud_query_channels_e4m3(native, ctx, t, hd, group, n):
 @pytest.mark.parametrize("hd,group,n", LOUD)
 def test_attention_loud_query_channels_int8(native, ctx, t, hd, group, n):
     check_loud_query_channels(native, ctx, 0, t, hd, group, n)
+
+
+@pytest.mark.parametrize("code", [0, 1])
+@pytest.mark.parametrize("t,group,n", [("f32", 2, 1), ("f16", 4, 1), ("bf16", 8, 2)])
+@pytest.mark.parametrize("scale", [3.0, 1e4, -1e4, 1e7, -1e7, 1.5e27, -1.5e27])
+def test_attention_scores_of_any_size(native, ctx, code, t, group, n, scale):
+    check_one_key(native, ctx, code, t, group, n, scale)
+
+
+def check_one_key(native, ctx, code, t, group, n, scale):
+    """Scores that lie a fifteenth of their size apart, up to 1e30 and more: the softmax is one key, and the output its
+    value, whatever the scales of the blocks of V."""
+    hd, lens = 64, [2100, 90]
+    p = Pool(native, ctx, code, 1, hd, 16, 2, 2100, seed=70)
+
+    def edit(kv):
+        for at, c in ((0, 2100), (2100, 90)):
+            j = np.arange(c)
+            kv[at:at + c, 0] = -(2.0 + j % 13)[:, None, None]
+            kv[at + 17, 0], kv[at + 40, 0] = -1.0, -15.0  # the only ones of their size
+            kv[at + 16:at + 32, 1] *= 2.0 ** 9
+            kv[at + 32:at + 48, 1] *= 2.0 ** -9
+    p.append(lens, [0, 0], 1, edit=edit)
+    got, _ = p.attn(np.ones((2 * n, group, hd)), [n, n], lens, t, scale)
+    best = 17 if scale > 0 else 40
+    for s in (0, 1):
+        want = p.ref[s].values(1, 64)[best]
+        # p = 1 for the one key, exactly; the others' sum, below 2100 2^(-64 * 3 * log2(e)) of it; then O / l (the quotient, the
+        # product and l's power of two: 2^-22 in all) and the output's rounding, which for f16 has its smallest step
+        tol = np.abs(want) * (R.EPS[t] / 2 * 1.01 + 2.0 ** -20) + (2.0 ** -25 if t == "f16" else 0)
+        assert np.all(np.abs(got[s * n:(s + 1) * n] - want) <= tol), (s, got[s * n, 0, :4], want[0, :4])
