@@ -468,7 +468,7 @@ constexpr int KT_WARPS = 4;
 constexpr int KT_COST = 32;
 __host__ __device__ constexpr int kt_stages(int hd) { return hd <= 64 ? 4 : 2; }
 constexpr float KT_RISE = 8.0f, KT_BIAS = 6.0f;  // p' <= 2^(8 + 6)
-constexpr float KT_LOW = -1e30f;
+constexpr float KT_LOW = -3e38f;         // a reference before the first score: below every score that f32 holds well
 constexpr float KT_FAR = 16777216.0f;
 constexpr float KT_QTOP = 32768.0f;  // queries in f16 lie below it
 constexpr float KT_EVEN = 32.0f;     // digits serve values down to this part of the power above the row's largest

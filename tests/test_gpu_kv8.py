@@ -635,3 +635,10 @@ def check_one_key(native, ctx, code, t, group, n, scale):
         # product and l's power of two: 2^-22 in all) and the output's rounding, which for f16 has its smallest step
         tol = np.abs(want) * (R.EPS[t] / 2 * 1.01 + 2.0 ** -20) + (2.0 ** -25 if t == "f16" else 0)
         assert np.all(np.abs(got[s * n:(s + 1) * n] - want) <= tol), (s, got[s * n, 0, :4], want[0, :4])
+
+
+@pytest.mark.parametrize("code", [0, 1])
+@pytest.mark.parametrize("t,group,n", [("f32", 2, 1), ("f16", 4, 1), ("bf16", 8, 2)])
+def test_attention_all_scores_far_below_zero(native, ctx, code, t, group, n):
+    """Every score below -9e31, scale at its limit: the softmax of one key, not of none."""
+    check_one_key(native, ctx, code, t, group, n, 1e30)
