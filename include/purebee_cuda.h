@@ -528,7 +528,8 @@ int64_t pb_kv8_pool_bytes(const pb_kv8_config* c);
 /* The handle: geometry and frequencies; it serves any number of pools.  Its
  * calls run on ctx's stream, and so do graphs that hold them: pb_kv8_attn's
  * workspace is the context's.  Not while recording; free it after the graphs
- * that use it and before the context. */
+ * that use it and before the context (while recording too: its memory is then
+ * given back by a later create or free, or with the context). */
 int pb_kv8_create(pb_ctx* ctx, const pb_kv8_config* c, pb_kv8** out);
 int pb_kv8_free(pb_kv8* kv);
 /* Append: rows k_dev, v_dev [n_kv_heads * head_dim] of sequence s become its

@@ -161,6 +161,7 @@ extern "C" int pb_shutdown(pb_ctx* ctx) {
   if (ctx->stream) cudaStreamSynchronize(ctx->stream);
   if (ctx->scratch) cudaFree(ctx->scratch);
   if (ctx->gemm_scratch) cudaFree(ctx->gemm_scratch);
+  pb_kv8_collect(ctx);
   for (void* p : ctx->kv8_ws) cudaFree(p);
   if (ctx->d_err) cudaFree(ctx->d_err);
   if (ctx->stream) cudaStreamDestroy(ctx->stream);

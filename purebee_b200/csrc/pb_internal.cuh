@@ -36,6 +36,7 @@ struct pb_ctx {
   // before the context, so recorded graphs stay valid)
   std::vector<void*> kv8_ws;
   size_t kv8_ws_bytes = 0;
+  struct pb_kv8* kv8_freed = nullptr;  // handles that were freed while recording, whose memory is still to be given back
 };
 
 // Device layouts of a quantized matrix (payload and scales split apart, so
@@ -563,6 +564,7 @@ int pb_setup_gemm_kernels(void);
 int pb_setup_sample_kernels(void);
 int pb_setup_packed_kernels(void);
 int pb_setup_kv8_kernels(void);
+void pb_kv8_collect(pb_ctx* ctx);  // gives back the memory of kv8_freed; not while recording
 // Top-K sampling (pb_sample.cu): candidate keys needed, and the two launches.
 size_t pb_sample_cand_count(int V, int K);
 int pb_launch_sample(pb_ctx* ctx, const float* logits, int V, int K, double temperature, uint64_t seed,

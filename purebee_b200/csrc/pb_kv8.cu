@@ -1226,6 +1226,21 @@ extern "C" int64_t pb_kv8_pool_bytes(const pb_kv8_config* c) {
   return g.page_bytes * g.n_pages;
 }
 
+static bool kv8_recording(pb_ctx* ctx) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  return cudaStreamIsCapturing(ctx->stream, &st) != cudaSuccess || st != cudaStreamCaptureStatusNone;
+}
+
+void pb_kv8_collect(pb_ctx* ctx) {
+  if (!ctx->kv8_freed) return;
+  cudaStreamSynchronize(ctx->stream);
+  while (pb_kv8* kv = ctx->kv8_freed) {
+    ctx->kv8_freed = kv->next;
+    cudaFree(kv->freqs);
+    delete kv;
+  }
+}
+
 extern "C" int pb_kv8_create(pb_ctx* ctx, const pb_kv8_config* c, pb_kv8** out) {
   if (!ctx || !c || !out) return PB_ERR_ARG;
   *out = nullptr;
@@ -1237,9 +1252,8 @@ extern "C" int pb_kv8_create(pb_ctx* ctx, const pb_kv8_config* c, pb_kv8** out) 
     return pb_set_error(ctx, PB_ERR_ARG, "pb_kv8: bad rotary base or frequency scaling");
   for (int j = 0; j < g.rope_dim / 2; ++j) freqs[128 + j] = cos(freqs[j]), freqs[256 + j] = sin(freqs[j]);
   pb_device_scope dev(ctx->device);
-  cudaStreamCaptureStatus recording = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(ctx->stream, &recording) != cudaSuccess || recording != cudaStreamCaptureStatusNone)
-    return pb_set_error(ctx, PB_ERR_STATE, "pb_kv8_create: not while recording");
+  if (kv8_recording(ctx)) return pb_set_error(ctx, PB_ERR_STATE, "pb_kv8_create: not while recording");
+  pb_kv8_collect(ctx);
   pb_kv8* kv = new pb_kv8();
   kv->ctx = ctx;
   kv->g = g;
@@ -1271,10 +1285,11 @@ extern "C" int pb_kv8_create(pb_ctx* ctx, const pb_kv8_config* c, pb_kv8** out) 
 
 extern "C" int pb_kv8_free(pb_kv8* kv) {
   if (!kv) return PB_OK;
-  pb_device_scope dev(kv->ctx->device);
-  cudaStreamSynchronize(kv->ctx->stream);
-  cudaFree(kv->freqs);
-  delete kv;
+  pb_ctx* ctx = kv->ctx;
+  kv->next = ctx->kv8_freed;
+  ctx->kv8_freed = kv;
+  pb_device_scope dev(ctx->device);
+  if (!kv8_recording(ctx)) pb_kv8_collect(ctx);  // a wait would end the recording
   return PB_OK;
 }
 

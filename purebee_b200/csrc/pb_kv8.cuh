@@ -50,6 +50,7 @@ struct pb_kv8 {
   float* ws = nullptr;
   unsigned int* cnt = nullptr;
   int ctas = 0;  // of pb_kv8_attn
+  pb_kv8* next = nullptr;  // of the context's kv8_freed
 };
 
 // The calls' device is the context's, whichever is current on the thread.

@@ -642,3 +642,26 @@ def check_one_key(native, ctx, code, t, group, n, scale):
 def test_attention_all_scores_far_below_zero(native, ctx, code, t, group, n):
     """Every score below -9e31, scale at its limit: the softmax of one key, not of none."""
     check_one_key(native, ctx, code, t, group, n, 1e30)
+
+
+def test_handle_freed_while_recording(native, ctx):
+    """Freeing a handle (as the collector does with a dead one) leaves the recording as it was; nothing is lost."""
+    p = Pool(native, ctx, 0, 1, 32, 16, 1, 40)
+    p.append([20], [0], 1)
+    q, out = ctx.to_device(np.ones((1, 64), np.float32)), ctx.to_device(np.zeros((1, 64), np.float32))
+    st, le = p.ints([0, 1]), p.ints([20])
+    others = [native.KV8(ctx, 0, 1, 64, 16, 4, native.ROPE_HALF, 64) for _ in range(3)]
+
+    def step():
+        others[0].free()
+        p.kv.attn(p.pages.ptr, 0, q.ptr, 64, 2, st.ptr, le.ptr, p.table.ptr, p.ld, 1, 1, 0.1, out.ptr, 64)
+        others[1].free()
+
+    graph = ctx.capture(step)
+    graph.launch()
+    got = out.download().copy()
+    assert np.any(got != 0)
+    p.kv.attn(p.pages.ptr, 0, q.ptr, 64, 2, st.ptr, le.ptr, p.table.ptr, p.ld, 1, 1, 0.1, out.ptr, 64)
+    np.testing.assert_array_equal(out.download(), got)
+    others[2].free()
+    graph.free()
