@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(KA_THREADS, 4) k_kv8_append(kv8_geo g, kv8_app
   }
   if (kv_part)
     for (int i = tid; i < 2 * heads; i += KA_THREADS) amax[i] = 0;
-  const bool ok = pb_mbar_wait(&bar, 0, a.err);
+  const bool ok = kv8_copies(&bar, 0, a.err);
   if (!__syncthreads_and(ok && (block0 || !kv_part))) return;
   if (!kv_part) {
     auto out = [&](auto ot) {
@@ -341,7 +341,7 @@ k_kv8_read(kv8_geo g, const uint8_t* pages, const int* __restrict__ starts, cons
   }
   const int pos0 = un.blk * PB_KV8_BLOCK, kept = un.lo - pos0, end = un.hi - pos0;
   const int64_t row0 = (int64_t)un.row0 + pos0 - un.first;
-  if (!__syncthreads_and(pb_mbar_wait(&bar, 0, err))) return;
+  if (!__syncthreads_and(kv8_copies(&bar, 0, err))) return;
   auto decode = [&](const uint4& w4, float sc, float (&val)[16]) {
     const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
@@ -1121,8 +1121,9 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
       constexpr int T = KT_WARPS * 32, COLS = HD / 4, J = (TR * COLS + T - 1) / T;
       const int live = min(TR, pd.rows - pd.rho0);
       kt_sum acc[J];
+      bool ok = true;  // the same on every thread
       __threadfence();
-      for (int i0 = 0; i0 < pd.n_parts; i0 += HOLD) {
+      for (int i0 = 0; i0 < pd.n_parts && ok; i0 += HOLD) {
         const int n = min(HOLD, pd.n_parts - i0);
         if (warp == 0) {
           asm volatile("fence.proxy.async;" ::: "memory");
@@ -1132,7 +1133,7 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
             pb_bulk_g2s(kt_raw + (size_t)i * SLOT * 4,
                         a.ws + (size_t)(i0 + i == 0 ? pd.first_part : 2 * (pd.c0 + i0 + i)) * SLOT, SLOT * 4, &part_bar);
         }
-        pb_mbar_wait(&part_bar, part_phase, a.err);
+        ok = kv8_copies(&part_bar, part_phase, a.err);
         part_phase ^= 1;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
@@ -1141,12 +1142,12 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
             acc[j].add(reinterpret_cast<const float*>(kt_raw) + 4 * x, SLOT, TR * HD + x / COLS * 4 - 4 * x, n);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncthreads();
+        ok = __syncthreads_and(ok);
       }
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const int x = tid + T * j;
-        if (x < live * COLS) kt_finish(g, a, pd.row0, pd.rows, pd.len, pd.kvh, pd.rho0 + x / COLS, x % COLS * 4, acc[j]);
+        if (ok && x < live * COLS) kt_finish(g, a, pd.row0, pd.rows, pd.len, pd.kvh, pd.rho0 + x / COLS, x % COLS * 4, acc[j]);
       }
     }
     __syncthreads();  // `last` and the ring are free again

@@ -177,6 +177,14 @@ __device__ __forceinline__ float kv8_decode(uint32_t b, int code) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3)));
 }
 
+// A wait for this CTA's copies; where it gave up, once more, so that none is on
+// its way when the CTA ends.
+__device__ __forceinline__ bool kv8_copies(uint64_t* bar, uint32_t parity, int* err) {
+  if (pb_mbar_wait(bar, parity, err)) return true;
+  pb_mbar_wait(bar, parity, err);
+  return false;
+}
+
 // Packed rows: rows starts[s] .. starts[s + 1] - 1 belong to sequence s, row
 // starts[s] + i to its token first[s] + i.  The blocks that they touch are
 // numbered: sequence s has the numbers from starts[s] / 16 + 2 s on, of which it
