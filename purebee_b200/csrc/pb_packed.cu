@@ -347,7 +347,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
   constexpr uint32_t IDESC_QK = IDESC | ((uint32_t)(PA_KEYS >> 3) << 17);
   constexpr uint32_t IDESC_PV = IDESC | ((uint32_t)(HDP >> 3) << 17) | (1u << 16);
   extern __shared__ __align__(1024) unsigned char pa_raw[];
-  __shared__ uint64_t q_full, k_full[NS], k_empty[NS], v_full[NS], v_mask[NS], v_ready[NS], v_empty[NS], s_full[NT], s_free, p_full[NT][2], o_half[NT][2];
+  __shared__ uint64_t q_full, k_full[NS], k_empty[NS], v_full[NS], v_mask[NS], v_ready[NS], v_empty[NS], s_full[NT], s_free, p_full[NT][2], o_half[NT][2], drained;
   __shared__ uint32_t tmem_base;
   __shared__ int redo;
   __shared__ pa_place place;
@@ -376,6 +376,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
       }
     }
     pb_mbar_init(&s_free, 4);
+    pb_mbar_init(&drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -430,9 +431,11 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
 
   if (warp == 4 * NT) {
     if (lane == 0 && nt > 0) {  // TMA
+      int kn = 1, vn = 0;  // tiles asked for
       for (int j = 0; j < nt; ++j) {
         const int s = j % NS, use = j / NS;
         if (j >= NS && !pb_mbar_wait_sleep(&k_empty[s], (use - 1) & 1, a.err)) break;
+        kn = j + 1;
         if (j > 0) {
           pb_mbar_arrive_tx(&k_full[s], KT);
           for (int p = 0; p < PN; ++p)
@@ -440,10 +443,16 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         }
         if (j >= NS && !pb_mbar_wait_sleep(&v_empty[s], (use - 1) & 1, a.err)) break;
         uint64_t* full = j < whole ? &v_full[s] : &v_mask[s];  // a tile under a mask goes to the helpers first
+        vn = j + 1;
         pb_mbar_arrive_tx(full, KT);
         for (int p = 0; p < PN; ++p)
           pb_tma_load_3d(sV + s * KT + p * PA_PANEL, &map_v, p * 64, kvh, k0 + j * PA_KEYS, full);
       }
+      // whatever wait gave up, no tile is on its way when the CTA ends
+      pb_mbar_wait_sleep(&q_full, 0, a.err);
+      for (int j = max(0, kn - NS); j < kn; ++j) pb_mbar_wait_sleep(&k_full[j % NS], (j / NS) & 1, a.err);
+      for (int j = max(0, vn - NS); j < vn; ++j)
+        pb_mbar_wait_sleep(j < whole ? &v_full[j % NS] : &v_mask[j % NS], ((j < whole ? j : j - whole) / NS) & 1, a.err);
     }
   } else if (warp == 4 * NT + 1) {
     if (nt > 0) {  // MMA
@@ -502,6 +511,8 @@ k_attn_packed(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         pa_commit(&v_empty[s], lead);
         if (j + 1 < nt) pa_commit(&k_empty[s1], lead);
       }
+      pa_commit(&drained, lead);  // nor a product, which would find its TMEM given back
+      arrived(&drained, 0);
     }
   } else if (warp > 4 * NT + 1) {  // V tiles under a mask
     const int u = tid - 128 * NT - 64;
