@@ -85,7 +85,7 @@ __device__ __noinline__ void pa_row_plain(const pa_args& a, float* qs, int64_t r
   const int lane = threadIdx.x & 31, kvh = h / a.group;
   auto at = [&](const void* p, int64_t i) { return kv8_from16(static_cast<const uint16_t*>(p)[i], a.type); };
   __syncwarp();
-  for (int d = lane; d < a.hd; d += 32) qs[d] = at(a.q, row * a.ldq + h * a.hd + d) * a.scale;
+  for (int d = lane; d < a.hd; d += 32) qs[d] = at(a.q, row * a.ldq + h * a.hd + d);
   __syncwarp();
   float m = -INFINITY, l = 0.0f, acc[4] = {0, 0, 0, 0};
   for (int j0 = 0; j0 < see; j0 += 32) {
@@ -100,6 +100,7 @@ __device__ __noinline__ void pa_row_plain(const pa_args& a, float* qs, int64_t r
 #pragma unroll
         for (int i = 0; i < 8; ++i) s = fmaf(qs[d + i], x[i], s);
       }
+      s *= a.scale;  // after the sum, as on the tensor cores: q times the scale may pass f32's range
     }
     const float mn = fmaxf(m, pb_warp_max_f(s)), ref = mn == -INFINITY ? 0.0f : mn, f = expf(m - ref), p = expf(s - ref);
     m = mn;

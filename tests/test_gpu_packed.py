@@ -291,3 +291,20 @@ def test_packed_scores_of_any_size(native, ctx, t, hd, scale):
     # p = 1 for the one key, exactly; the others' sum to less than 450 2^(-64 * 3 * log2(e)); 1 / l and its product: two roundings
     tol = np.abs(want) * (R.EPS[t] / 2 * 1.01 + 2.0 ** -22)
     assert np.all(np.abs(got - want)[rows] <= tol[rows])
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_packed_large_queries_beside_values_not_finite(native, ctx, hd):
+    """Rows that are done again in the plain form, as a hidden value is not finite, with queries whose product with the scale
+    passes f32's range and whose scores do not."""
+    rng = np.random.default_rng(34)
+    q, (k, v) = rng.standard_normal((120, 2, hd)), rng.standard_normal((2, 120, 1, hd))
+    q = np.sign(q) * np.clip(np.abs(q), 0.25, 0.9) * 2.0 ** 127
+    k *= 2.0 ** -125
+    v[100] = np.inf
+    got, q, k, v = run(native, ctx, "bf16", q, k, v, [120], [120], True, 4.0, same=True)
+    w, mag, dots = R.attention(q[:100], k[:100], v[:100], 4.0)
+    tol = R.attention_tolerance(w, mag, dots, hd, 100, "bf16", R.EPS["bf16"] / 2)
+    assert np.isfinite(w).all() and not R.differs(got[:100], w, tol, "bf16").any()
+    # the others see the infinity: inf, or NaN where the f32 softmax has 0 beside it (scores lie hundreds apart)
+    assert not np.isfinite(got[100:]).any()
