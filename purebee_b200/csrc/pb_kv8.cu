@@ -763,8 +763,10 @@ __global__ void __launch_bounds__(KT_WARPS * 32, HD <= 128 ? 3 : HD <= 192 ? 2 :
       const float up = nan ? __int_as_float(0x7fc00000) : tiny ? 0.0f : 1.0f;
       if (a.scale < 0.0f) inv = -inv;  // the factor stays positive
       if (DIG) inv *= 127.0f;
-      qf[r] = fabsf(a.scale) * (up * kv8_pow2(max(-126, min(127, e)))) * (DIG ? 1.0f / (127.0f * 254.0f) : 1.0f / KT_QTOP);
-      if (e == 128) qf[r] *= 2.0f;  // 2^128 in two steps
+      // the small factor first, 2^128 in two steps; no infinity, which would make NaN of a score of 0
+      qf[r] = fabsf(a.scale) * (DIG ? 1.0f / (127.0f * 254.0f) : 1.0f / KT_QTOP) * (up * kv8_pow2(max(-126, min(127, e))));
+      if (e == 128) qf[r] *= 2.0f;
+      if (qf[r] > 3e38f) qf[r] = 3e38f;
       int low = 0;
 #pragma unroll
       for (int i = 0; i < NT; ++i)

@@ -665,3 +665,28 @@ def test_handle_freed_while_recording(native, ctx):
     np.testing.assert_array_equal(out.download(), got)
     others[2].free()
     graph.free()
+
+
+@pytest.mark.parametrize("code", [0, 1])
+@pytest.mark.parametrize("t,scale", [("f32", 4.0), ("bf16", 4.0), ("bf16", -4.0), ("f32", 1e30)])
+def test_attention_queries_near_the_largest_value(native, ctx, code, t, scale):
+    """Queries of 2^127, whose product with the scale passes f32's range, over keys of 2^-40 and of zeros."""
+    hd, n = 32, 90
+    p = Pool(native, ctx, code, 1, hd, 16, 1, n, seed=71)
+
+    def edit(kv):
+        kv[:, 0] = 0
+        if scale < 1e30:  # scores of 2^87 and more
+            kv[16:32, 0] = (np.arange(16) % 3 - 1.0)[:, None, None] * 2.0 ** -40
+            kv[40, 0], kv[60, 0] = 3 * 2.0 ** -40, -3 * 2.0 ** -40  # the only ones of their size
+    p.append([n], [0], 1, edit=edit)
+    got, _ = p.attn(np.full((2, 4, hd), 2.0 ** 127), [2], [n], t, scale)
+    v = p.ref[0].values(1, n)[:, 0]
+    if scale < 1e30:
+        want = v[40 if scale > 0 else 60] + np.zeros((2, 4, 1))
+        tol = np.abs(want) * (R.EPS[t] / 2 * 1.01 + 2.0 ** -20)
+    else:  # every score is 0: the mean of what a row sees
+        want = np.stack([v[:n - 1].mean(0), v.mean(0)])[:, None] + np.zeros((2, 4, 1))
+        mag = np.abs(v).mean(0)
+        tol = R.attention_tolerance(want, mag, np.zeros((2, 4)), hd, n, t, 2.0 ** -22)
+    assert np.all(np.abs(got - want) <= tol)
