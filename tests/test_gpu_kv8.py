@@ -690,3 +690,36 @@ def test_attention_queries_near_the_largest_value(native, ctx, code, t, scale):
         mag = np.abs(v).mean(0)
         tol = R.attention_tolerance(want, mag, np.zeros((2, 4)), hd, n, t, 2.0 ** -22)
     assert np.all(np.abs(got - want) <= tol)
+
+
+@pytest.mark.parametrize("code", [0, 1])
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("nkv,nh,page", [(1, 4, 16), (2, 16, 64)])
+def test_attention_ragged_heads_of_160(native, ctx, code, t, nkv, nh, page):
+    lens = [1, 17, 0, 300, 64]
+    p = Pool(native, ctx, code, nkv, 160, page, len(lens), 310, seed=80 + nh)
+    p.append(lens, [0] * 5, nkv)
+    p.check_attn(nh, [1, 1, 0, 1, 1], lens, t)
+    p.check_attn(nh, [1, 3, 0, 7, 2], lens, t)
+
+
+@pytest.mark.parametrize("code", [0, 1])
+def test_append_first_rows_that_belong_to_nobody(native, ctx, code):
+    """starts[0] above 0 and above a block: the rows before it are neither read into the cache nor written."""
+    p = Pool(native, ctx, code, 2, 64, 16, 2, 64, seed=51)
+    off, counts, w = 37, [20, 5], 8 * 64
+    x = p.rng.standard_normal((off + 25, w)).astype(np.float32)
+    x[:off] = np.nan
+    dx, st, past = ctx.to_device(x), p.ints([off, off + 20, off + 25]), p.ints([0, 0])
+    o = [ctx.to_device(np.full((off + 25, n * 64), 7, np.float32)) for n in (4, 2, 2)]
+    p.kv.append(p.pages.ptr, 0, dx.ptr, w, dx.ptr + 4 * 256, w, dx.ptr + 4 * 384, w, 4, st.ptr, past.ptr, p.table.ptr, p.ld, 2, off + 25,
+                0, o[0].ptr, 256, o[1].ptr, 128, o[2].ptr, 128)
+    for b, lo, hi in zip(o, (0, 256, 384), (256, 384, 512)):
+        got = b.download().reshape(off + 25, -1)
+        assert np.all(got[:off] == 7)
+        np.testing.assert_array_equal(got[off:], x[off:, lo:hi])
+    at = off
+    for s, n in enumerate(counts):
+        p.ref[s].append(0, *(x[at:at + n, a:a + 128].astype(np.float64).reshape(n, 2, 64) for a in (256, 384)))
+        at += n
+    p.check()

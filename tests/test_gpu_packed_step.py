@@ -105,3 +105,32 @@ def test_captured_serving_step(native, ctx):
         g.launch()
     for a, b, w in zip(outs[0], outs[1], (n * nh, n * nkv, n * nkv, n * nh, 2 * nh)):
         assert np.array_equal(a.download(np.uint16, w * hd), b.download(np.uint16, w * hd))
+
+
+def test_tensors_on_the_context_stream(native, ctx):
+    """torch's work on the context's stream, as a program with tensors has it: inputs refilled right before a call and outputs
+    used right behind it, without a wait of the host."""
+    torch = pytest.importorskip("torch")
+    n, nh, hd = 3000, 8, 128
+    with torch.cuda.stream(torch.cuda.ExternalStream(native.lib().pb_stream(ctx.h))):
+        gen = torch.Generator(device="cuda").manual_seed(3)
+        x = [torch.randn(n, nh * hd, generator=gen, device="cuda").to(torch.bfloat16) for _ in range(3)]
+        st = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+        q, out = torch.empty_like(x[0]), torch.empty_like(x[0])
+        got = []
+        for i in range(6):
+            q.zero_()
+            out.zero_()
+            torch.ones(1 << 26, device="cuda").add_(1)  # keeps the stream busy
+            q.copy_(x[0])
+            ctx.attn_packed(native.TYPE_BF16, q.data_ptr(), nh * hd, x[1].data_ptr(), nh * hd, x[2].data_ptr(), nh * hd, st.data_ptr(),
+                            st.data_ptr(), 1, n, n, nh, nh, hd, hd ** -0.5, 1, out.data_ptr(), nh * hd)
+            got.append(out.clone())
+        q.zero_()
+        assert all(torch.equal(g, got[0]) for g in got)
+        rows = [0, 1, 777, n - 1]
+        a, k, v = (y.double().view(n, nh, hd).cpu().numpy() for y in x)
+        for r in rows:
+            w, mag, dots = R.attention(a[r:r + 1], k[:r + 1], v[:r + 1], hd ** -0.5)
+            g = got[0].view(n, nh, hd)[r:r + 1].double().cpu().numpy()
+            assert not R.differs(g, w, R.attention_tolerance(w, mag, dots, hd, r + 1, "bf16", 2.0 ** -8), "bf16").any(), r
