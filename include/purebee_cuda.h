@@ -75,7 +75,10 @@ int pb_abi_version(void);
 int pb_set_timeout_ms(pb_ctx* ctx, int timeout_ms);
 /* purebee.js:193-197 SYNC(): wait for all queued work, bounded by the deadline. */
 int pb_sync(pb_ctx* ctx);
-/* The cudaStream_t the context enqueues on, as an opaque pointer. */
+/* The cudaStream_t the context enqueues on, as an opaque pointer.  It is a
+ * non-blocking stream: device arrays that another stream fills or uses are
+ * ordered with the context's calls by the caller (events on both sides, or
+ * that work on this stream too). */
 void* pb_stream(pb_ctx* ctx);
 /* Device error word: non-zero once a kernel recorded an error. */
 int pb_device_error(pb_ctx* ctx, int* code_out);
@@ -537,11 +540,13 @@ int pb_kv8_free(pb_kv8* kv);
  * position (in double, then rounded to f32), both are coded, and the scale of
  * a block that already holds tokens grows where the new ones need it (its
  * older codes are rounded once more under the larger scale).  A value that is
- * not finite, or above 2^66 in magnitude, makes its block and head read as NaN
- * until the block is begun anew.  Appending again at an earlier past_dev[s]
- * rolls the sequence back; a block then begun in its middle keeps its scale.
- * q_dev [n_heads * head_dim] (optional, with q_out_dev) is rotated into
- * q_out_dev; k_out_dev, v_out_dev (optional) get the rotated k and v without
+ * not finite, or above 127 (e4m3: 448) times 2^60 in magnitude, makes its
+ * block and head read as NaN until the block is begun anew: for all 16 tokens
+ * of the block, the ones before it too.  Appending again at an earlier
+ * past_dev[s] rolls the sequence back; a block then begun in its middle keeps
+ * its scale.  q_dev [n_heads * head_dim] (optional, with q_out_dev) is rotated
+ * into q_out_dev, in f32 with sines and cosines rounded to f32 (off by up to 5
+ * half steps of f32); k_out_dev, v_out_dev (optional) get the rotated k and v without
  * the coding, for pb_attn_packed.  Outputs are of type otype and may not
  * overlap the inputs or each other.  A page that two sequences share (or that
  * is twice in a table) is read by both, but appended to by none. */
@@ -561,8 +566,15 @@ int pb_kv8_read(pb_kv8* kv, const void* pages_dev, const int* starts_dev, const 
  * being cached with them; each sees the tokens up to its own, kv head h /
  * (n_heads / n_kv_heads) for head h.  out = sum_j softmax_j(scale q.k_j) v_j
  * with f32 sums; a row that sees no token (lens_dev[s] less than its rows)
- * gets zeros, and a query whose values all lie below 2^-118 counts as zeros.  q_dev and out_dev [n_rows][n_heads * head_dim] are of one type
- * and do not overlap. */
+ * gets zeros, and a query whose values all lie below 2^-118 counts as zeros.
+ * What is held in fewer bits than f32: for f32 rows, queries and probabilities
+ * to 22 bits; for f16 and bf16 rows, probabilities to f16 (half a step, 2^-11),
+ * queries as they are (f16 after a power of two), but over int8 codes where at
+ * least half of a row's values lie within 1/32 of the power of two above its
+ * largest: there to 2^-16 of that power.  A probability times its block's V
+ * scale is held no finer than 2^-31 of the row's largest such product.
+ * q_dev and out_dev [n_rows][n_heads * head_dim] are of one type and do not
+ * overlap. */
 int pb_kv8_attn(pb_kv8* kv, const void* pages_dev, int type, const void* q_dev, int ldq, int n_heads,
                 const int* starts_dev, const int* lens_dev, const int* table_dev, int ld_table, int n_seqs, int n_rows,
                 double scale, void* out_dev, int ldo);
@@ -571,10 +583,12 @@ int pb_kv8_attn(pb_kv8* kv, const void* pages_dev, int type, const void* q_dev, 
  * v_dev [k_rows][n_kv * head_dim] (llama-streaming.js:422-464 for one sequence
  * in f32; pb_attn_cached).  causal = 1: the queries are the sequence's last
  * tokens, query i of nq sees keys up to nk - nq + i; 0: all of them.  A query
- * that sees no key gets zeros.  f16 or bf16 rows and output, f32 scores and
- * sums, the probabilities rounded to the rows' type; head_dim a multiple of 8,
- * up to 128.  q_starts_dev and k_starts_dev may be one array; out_dev overlaps
- * no input. */
+ * that sees no key gets zeros, and no value that a query does not see touches
+ * it, not one that is not finite either.  f16 or bf16 rows and output, f32
+ * scores and sums, the probabilities rounded to the rows' type (the sum takes
+ * them unrounded; a part of the exponentials is off by up to 7.5e-5 for bf16,
+ * 2.6e-6 for f16); head_dim a multiple of 8, up to 128.  q_starts_dev and
+ * k_starts_dev may be one array; out_dev overlaps no input. */
 int pb_attn_packed(pb_ctx* ctx, int type, const void* q_dev, int ldq, const void* k_dev, int ldk, const void* v_dev,
                    int ldv, const int* q_starts_dev, const int* k_starts_dev, int n_seqs, int q_rows, int k_rows,
                    int n_heads, int n_kv, int head_dim, double scale, int causal, void* out_dev, int ldo);

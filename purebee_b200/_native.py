@@ -346,7 +346,7 @@ class Context:
 
     def attn_packed(self, type_, q, ldq, k, ldk, v, ldv, q_starts, k_starts, n_seqs, q_rows, k_rows, n_heads, n_kv,
                     head_dim, scale, causal, out, ldo) -> None:
-        """Attention of whole packed prompts (pb_attn_packed); arrays are device addresses."""
+        """Attention of whole packed prompts (pb_attn_packed); arrays are device addresses, ordered as KV8's."""
         self._check(lib().pb_attn_packed(self.h, type_, q, ldq, k, ldk, v, ldv, q_starts, k_starts, n_seqs, q_rows,
                                          k_rows, n_heads, n_kv, head_dim, scale, causal, out, ldo))
 
@@ -388,7 +388,9 @@ class QMat:
 class KV8:
     """A paged 8-bit KV cache's geometry, rotation and workspace (pb_kv8); it serves any number of page pools.
 
-    Arrays are device addresses (a DeviceBuffer's ptr, a tensor's data_ptr()).
+    Arrays are device addresses (a DeviceBuffer's ptr, a tensor's data_ptr()).  Calls run on the context's stream, which
+    is not ordered with torch's: have the tensors' work on it too (torch.cuda.ExternalStream(lib().pb_stream(ctx.h)) as
+    the current stream), or let each stream wait for the other's event, before a call and behind it.
     """
 
     def __init__(self, ctx: Context, code: int, n_kv_heads: int, head_dim: int, page_size: int, n_pages: int,

@@ -24,8 +24,8 @@ struct kv8_append_args {
 };
 
 constexpr int KA_THREADS = 128;
-// bytes of a CTA's rows (16 tokens of its heads, k in f32 too): 4 CTAs fit on an SM.  9776 prompt rows and the read back: 97.5
-// us; 121 with 24 KB, 113 with 48, 103 with 64; 108 with 256 threads
+// bytes of a CTA's rows (16 tokens of its heads, k in f32 too): 4 CTAs fit on an SM.  9776 prompt rows and the read back (99.5
+// us by now), in one sweep: 97.5 us; 121 with 24 KB, 113 with 48, 103 with 64; 108 with 256 threads
 constexpr int KA_ROWS = 32 << 10;
 
 template <int TYPE>
@@ -134,8 +134,8 @@ __device__ __forceinline__ void ka_rotate(const unsigned char* rows, int stride,
 // order.  Many small CTAs keep about 128 KB a SM in flight.  k is rotated in
 // double, so that its codes are those of the exact values; q in f32.
 // 9 prompts of 37 to 3001 f32 rows (32 heads over 8 of 128 values, half of them
-// rotated; 9776 rows, 340 MB): about 79 us, 4.3 TB/s; a step of 96
-// bf16 rows 13 us and of 4 f32 rows 9.5 us with the read that follows, the
+// rotated; 9776 rows, 340 MB): 82 us, 4.2 TB/s; a step of 96 bf16 rows 10.5 us,
+// 16.3 with the read that follows, and of 4 f32 rows 9.8 with it, recorded: the
 // latency of one block's chain (starts, rows, rotation, codes).
 template <int TYPE, int ROPE>
 __global__ void __launch_bounds__(KA_THREADS, 4) k_kv8_append(kv8_geo g, kv8_append_args a, int y_kv) {
@@ -458,12 +458,14 @@ static kr_kernel kr_kernel_of(int code, int otype) {
 // product and its rounded form, which m1 is, may lie whole numbers apart: it is
 // rounded for all keys there.
 //
-// Measured (8 kv heads of 128 values): 2 x 131072 tokens, int8, 64 f16 heads: 93
-// us, 5.4 TB/s of codes; 64 ragged sequences up to 9000 tokens, e4m3, 32 bf16
-// heads: 105 to 108 us, 5.5 TB/s; memory bound.  12 sequences of 1 to 5 drafted
-// tokens, int8, f16: 75 us, 3.9 TB/s, bound by the work on two rows a thread and
-// by the second pass over the codes where 20 rows need two tiles.  One sequence
-// of 640 tokens, f32: 8.5 us, latency.
+// Measured (8 kv heads of 128 values): 2 x 131072 tokens, int8, 64 f16 heads: 95
+// to 97 us, 5.1 to 5.3 TB/s of codes; 64 ragged sequences up to 9000 tokens, e4m3,
+// 32 bf16 heads: 108 to 111 us, 5.3 to 5.4 TB/s; memory bound.  12 sequences of 1 to
+// 5 drafted tokens, int8, f16: 75 to 80 us, 3.6 to 3.9 TB/s, bound by the work on two
+// rows a thread and by the second pass over the codes where 20 rows need two tiles.
+// One sequence of 640 tokens, f32: 8.4 us, latency.  Heads of 160 to 256 values, 8 or
+// 4 warps a SM: 5.5 to 6.0 TB/s on the long ones; on the ragged batch 5.8 up to 192
+// values, 5.0 at 224 and 5.2 at 256.
 constexpr int KT_WARPS = 4;
 constexpr int KT_COST = 32;
 __host__ __device__ constexpr int kt_stages(int hd) { return hd <= 64 ? 4 : 2; }

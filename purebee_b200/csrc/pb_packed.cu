@@ -38,11 +38,12 @@
 // A part of the exponentials run on the FMA pipe (pa_ex2_poly).
 //
 // Bound by the chain of a tile (S, maximum, exponentials, P) and its issue slots,
-// not by the products: 8192 causal rows, 32 heads over 8, in bf16 take 455 us with
-// 128 values a head (1.21 PFLOP/s; about 540 us, 1.02 PFLOP/s, where the power
-// limit holds the clock at 1.45 GHz) and 425 us with 64 (the exponentials alone
-// 250 us); 24 ragged f16 prompts of 65 to 1024 rows with 64 values 162 us, of
-// which a third is the CTAs' starts and ends.
+// not by the products: 8192 causal rows, 32 heads over 8, in bf16 take 483 us with
+// 128 values a head where calls lie 50 ms apart (1.14 PFLOP/s; clock at 1965 MHz) and
+// 530 to 540 us, 1.03 PFLOP/s, one after the other, where the power limit holds the
+// clock at 1640 MHz; with 64 values 428 us (the exponentials alone 250 us); 24 ragged
+// f16 prompts of 65 to 1024 rows with 64 values 163 us, of which a third is the CTAs'
+// starts and ends.
 #include <math.h>
 
 #include "pb_kv8.cuh"
